@@ -342,7 +342,7 @@ def _fork(k, v, table, lens, refs, parents, grow):
     before = need.cumsum(0) - need
     free = count == 0
     n_free = free.sum()
-    granted = wants & (before + need <= n_free)
+    granted = wants & ((need == 0) | (before + need <= n_free))
     order = torch.sort(torch.where(free, 0, 1), stable=True).indices  # free pages, ascending
     take = lambda n: order[n.clamp(max=pages - 1)]  # noqa: E731
     copies &= granted
