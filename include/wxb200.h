@@ -31,6 +31,7 @@ extern "C" {
 
 /* bits of the device error word (wx_device_error) */
 #define WX_DEVERR_TIMEOUT 1 /* a bounded wait inside a kernel gave up */
+#define WX_DEVERR_PAGE 2    /* a cache kernel met a page, length or parent out of range */
 
 /* element types */
 #define WX_DTYPE_BF16 0
@@ -193,6 +194,125 @@ int wx_gemm_f32(const float* A, const float* B, const float* bias, float* C, int
 int wx_attention(const void* q, const void* k, const void* v, void* o, int64_t B, int64_t H,
                  int64_t T, int64_t hd, int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo,
                  float scale, void* stream);
+
+/* ------------------------------------------------------------ decoder: the cache */
+
+/* A paged key-value cache for a text decoder on the encoder's features. It has
+ * no counterpart in the reference, whose decoder is openai-whisper's on the CPU
+ * (serve/npu_stt_server.py:347-353).
+ *
+ * The cache is two pools, K and V, alike in layout: element (page, token, head,
+ * d) of a layer is at page * page_stride + token * tok_stride + head *
+ * head_stride + d (strides in elements; token-major and head-major pages are
+ * both a choice of strides). Rows of head_dim elements are contiguous and
+ * 16-byte aligned. table (n_seqs x width, int32) names a sequence's pages in
+ * order, -1 past its last; lens (int32) its tokens, of which page i holds
+ * [i * page_size, (i + 1) * page_size). refs (n_pages, int32) counts the table
+ * entries that name a page; 0 is free. A page that several sequences share
+ * stands at the same place in their rows, as wx_kv_fork leaves it. All of these
+ * are device memory, and no call reads them on the host.
+ *
+ * A page, length or parent out of range in those arrays is left out (its tokens
+ * are not written, or not attended to) and recorded as WX_DEVERR_PAGE, which
+ * wx_device_error reports and clears. dtype is WX_DTYPE_BF16 or WX_DTYPE_F32. */
+
+/* Writes new tokens: row t < counts[i] (all n_tokens if counts is NULL) of
+ * sequence i's k and v goes to position lens[i] - counts[i] + t, that is, lens
+ * counts the new tokens already (wx_kv_fork's lens_out and grown_out). k and v
+ * are (n_seqs, n_tokens, n_heads, head_dim) with the given strides, head_dim
+ * contiguous; column slices of one QKV buffer are fine. */
+int wx_kv_append(const void* k, const void* v, int64_t src_seq_stride, int64_t src_tok_stride,
+                 int64_t src_head_stride, void* k_cache, void* v_cache, int64_t page_stride,
+                 int64_t tok_stride, int64_t head_stride, const int32_t* table, int64_t ld_table,
+                 const int32_t* lens, const int32_t* counts, int64_t n_seqs, int64_t n_tokens,
+                 int64_t n_heads, int64_t head_dim, int64_t n_pages, int64_t page_size,
+                 int dtype, void* stream);
+
+/* Bytes of device workspace (16-byte aligned) for wx_kv_fork and wx_kv_compact;
+ * its contents need no preparation and mean nothing after the call. */
+int64_t wx_kv_workspace(int64_t n_seqs, int64_t n_pages);
+
+/* One step of every sequence's pages, for all n_layers layers of a cache:
+ * sequence i goes on as sequence parents[i] was (-1: it starts empty, and what
+ * it held is given back; parents NULL: each goes on as itself), with room for
+ * grow[i] more tokens (grow NULL: none). So beams are reordered and copied,
+ * finished sequences freed and new ones started, and each step's tokens given
+ * their pages, in one call.
+ *   - Pages are shared with the parent, not copied, but for a partly filled last
+ *     page that another sequence shares too and this one is about to write in:
+ *     its filled tokens are copied to a page of its own. The longest of the
+ *     sharers, the first among equals, keeps the page.
+ *   - Pages are taken from the free ones in ascending order, for sequences in
+ *     ascending order. A sequence whose pages the pool does not hold, or whose
+ *     tokens the table's width does not, is not grown and stays as it is.
+ * table_out (n_seqs x width, -1 past the last page), lens_out (with the tokens
+ * granted), refs_out, grown_out (tokens granted; may be NULL) and status_out[2]
+ * (pages left free, pages short) are written; none of them may be an input. The
+ * k and v pools are written only in pages that were free. */
+int wx_kv_fork(void* k_cache, void* v_cache, int64_t n_layers, int64_t layer_stride,
+               int64_t page_stride, int64_t tok_stride, int64_t head_stride, int64_t n_heads,
+               int64_t head_dim, int64_t n_pages, int64_t page_size, int dtype,
+               const int32_t* table, const int32_t* lens, const int32_t* refs,
+               const int32_t* parents, const int32_t* grow, int64_t n_seqs, int64_t width,
+               int32_t* table_out, int32_t* lens_out, int32_t* refs_out, int32_t* grown_out,
+               int32_t* status_out, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Moves the pages in use to the front of the pool, in all layers: with n_used
+ * pages in use, those numbered n_used or more go to the free ones below, both in
+ * ascending order, and the table is renumbered (table_out may be table).
+ * status_out[2]: n_used and the pages moved. */
+int wx_kv_compact(void* k_cache, void* v_cache, int64_t n_layers, int64_t layer_stride,
+                  int64_t page_stride, int64_t tok_stride, int64_t head_stride, int64_t n_heads,
+                  int64_t head_dim, int64_t n_pages, int64_t page_size, int dtype,
+                  const int32_t* table, const int32_t* refs, int64_t n_seqs, int64_t width,
+                  int32_t* table_out, int32_t* refs_out, int32_t* status_out, void* workspace,
+                  int64_t workspace_bytes, void* stream);
+
+/* Attention of one new token a sequence over the cache: query row g < group of
+ * head h < n_heads (the cache's heads) of sequence i attends to the keys
+ * starts[i] <= j < lens[i] (starts NULL: from 0),
+ *   o = sum_j softmax_j(scale * q . k_j) v_j,  lse = log sum_j e^(scale * q . k_j).
+ * group is the query heads that share a key-value head, or the beams that share
+ * a clip's keys, or both: q and out are (n_seqs, n_heads, group, head_dim) with
+ * any strides, head_dim contiguous. lse (n_seqs, n_heads, group) fp32 or NULL. A
+ * row without keys (or with all scores -inf) gives o = 0 and lse = -inf. q, the
+ * cache and out are of one dtype; head_dim 64 or 128; sums in fp32, bf16
+ * probabilities rounded once before the product with V.
+ * max_len: an upper bound of lens, at most ld_table * page_size (longer
+ * sequences are cut there, WX_DEVERR_PAGE): it shapes the launch. The workspace
+ * (wx_paged_attention_workspace bytes, 16-byte aligned; may be 0) needs no
+ * preparation; calls that may overlap each need their own. */
+int64_t wx_paged_attention_workspace(int64_t n_seqs, int64_t n_heads, int64_t group,
+                                     int64_t head_dim, int64_t max_len);
+int wx_paged_attention(const void* q, int64_t q_seq_stride, int64_t q_head_stride,
+                       int64_t q_group_stride, const void* k_cache, const void* v_cache,
+                       int64_t page_stride, int64_t tok_stride, int64_t head_stride,
+                       const int32_t* table, int64_t ld_table, const int32_t* lens,
+                       const int32_t* starts, void* out, int64_t o_seq_stride,
+                       int64_t o_head_stride, int64_t o_group_stride, float* lse, int64_t n_seqs,
+                       int64_t n_heads, int64_t group, int64_t head_dim, int64_t n_pages,
+                       int64_t page_size, int64_t max_len, float scale, int dtype,
+                       void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------ decoder: scores */
+
+/* Scores of tokens under rows of logits (rows x vocab, bf16 or fp32, row stride
+ * ld), with z = logits / temperature:
+ *   logprob[r] = z[tokens[r]] - log sum e^z        (average log probability, the
+ *       no-speech probability, language detection; openai-whisper computes them
+ *       in torch after the reference's encoder)
+ *   entropy[r] = the entropy of softmax(z), in nats
+ *   top_logprob, top_index (rows x top_k): the largest logits' log probabilities
+ *       and tokens, best first, equal logits by the lowest token.
+ * A token below 0 is none and has logprob 0; one at or past vocab has -inf.
+ * Logits of -inf are masked tokens (probability 0). A row that is all -inf has
+ * logprob and top_logprob -inf and entropy 0; one that holds NaN or +inf has NaN
+ * scores, and its order puts NaN above +inf. top_k <= 32 and <= vocab.
+ * logprob (with tokens) and entropy may be NULL; so may the top outputs if
+ * top_k is 0. */
+int wx_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ld,
+                      const int64_t* tokens, int64_t top_k, float temperature, float* logprob,
+                      float* entropy, float* top_logprob, int32_t* top_index, void* stream);
 
 /* ------------------------------------------------------------ no allocation */
 

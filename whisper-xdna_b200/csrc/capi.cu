@@ -6,6 +6,7 @@
 #include <vector>
 
 #include "common.cuh"
+#include "kvcache.cuh"
 #include "plans.cuh"
 #include "wxb200_internal.h"
 
@@ -116,7 +117,10 @@ int wx_device_error(int* flags, int clear) {
   WX_CUDA_TRY(cudaDeviceSynchronize());
   WX_CUDA_TRY(cudaMemcpy(flags, w, sizeof(int), cudaMemcpyDeviceToHost));
   if (clear) WX_CUDA_TRY(cudaMemset(w, 0, sizeof(int)));
-  // the allocation-free entry point records into a word of its own
+  // the cache's kernels and the allocation-free entry point record into words
+  // of their own
+  WX_TRY(wx::kv_take_error(flags, clear != 0));
+  WX_TRY(wx::paged_attention_take_error(flags, clear != 0));
   return wx::noalloc_take_error(flags, clear != 0);
 }
 

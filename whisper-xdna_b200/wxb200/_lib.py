@@ -16,6 +16,7 @@ WX_ERR_UNSUPPORTED = -3
 WX_ERR_DEVICE = -4
 WX_ERR_NOMEM = -5
 WX_DEVERR_TIMEOUT = 1
+WX_DEVERR_PAGE = 2
 WX_DTYPE_BF16 = 0
 WX_DTYPE_F32 = 1
 WX_ROUND_TRUNC = 0
@@ -54,6 +55,18 @@ SIGNATURES = {
                         _p, _p]),
     "wx_gemm_f32": (_i, [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _p]),
     "wx_attention": (_i, [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f, _p]),
+    "wx_kv_append": (_i, [_p, _p, _i64, _i64, _i64, _p, _p, _i64, _i64, _i64, _p, _i64, _p, _p,
+                          _i64, _i64, _i64, _i64, _i64, _i64, _i, _p]),
+    "wx_kv_workspace": (_i64, [_i64, _i64]),
+    "wx_kv_fork": (_i, [_p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i, _p, _p,
+                        _p, _p, _p, _i64, _i64, _p, _p, _p, _p, _p, _p, _i64, _p]),
+    "wx_kv_compact": (_i, [_p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i, _p,
+                           _p, _i64, _i64, _p, _p, _p, _p, _i64, _p]),
+    "wx_paged_attention_workspace": (_i64, [_i64, _i64, _i64, _i64, _i64]),
+    "wx_paged_attention": (_i, [_p, _i64, _i64, _i64, _p, _p, _i64, _i64, _i64, _p, _i64, _p, _p,
+                                _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64,
+                                _i64, _f, _i, _p, _i64, _p]),
+    "wx_token_logprobs": (_i, [_p, _i, _i64, _i64, _i64, _p, _i64, _f, _p, _p, _p, _p, _p]),
     "wx_mlp_bf16_noalloc": (_i, [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i, _p]),
     "wx_encoder_create": (_i, [_c.POINTER(_p), _i, _i, _i, _i, _i, _i, _i, _i]),
     "wx_encoder_destroy": (_i, [_p]),

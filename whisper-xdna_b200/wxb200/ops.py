@@ -7,6 +7,7 @@ buffers are accepted as they are -- the banded outputs of src/rowops.py:80-88
 and the per-head slices of a fused QKV buffer.
 """
 import ctypes
+import functools
 
 import torch
 
@@ -274,3 +275,225 @@ def log_mel(audio, n_mels=80, out=None):
     L.check(L.lib().wx_log_mel(_ptr(a), B, n, a.stride(0) if B > 1 else n, int(n_mels),
                                _ptr(out), _stream()))
     return out[0] if squeeze else out
+
+
+# ---------------------------------------------------------------- decoder operators
+# Paged key-value cache: pools of shape (pages, page, heads, head_dim) for a
+# layer, (layers, pages, page, heads, head_dim) for a whole cache, any strides
+# with head_dim contiguous (a head-major pool is passed transposed). The page
+# table is (n_seqs, width) int32, -1 past a sequence's last page.
+
+_KV_DTYPES = {torch.bfloat16: L.WX_DTYPE_BF16, torch.float32: L.WX_DTYPE_F32}
+
+
+def _on(dev, name, t, dtype, shape=None):
+    """t on device `dev`, of dtype, contiguous, of the shape given."""
+    if not isinstance(t, torch.Tensor) or t.get_device() != dev:
+        raise ValueError(f"{name} must be a CUDA tensor on the cache's device")
+    if t.dtype != dtype or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous {dtype}, got {t.dtype}")
+    if shape is not None and t.shape != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    return t.data_ptr()
+
+
+def _pools(k_cache, v_cache, dim):
+    """Checks a cache's two pools; returns (device, dtype code, shape, strides)."""
+    for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise ValueError(f"{name} must be a CUDA tensor")
+        if t.dim() != dim:
+            raise ValueError(f"{name} must have {dim} dimensions, got {t.dim()}")
+    dtype, shape, strides = k_cache.dtype, k_cache.shape, k_cache.stride()
+    if dtype not in _KV_DTYPES:
+        raise ValueError(f"cache dtype {dtype} not in {list(_KV_DTYPES)}")
+    if v_cache.dtype != dtype or v_cache.shape != shape or v_cache.stride() != strides:
+        raise ValueError("k_cache and v_cache must have the same dtype, shape and strides")
+    if strides[-1] != 1:
+        raise ValueError("the cache's head_dim must be contiguous")
+    dev = k_cache.get_device()
+    if v_cache.get_device() != dev or dev != torch.cuda.current_device():
+        raise ValueError("the cache must be on the current CUDA device")
+    return dev, _KV_DTYPES[dtype], shape, strides
+
+
+def _table(dev, table, lens, name="lens"):
+    n, width = table.shape if isinstance(table, torch.Tensor) and table.dim() == 2 else (0, 0)
+    if width == 0:
+        raise ValueError("table must be a (n_seqs, width) tensor")
+    return (n, width, _on(dev, "table", table, torch.int32),
+            _on(dev, name, lens, torch.int32, (n,)) if lens is not None else None)
+
+
+def _raw_stream(dev):
+    return torch.cuda.current_stream(dev).cuda_stream
+
+
+@functools.lru_cache(maxsize=1024)
+def _attend_space(n_seqs, n_heads, group, head_dim, max_len):
+    n = L.lib().wx_paged_attention_workspace(n_seqs, n_heads, group, head_dim, max_len)
+    if n < 0:
+        L.check(n)
+    return n
+
+
+def paged_attention(q, k_cache, v_cache, table, lens, scale=None, starts=None, max_len=None,
+                    out=None, return_lse=False):
+    """Attention of one new token a sequence over a paged cache: query row g of
+    cache head h of sequence i attends to the keys starts[i] <= j < lens[i].
+
+    q: (n_seqs, heads, head_dim), its heads in groups that share a cache head, or
+    (n_seqs, cache heads, group, head_dim) with any strides -- for beams over one
+    clip's keys, x.view(clips, beams, heads, hd).transpose(1, 2). scale: default
+    head_dim ** -0.5. max_len: an upper bound of lens, by default what the table
+    holds; a close one makes a better split. Returns out (q's shape and strides,
+    q's dtype), with return_lse also log sum_j e^(scale q.k_j), fp32, q's shape
+    without head_dim. A row without keys gives 0 and -inf."""
+    dev, dt, shape, st = _pools(k_cache, v_cache, 4)
+    n_pages, page, n_heads, hd = shape
+    n, width, table_p, lens_p = _table(dev, table, lens)
+    if not isinstance(q, torch.Tensor) or q.get_device() != dev or q.dtype != k_cache.dtype:
+        raise ValueError("q must be a CUDA tensor on the cache's device, of its dtype")
+    qs = q.shape
+    if q.dim() == 3:
+        if qs[1] % n_heads:
+            raise ValueError(f"{qs[1]} query heads are no multiple of {n_heads} cache heads")
+        group = qs[1] // n_heads
+    elif q.dim() == 4:
+        group = qs[2]
+        if qs[1] != n_heads:
+            raise ValueError(f"q has {qs[1]} cache heads, the cache {n_heads}")
+    else:
+        raise ValueError("q must have 3 or 4 dimensions")
+    if qs[0] != n or qs[-1] != hd or q.stride(-1) != 1:
+        raise ValueError(f"q of shape {tuple(qs)} does not fit {n} sequences of head_dim {hd} "
+                         "(contiguous)")
+    if out is None:
+        out = torch.empty_like(q)
+    elif (out.shape != qs or out.dtype != q.dtype or out.get_device() != dev
+          or out.stride(-1) != 1):
+        raise ValueError("out must be like q, with a contiguous head_dim")
+    lse = torch.empty(qs[:-1], dtype=torch.float32, device=q.device) if return_lse else None
+    if group == 0:
+        raise ValueError("q has no rows")
+    if max_len is None:
+        max_len = width * page
+    starts_p = _on(dev, "starts", starts, torch.int32, (n,)) if starts is not None else None
+    space = _attend_space(n, n_heads, group, hd, max_len)
+    ws = torch.empty(space, dtype=torch.uint8, device=q.device) if space else None
+    qt, ot = q.stride(), out.stride()
+    if q.dim() == 3:
+        qt, ot = (qt[0], qt[1] * group, qt[1]), (ot[0], ot[1] * group, ot[1])
+    L.check(L.lib().wx_paged_attention(
+        q.data_ptr(), qt[0], qt[1], qt[2], k_cache.data_ptr(), v_cache.data_ptr(), st[0], st[1],
+        st[2], table_p, width, lens_p, starts_p, out.data_ptr(), ot[0], ot[1], ot[2],
+        lse.data_ptr() if return_lse else None, n, n_heads, group, hd, n_pages, page, max_len,
+        hd ** -0.5 if scale is None else float(scale), dt, ws.data_ptr() if space else None,
+        space, _raw_stream(dev)))
+    return (out, lse) if return_lse else out
+
+
+def kv_append(k, v, k_cache, v_cache, table, lens, counts=None):
+    """Writes new tokens into a layer's cache, in place: k, v (n_seqs, tokens,
+    heads, head_dim) or, for one token each, (n_seqs, heads, head_dim), of the
+    cache's dtype; row t < counts[i] (all if None) of sequence i goes to position
+    lens[i] - counts[i] + t."""
+    dev, dt, shape, st = _pools(k_cache, v_cache, 4)
+    n_pages, page, n_heads, hd = shape
+    n, width, table_p, lens_p = _table(dev, table, lens)
+    for t, name in ((k, "k"), (v, "v")):
+        if not isinstance(t, torch.Tensor) or t.get_device() != dev or t.dtype != k_cache.dtype:
+            raise ValueError(f"{name} must be a CUDA tensor on the cache's device, of its dtype")
+    if k.shape != v.shape or k.stride() != v.stride():
+        raise ValueError("k and v must have the same shape and strides")
+    ks, kt = k.shape, k.stride()
+    if k.dim() == 3:
+        ks, kt = (ks[0], 1, ks[1], ks[2]), (kt[0], 0, kt[1], kt[2])
+    if len(ks) != 4 or ks[0] != n or ks[2] != n_heads or ks[3] != hd or kt[3] != 1:
+        raise ValueError(f"k of shape {tuple(k.shape)} does not fit {n} sequences of {n_heads} "
+                         f"heads of {hd} (contiguous)")
+    counts_p = _on(dev, "counts", counts, torch.int32, (n,)) if counts is not None else None
+    L.check(L.lib().wx_kv_append(
+        k.data_ptr(), v.data_ptr(), kt[0], kt[1], kt[2], k_cache.data_ptr(), v_cache.data_ptr(),
+        st[0], st[1], st[2], table_p, width, lens_p, counts_p, n, ks[1], n_heads, hd, n_pages,
+        page, dt, _raw_stream(dev)))
+
+
+@functools.lru_cache(maxsize=1024)
+def _plan_space(n_seqs, n_pages):
+    return L.lib().wx_kv_workspace(n_seqs, n_pages)
+
+
+def kv_fork(k_cache, v_cache, table, lens, refs, parents=None, grow=None):
+    """One step of every sequence's pages in all layers of a cache: sequence i
+    goes on as parents[i] was (-1: it starts empty; None: as itself), with room
+    for grow[i] more tokens (None: no tokens). Shared pages about to be written
+    are copied, pages nobody names are freed, new ones are the lowest free ones.
+    Nothing waits for the GPU.
+
+    Returns new int32 tensors (table, lens, refs, grown, status): lens counts the
+    tokens granted (grown), status is (pages left free, pages short). A sequence
+    whose pages the pool does not hold is not grown."""
+    dev, dt, shape, st = _pools(k_cache, v_cache, 5)
+    n_layers, n_pages, page, n_heads, hd = shape
+    n, width, table_p, lens_p = _table(dev, table, lens)
+    refs_p = _on(dev, "refs", refs, torch.int32, (n_pages,))
+    parents_p = _on(dev, "parents", parents, torch.int32, (n,)) if parents is not None else None
+    grow_p = _on(dev, "grow", grow, torch.int32, (n,)) if grow is not None else None
+    space = _plan_space(n, n_pages)
+    i32 = dict(dtype=torch.int32, device=table.device)
+    new = (torch.empty((n, width), **i32), torch.empty(n, **i32), torch.empty(n_pages, **i32),
+           torch.empty(n, **i32), torch.empty(2, **i32))
+    ws = torch.empty(space, dtype=torch.uint8, device=table.device)
+    L.check(L.lib().wx_kv_fork(
+        k_cache.data_ptr(), v_cache.data_ptr(), n_layers, st[0], st[1], st[2], st[3], n_heads, hd,
+        n_pages, page, dt, table_p, lens_p, refs_p, parents_p, grow_p, n, width,
+        *(t.data_ptr() for t in new), ws.data_ptr(), space, _raw_stream(dev)))
+    return new
+
+
+def kv_compact(k_cache, v_cache, table, refs):
+    """Moves the pages in use to the front of the pool in all layers of a cache,
+    with the fewest moves. Returns new int32 tensors (table, refs, status), status
+    being (pages in use, pages moved)."""
+    dev, dt, shape, st = _pools(k_cache, v_cache, 5)
+    n_layers, n_pages, page, n_heads, hd = shape
+    n, width, table_p, _ = _table(dev, table, None)
+    refs_p = _on(dev, "refs", refs, torch.int32, (n_pages,))
+    space = _plan_space(n, n_pages)
+    i32 = dict(dtype=torch.int32, device=table.device)
+    new = (torch.empty((n, width), **i32), torch.empty(n_pages, **i32), torch.empty(2, **i32))
+    ws = torch.empty(space, dtype=torch.uint8, device=table.device)
+    L.check(L.lib().wx_kv_compact(
+        k_cache.data_ptr(), v_cache.data_ptr(), n_layers, st[0], st[1], st[2], st[3], n_heads, hd,
+        n_pages, page, dt, table_p, refs_p, n, width, *(t.data_ptr() for t in new),
+        ws.data_ptr(), space, _raw_stream(dev)))
+    return new
+
+
+def token_logprobs(logits, tokens, top_k=0, temperature=1.0):
+    """Scores under rows of logits ((rows, vocab), bf16 or fp32, masked tokens
+    -inf), with z = logits / temperature: returns (logprob, entropy, top_logprob,
+    top_index) -- log softmax(z)[tokens] (tokens (rows,) int64; a token below 0 is
+    none and scores 0) and the entropy in nats, fp32 (rows,), and the top_k (<= 32)
+    likeliest tokens with their log probabilities, (rows, top_k) fp32 and int32,
+    equal logits by the lowest token. A row that is all -inf scores -inf, with
+    entropy 0."""
+    _mat(logits, "logits", (torch.bfloat16, torch.float32))
+    rows, vocab = logits.shape
+    dev = logits.get_device()
+    if dev != torch.cuda.current_device():
+        raise ValueError("logits must be on the current CUDA device")
+    tokens_p = _on(dev, "tokens", tokens, torch.int64, (rows,))
+    if not 0 <= top_k <= min(32, vocab):
+        raise ValueError(f"top_k {top_k} not in [0, min(32, vocabulary {vocab})]")
+    f32 = dict(dtype=torch.float32, device=logits.device)
+    logprob, entropy = torch.empty(rows, **f32), torch.empty(rows, **f32)
+    top = torch.empty((rows, top_k), **f32)
+    index = torch.empty((rows, top_k), dtype=torch.int32, device=logits.device)
+    L.check(L.lib().wx_token_logprobs(
+        logits.data_ptr(), _KV_DTYPES[logits.dtype], rows, vocab, logits.stride(0), tokens_p,
+        top_k, float(temperature), logprob.data_ptr(), entropy.data_ptr(),
+        top.data_ptr() if top_k else None, index.data_ptr() if top_k else None,
+        _raw_stream(dev)))
+    return logprob, entropy, top, index
