@@ -276,14 +276,14 @@ int wx_kv_compact(void* k_cache, void* v_cache, int64_t n_layers, int64_t layer_
  * a clip's keys, or both: q and out are (n_seqs, n_heads, group, head_dim) with
  * any strides, head_dim contiguous. lse (n_seqs, n_heads, group) fp32 or NULL. A
  * row without keys (or with all scores -inf) gives o = 0 and lse = -inf. q, the
- * cache and out are of one dtype; head_dim 64 or 128; sums in fp32, bf16
- * probabilities rounded once before the product with V.
+ * cache and out are of one dtype; head_dim 64 or 128; sums in fp32, the
+ * result rounded once.
  * max_len: an upper bound of lens, at most ld_table * page_size (longer
  * sequences are cut there, WX_DEVERR_PAGE): it shapes the launch. The workspace
  * (wx_paged_attention_workspace bytes, 16-byte aligned; may be 0) needs no
  * preparation; calls that may overlap each need their own. */
 int64_t wx_paged_attention_workspace(int64_t n_seqs, int64_t n_heads, int64_t group,
-                                     int64_t head_dim, int64_t max_len);
+                                     int64_t head_dim, int64_t max_len, int dtype);
 int wx_paged_attention(const void* q, int64_t q_seq_stride, int64_t q_head_stride,
                        int64_t q_group_stride, const void* k_cache, const void* v_cache,
                        int64_t page_stride, int64_t tok_stride, int64_t head_stride,

@@ -7,7 +7,7 @@ import math
 import torch
 
 U32 = 2.0 ** -24     # unit roundoff of fp32
-U16 = 2.0 ** -9      # of bf16
+U16 = 2.0 ** -9      # half of bf16's
 
 
 def attend64(q, k_cache, v_cache, table, lens, scale, starts=None):
@@ -16,8 +16,8 @@ def attend64(q, k_cache, v_cache, table, lens, scale, starts=None):
     Bounds, with a_j = scale sum |q||k_j| and A = max_j a_j: a score carries at
     most (hd + 3) u A; a weight twice that, the exponential's 2^-22 and the
     exponent's rounding (|s_j - m| <= 2 A, in log2 units: 2 A 2^-23); a sum of n
-    terms n u. For bf16 each weight is rounded once more (2^-9) before the
-    product with V, and the result once."""
+    terms n u. A bf16 result is rounded once, 2^-8 |o|, which is at most 2^-9
+    sum p|v| + 2^-9 |o|; its weights have to be kept to more bits than bf16's."""
     q, dev = q.double(), q.device
     S, H, G, hd = q.shape
     page = k_cache.shape[1]

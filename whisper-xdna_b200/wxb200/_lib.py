@@ -62,7 +62,7 @@ SIGNATURES = {
                         _p, _p, _p, _i64, _i64, _p, _p, _p, _p, _p, _p, _i64, _p]),
     "wx_kv_compact": (_i, [_p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i, _p,
                            _p, _i64, _i64, _p, _p, _p, _p, _i64, _p]),
-    "wx_paged_attention_workspace": (_i64, [_i64, _i64, _i64, _i64, _i64]),
+    "wx_paged_attention_workspace": (_i64, [_i64, _i64, _i64, _i64, _i64, _i]),
     "wx_paged_attention": (_i, [_p, _i64, _i64, _i64, _p, _p, _i64, _i64, _i64, _p, _i64, _p, _p,
                                 _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64,
                                 _i64, _f, _i, _p, _i64, _p]),

@@ -330,8 +330,8 @@ def _raw_stream(dev):
 
 
 @functools.lru_cache(maxsize=1024)
-def _attend_space(n_seqs, n_heads, group, head_dim, max_len):
-    n = L.lib().wx_paged_attention_workspace(n_seqs, n_heads, group, head_dim, max_len)
+def _attend_space(n_seqs, n_heads, group, head_dim, max_len, dtype):
+    n = L.lib().wx_paged_attention_workspace(n_seqs, n_heads, group, head_dim, max_len, dtype)
     if n < 0:
         L.check(n)
     return n
@@ -379,7 +379,7 @@ def paged_attention(q, k_cache, v_cache, table, lens, scale=None, starts=None, m
     if max_len is None:
         max_len = width * page
     starts_p = _on(dev, "starts", starts, torch.int32, (n,)) if starts is not None else None
-    space = _attend_space(n, n_heads, group, hd, max_len)
+    space = _attend_space(n, n_heads, group, hd, max_len, dt)
     ws = torch.empty(space, dtype=torch.uint8, device=q.device) if space else None
     qt, ot = q.stride(), out.stride()
     if q.dim() == 3:
