@@ -17,7 +17,8 @@ namespace wx {
 constexpr int kScoreThreads = 256, kScoreWarps = kScoreThreads / 32;
 constexpr int kScoreMaxCtas = 8;    // CTAs (one cluster) on a row
 constexpr int kScoreMaxTop = 32;    // one lane each
-constexpr int kScoreVecs = 4;       // 16-byte loads in flight a thread
+constexpr int kScoreVecs = 2;       // 16-byte vectors of a thread's step
+constexpr int kScoreStages = 5;     // steps in flight
 
 struct ScoreArgs {
   const void* logits;
@@ -48,8 +49,8 @@ __device__ __forceinline__ float order_value(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
 // (value, lowest index first) as one number; 0 is below every entry
-__device__ __forceinline__ uint64_t entry(float x, int64_t index) {
-  return ((uint64_t)order_key(x) << 32) | (uint32_t)~(uint32_t)index;
+__device__ __forceinline__ uint64_t entry(float x, uint32_t index) {
+  return ((uint64_t)order_key(x) << 32) | ~index;
 }
 
 // The running sums of one thread or of a part of a row.
@@ -71,11 +72,25 @@ __device__ __forceinline__ Sums join(Sums a, Sums b, float c) {
   return {m, a.s * fa + b.s * fb, ua + ub};
 }
 
-// The warp's best top_k entries, one a lane, best first.
+// The warp's best entries, one a lane, best first; the first top_k count.
 struct TopList {
   uint64_t mine = 0;   // this lane's entry
   uint64_t last = 0;   // entry top_k - 1: what a newcomer has to beat
 
+  // each lane's x, sorted: the list's first contents
+  __device__ __forceinline__ void start(uint64_t x, int top_k) {
+    const int lane = lane_id();
+#pragma unroll
+    for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+      for (int j = k >> 1; j > 0; j >>= 1) {
+        const uint64_t y = __shfl_xor_sync(0xffffffffu, x, j);
+        const bool keep_max = ((lane & k) == 0) == ((lane & j) == 0);
+        x = keep_max == (x > y) ? x : y;
+      }
+    mine = x;
+    last = __shfl_sync(0xffffffffu, mine, top_k - 1);
+  }
   // x (the same in all lanes) takes its place
   __device__ __forceinline__ void insert(uint64_t x, int top_k) {
     const int lane = lane_id();
@@ -146,117 +161,185 @@ __device__ __forceinline__ void score_cluster_sync() {
                ::: "memory");
 }
 
-// best top_k of n sorted lists of top_k entries each (n <= 32), list l read by
-// lane l through at(i): every round the best head leaves its list
-template <typename At>
-__device__ __forceinline__ uint64_t merge_lists(int n, int top_k, At at) {
-  const int lane = lane_id();
-  int i = 0;
-  uint64_t head = lane < n ? at(0) : 0, mine = 0;
-  for (int r = 0; r < top_k; r++) {
-    uint64_t best = head;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const uint64_t x = __shfl_xor_sync(0xffffffffu, best, o);
-      best = x > best ? x : best;
-    }
-    if (lane == r) mine = best;
-    if (head == best && best != 0) {   // entries are distinct: one lane's head
-      i++;
-      head = i < top_k ? at(i) : 0;
-    }
+// The first top_k of n entries (n <= kScoreThreads, distinct but for 0) in order:
+// every thread counts the entries above its own. Called by the whole CTA.
+__device__ __forceinline__ void rank_entries(const uint64_t* from, int n, int top_k,
+                                             uint64_t* to) {
+  const int t = threadIdx.x;
+  if (t < n) {
+    const uint64_t x = from[t];
+    int rank = 0;
+#pragma unroll 8
+    for (int i = 0; i < n; i++) rank += from[i] > x;
+    if (x && rank < top_k) to[rank] = x;
   }
-  return mine;
 }
 
 // Row blockIdx.y by a cluster of gridDim.x CTAs, each a contiguous part of it.
-// A thread takes kScoreVecs 16-byte vectors a step, rescales its sums when its
-// own maximum moves, and the warp looks for newcomers to its list of top_k only
-// when some lane holds a logit that is not below the list's last. The parts are
-// joined in shared memory, then over the cluster's: always in the same order.
+//
+// A thread takes kScoreVecs 16-byte vectors a step, copied kScoreStages - 1 steps
+// ahead into shared memory, and rescales its sums when its
+// own maximum moves. A warp's list starts as its lanes' first maxima, sorted. From
+// then on a vector is looked into only if its largest logit passes the list's last
+// one and is not below `bound`, the CTA's top_k-th logit so far, which the lists
+// are joined for after steps 1, 4, 16 and so on: about top_k logits of a row pass
+// each time the logits seen have grown fourfold. The parts are joined in shared
+// memory, then over the cluster's, the lists by counting ranks.
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kScoreThreads) token_score_kernel(const ScoreArgs a) {
   constexpr int N = Lanes<T>::N;
   __shared__ Sums sums[kScoreWarps];
   __shared__ Sums cta_sums;
-  __shared__ uint64_t lists[kScoreWarps][kScoreMaxTop];
-  __shared__ uint64_t cta_list[kScoreMaxTop];
+  __shared__ uint64_t lists[kScoreThreads];   // kScoreWarps or kScoreMaxCtas lists
+  __shared__ uint64_t cta_list[kScoreMaxTop], best[kScoreMaxTop];
+  __shared__ uint4 ring[kScoreStages][kScoreVecs][kScoreThreads];
+  static_assert(kScoreMaxCtas * kScoreMaxTop <= kScoreThreads, "");
   const int lane = lane_id(), w = warp_id();
   const int rank = blockIdx.x, n_ctas = gridDim.x;
   const int64_t row = blockIdx.y;
   const T* x = static_cast<const T*>(a.logits) + row * a.ld;
   const float c = 1.4426950408889634f * a.inv_t;
-
-  Sums acc = {-INFINITY, 0.0f, 0.0f};
-  TopList top;
-  float seen = -INFINITY;   // the list's last logit
-
-  // one step: `count` valid logits of v in this lane, index of the first
-  auto step = [&](auto& v, auto index_of, auto valid) {
-    constexpr int K = sizeof(v) / sizeof(float);
-    float vm = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < K; i++) vm = max_nan(vm, v[i]);
-    if (!(vm <= acc.m)) {
-      const Sums fresh = {vm, 0.0f, 0.0f};
-      const float d = (acc.m - vm) * c, f = acc.s == 0.0f ? 0.0f : exp2f(d);
-      acc.u = f == 0.0f ? 0.0f : (acc.u + acc.s * d) * f;
-      acc.s *= f;
-      acc.m = fresh.m;
-    }
-    const float m = acc.m == -INFINITY ? 0.0f : acc.m;
-#pragma unroll
-    for (int i = 0; i < K; i++) {
-      // the bound keeps d finite where e is 0 (a masked logit)
-      const float d = max_nan((v[i] - m) * c, -1e4f);
-      const float e = fast_exp2(d);
-      acc.s += e;
-      acc.u = fmaf(e, d, acc.u);
-    }
-    if (TOP && __any_sync(0xffffffffu, !(vm < seen))) {
-#pragma unroll
-      for (int i = 0; i < K; i++) top.offer(valid(i) ? entry(v[i], index_of(i)) : 0, a.top_k);
-      seen = top.last ? order_value((uint32_t)(top.last >> 32)) : -INFINITY;
-    }
-  };
-
-  // head and tail: the elements before the first and past the last whole vector
-  const int64_t lead = min(a.vocab, (int64_t)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T));
-  const int64_t n_vec = (a.vocab - lead) / N;
-  if (rank == 0 && w == 0) {
-    float v[1] = {lane < lead ? Lanes<T>::one(x + lane) : -INFINITY};
-    step(v, [&](int) { return (int64_t)lane; }, [&](int) { return lane < lead; });
+  if (TOP) {
+    if (threadIdx.x < kScoreMaxTop) cta_list[threadIdx.x] = best[threadIdx.x] = 0;
+    __syncthreads();
   }
+
+  float m = -INFINITY;
+  float2 s2 = {0.0f, 0.0f}, u2 = {0.0f, 0.0f};
+  auto raise = [&](float vm) {   // the maximum becomes vm
+    const float d = (m - vm) * c;
+    const float f = m == -INFINITY ? 0.0f : exp2f(d);
+    // s d f -> 0 as f -> 0: what is too small to count adds nothing
+    u2.x = f == 0.0f ? 0.0f : (u2.x + s2.x * d) * f;
+    u2.y = f == 0.0f ? 0.0f : (u2.y + s2.y * d) * f;
+    s2.x *= f;
+    s2.y *= f;
+    m = vm;
+  };
+  TopList top;
+  float floor = -INFINITY;   // the CTA's top_k-th logit so far
+
+  // the elements before the first and past the last whole vector: `edges`, at the
+  // end, by the first CTA's first warp
+  const int lead = (int)min(a.vocab, (int64_t)(((16 - ((uintptr_t)x & 15)) & 15) / sizeof(T)));
+  const int n_vec = (int)((a.vocab - lead) / N);
   const uint4* xv = reinterpret_cast<const uint4*>(x + lead);
-  const int64_t v0 = n_vec * rank / n_ctas, v1 = n_vec * (rank + 1) / n_ctas;
-  // a warp's vectors of a step lie side by side, so its indices only grow
-  for (int64_t i = v0 + w * 32 * kScoreVecs; i < v1; i += kScoreThreads * kScoreVecs) {
-    float v[kScoreVecs * N];
+  const int v0 = (int)((int64_t)n_vec * rank / n_ctas);
+  const int v1 = (int)((int64_t)n_vec * (rank + 1) / n_ctas);
+  constexpr int kStep = kScoreThreads * kScoreVecs;
+  const int n_steps = (v1 - v0 + kStep - 1) / kStep;
+  // each thread copies its vectors ahead into slots that only it reads
+  auto fetch = [&](int it) {
+    const int i = v0 + it * kStep + w * 32 * kScoreVecs + lane;
+#pragma unroll
+    for (int j = 0; j < kScoreVecs; j++)
+      if (i + j * 32 < v1)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                         smem_u32(&ring[it % kScoreStages][j][threadIdx.x])),
+                     "l"(xv + i + j * 32)
+                     : "memory");
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int it = 0; it < kScoreStages - 1; it++) fetch(it);
+  int refresh = 1;
+  for (int it = 0; it < n_steps; it++) {
+    // a warp's vectors of a step lie side by side, so its indices only grow
+    const int i = v0 + it * kStep + w * 32 * kScoreVecs + lane;
+    fetch(it + kScoreStages - 1);
+    asm volatile("cp.async.wait_group %0;" ::"n"(kScoreStages - 1) : "memory");
+    float v[kScoreVecs][N], vmax[kScoreVecs];
 #pragma unroll
     for (int j = 0; j < kScoreVecs; j++) {
-      const int64_t k = i + j * 32 + lane;
-      float p[N];
-      if (k < v1) {
-        Lanes<T>::unpack(__ldg(xv + k), p);
-      } else {
+      Lanes<T>::unpack(ring[it % kScoreStages][j][threadIdx.x], v[j]);
+      if (i + j * 32 >= v1) {
 #pragma unroll
-        for (int e = 0; e < N; e++) p[e] = -INFINITY;
+        for (int e = 0; e < N; e++) v[j][e] = -INFINITY;
       }
+      vmax[j] = v[j][0];
 #pragma unroll
-      for (int e = 0; e < N; e++) v[j * N + e] = p[e];
+      for (int e = 1; e < N; e++) vmax[j] = max_nan(vmax[j], v[j][e]);
     }
-    step(
-        v,
-        [&](int e) { return lead + (i + (e / N) * 32 + lane) * N + e % N; },
-        [&](int e) { return i + (e / N) * 32 + lane < v1; });
+    float vm = vmax[0];
+#pragma unroll
+    for (int j = 1; j < kScoreVecs; j++) vm = max_nan(vm, vmax[j]);
+    if (!(vm <= m)) raise(vm);
+    const float ref = m == -INFINITY ? 0.0f : m;
+    const float2 neg = {-ref, -ref}, c2 = {c, c};
+#pragma unroll
+    for (int j = 0; j < kScoreVecs; j++)
+#pragma unroll
+      for (int e = 0; e < N; e += 2) {
+        float2 d = __fmul2_rn(__fadd2_rn(make_float2(v[j][e], v[j][e + 1]), neg), c2);
+        // the bound keeps d finite where its power is 0 (a masked logit)
+        d.x = max_nan(d.x, -1e4f);
+        d.y = max_nan(d.y, -1e4f);
+        const float2 p = {fast_exp2(d.x), fast_exp2(d.y)};
+        s2 = __fadd2_rn(s2, p);
+        u2 = __ffma2_rn(p, d, u2);
+      }
+    if (!TOP) continue;
+
+    const uint32_t at0 = (uint32_t)lead + (uint32_t)i * N;   // vector j: + 32 N j
+    uint32_t own = 0xFFFFFFFFu;   // the lane's entry of the list's start
+    if (it == 0) {
+      bool got = false;
+#pragma unroll
+      for (int j = 0; j < kScoreVecs; j++)
+#pragma unroll
+        for (int e = 0; e < N; e++)
+          if (!got && (v[j][e] == vm || v[j][e] != v[j][e])) {
+            got = true;
+            own = at0 + 32 * N * j + e;
+          }
+      top.start(i < v1 ? entry(vm, own) : 0, a.top_k);
+    }
+    // later steps have higher indices, so a logit equal to the list's last comes
+    // after it; within the first step, and against other warps, it may come before
+    const bool first = it == 0;
+    float seen = top.last ? order_value((uint32_t)(top.last >> 32)) : -INFINITY;
+    auto passes = [&](float y) {
+      return (!(y <= seen) || (y == seen && (first || top.last == 0))) && !(y < floor);
+    };
+    if (__any_sync(0xffffffffu, passes(vm))) {
+#pragma unroll
+      for (int j = 0; j < kScoreVecs; j++) {
+        if (!__any_sync(0xffffffffu, passes(vmax[j]))) continue;
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+          const uint32_t at = at0 + 32 * N * j + e;
+          const bool in = i + j * 32 < v1 && at != own && passes(v[j][e]);
+          if (__any_sync(0xffffffffu, in)) {
+            top.offer(in ? entry(v[j][e], at) : 0, a.top_k);
+            seen = top.last ? order_value((uint32_t)(top.last >> 32)) : -INFINITY;
+          }
+        }
+      }
+    }
+    if (it + 1 == refresh && it + 1 < n_steps) {
+      refresh *= 4;
+      if (lane < a.top_k) lists[w * a.top_k + lane] = top.mine;
+      __syncthreads();
+      rank_entries(lists, kScoreWarps * a.top_k, a.top_k, best);
+      __syncthreads();
+      const uint64_t kth = best[a.top_k - 1];
+      floor = kth ? order_value((uint32_t)(kth >> 32)) : -INFINITY;
+    }
   }
-  if (rank == n_ctas - 1 && w == kScoreWarps - 1) {
-    const int64_t k = lead + n_vec * N + lane;
-    float v[1] = {k < a.vocab ? Lanes<T>::one(x + k) : -INFINITY};
-    step(v, [&](int) { return k; }, [&](int) { return k < a.vocab; });
+  if (rank == 0 && w == 0) {
+    const int tail = lead + n_vec * N + lane - 16;
+    const bool is = lane < 16 ? lane < lead : tail < a.vocab;
+    const int at = lane < 16 ? lane : tail;
+    const float y = is ? Lanes<T>::one(x + at) : -INFINITY;
+    if (!(y <= m)) raise(y);
+    const float d = max_nan((y - (m == -INFINITY ? 0.0f : m)) * c, -1e4f), p = fast_exp2(d);
+    s2.x += p;
+    u2.x = fmaf(p, d, u2.x);
+    if (TOP) top.offer(is ? entry(y, (uint32_t)at) : 0, a.top_k);
   }
 
   // the warp's, the CTA's, the row's
+  Sums acc = {m, s2.x + s2.y, u2.x + u2.y};
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     Sums b = {__shfl_xor_sync(0xffffffffu, acc.m, o), __shfl_xor_sync(0xffffffffu, acc.s, o),
@@ -264,29 +347,34 @@ __global__ void __launch_bounds__(kScoreThreads) token_score_kernel(const ScoreA
     acc = join(acc, b, c);
   }
   if (lane == 0) sums[w] = acc;
-  if (TOP) lists[w][lane] = top.mine;
+  if (TOP && lane < a.top_k) lists[w * a.top_k + lane] = top.mine;
   __syncthreads();
   if (w == 0) {
     for (int i = 1; i < kScoreWarps; i++) acc = join(acc, sums[i], c);
     if (lane == 0) cta_sums = acc;
-    if (TOP)
-      cta_list[lane] = merge_lists(kScoreWarps, a.top_k, [&](int i) { return lists[lane][i]; });
   }
+  if (TOP) rank_entries(lists, kScoreWarps * a.top_k, a.top_k, n_ctas > 1 ? cta_list : best);
   if (n_ctas > 1) {
     score_cluster_sync();
-    if (rank == 0 && w == 0) {
-      for (int r = 1; r < n_ctas; r++) {
-        const uint32_t p = cluster_peer(&cta_sums, r);
-        acc = join(acc, Sums{peer_f32(p), peer_f32(p + 4), peer_f32(p + 8)}, c);
-      }
+    if (rank == 0) {
+      if (w == 0)
+        for (int r = 1; r < n_ctas; r++) {
+          const uint32_t p = cluster_peer(&cta_sums, r);
+          acc = join(acc, Sums{peer_f32(p), peer_f32(p + 4), peer_f32(p + 8)}, c);
+        }
       if (TOP) {
-        const uint32_t p = cluster_peer(cta_list, lane < n_ctas ? lane : 0);
-        top.mine = merge_lists(n_ctas, a.top_k, [&](int i) { return peer_u64(p + 8 * i); });
+        if (threadIdx.x < n_ctas * a.top_k) {
+          const int r = threadIdx.x / a.top_k;
+          lists[threadIdx.x] =
+              peer_u64(cluster_peer(cta_list + (threadIdx.x - r * a.top_k), r));
+        }
+        __syncthreads();
+        rank_entries(lists, n_ctas * a.top_k, a.top_k, best);
       }
     }
     score_cluster_sync();   // a CTA's shared memory outlives its readers
-  } else if (TOP && w == 0) {
-    top.mine = cta_list[lane];
+  } else if (TOP) {
+    __syncthreads();
   }
   if (rank != 0 || w != 0) return;
 
@@ -302,8 +390,9 @@ __global__ void __launch_bounds__(kScoreThreads) token_score_kernel(const ScoreA
       a.entropy[row] = empty ? 0.0f : log_s - 0.6931471805599453f * (acc.u / acc.s);
   }
   if (TOP && lane < a.top_k) {
-    a.top_logprob[row * a.top_k + lane] = logprob(order_value((uint32_t)(top.mine >> 32)));
-    a.top_index[row * a.top_k + lane] = (int32_t)~(uint32_t)top.mine;
+    const uint64_t e = best[lane];
+    a.top_logprob[row * a.top_k + lane] = logprob(order_value((uint32_t)(e >> 32)));
+    a.top_index[row * a.top_k + lane] = (int32_t)~(uint32_t)e;
   }
 }
 
