@@ -37,6 +37,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 
 // Order of logits as unsigned integers: NaN above +inf, -0 equal to +0.
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -58,18 +63,28 @@ struct Sums {
   float m, s, u;   // maximum logit, sum 2^d, sum 2^d d (d in log2 units)
 };
 
-// a joined with b; c = log2(e) / T
-__device__ __forceinline__ Sums join(Sums a, Sums b, float c) {
-  // a part without weight (nothing in it, or all -inf) leaves the other as it is
-  if (b.s == 0.0f) return {max_nan(a.m, b.m), a.s, a.u};
-  if (a.s == 0.0f) return {max_nan(a.m, b.m), b.s, b.u};
-  const float m = max_nan(a.m, b.m);
-  const float da = (a.m - m) * c, db = (b.m - m) * c;
-  const float fa = exp2f(da), fb = exp2f(db);
-  // f d -> 0 as f -> 0: a part too small to count adds nothing
-  const float ua = fa == 0.0f ? 0.0f : (a.u + a.s * da) * fa;
-  const float ub = fb == 0.0f ? 0.0f : (b.u + b.s * db) * fb;
-  return {m, a.s * fa + b.s * fb, ua + ub};
+// x with the reference m in place of its own, m at least x.m; c = log2(e) / T
+__device__ __forceinline__ Sums refer(Sums x, float m, float c) {
+  // a part without weight (nothing in it, or all -inf) keeps none
+  if (x.s == 0.0f) return {m, 0.0f, 0.0f};
+  const float d = (x.m - m) * c, f = fast_exp2(d);
+  // s d f -> 0 as f -> 0: what is too small to count adds nothing
+  return {m, x.s * f, f == 0.0f ? 0.0f : (x.u + x.s * d) * f};
+}
+// The lanes' parts joined, a fixed tree: every lane gets the whole.
+__device__ __forceinline__ float warp_max(float m) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+  return m;
+}
+__device__ __forceinline__ Sums join_lanes(Sums x, float c) {
+  x = refer(x, warp_max(x.m), c);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    x.s += __shfl_xor_sync(0xffffffffu, x.s, o);
+    x.u += __shfl_xor_sync(0xffffffffu, x.u, o);
+  }
+  return x;
 }
 
 // The warp's best entries, one a lane, best first; the first top_k count.
@@ -190,10 +205,10 @@ __global__ void __launch_bounds__(kScoreThreads) token_score_kernel(const ScoreA
   constexpr int N = Lanes<T>::N;
   __shared__ Sums sums[kScoreWarps];
   __shared__ Sums cta_sums;
-  __shared__ uint64_t lists[kScoreThreads];   // kScoreWarps or kScoreMaxCtas lists
+  __shared__ uint64_t lists[kScoreThreads];   // of kScoreWarps warps or kScoreMaxCtas CTAs
   __shared__ uint64_t cta_list[kScoreMaxTop], best[kScoreMaxTop];
   __shared__ uint4 ring[kScoreStages][kScoreVecs][kScoreThreads];
-  static_assert(kScoreMaxCtas * kScoreMaxTop <= kScoreThreads, "");
+  static_assert(kScoreMaxCtas * kScoreMaxTop <= kScoreThreads && kScoreMaxCtas <= 32, "");
   const int lane = lane_id(), w = warp_id();
   const int rank = blockIdx.x, n_ctas = gridDim.x;
   const int64_t row = blockIdx.y;
@@ -206,18 +221,28 @@ __global__ void __launch_bounds__(kScoreThreads) token_score_kernel(const ScoreA
 
   float m = -INFINITY;
   float2 s2 = {0.0f, 0.0f}, u2 = {0.0f, 0.0f};
-  auto raise = [&](float vm) {   // the maximum becomes vm
-    const float d = (m - vm) * c;
-    const float f = m == -INFINITY ? 0.0f : exp2f(d);
-    // s d f -> 0 as f -> 0: what is too small to count adds nothing
-    u2.x = f == 0.0f ? 0.0f : (u2.x + s2.x * d) * f;
-    u2.y = f == 0.0f ? 0.0f : (u2.y + s2.y * d) * f;
-    s2.x *= f;
-    s2.y *= f;
-    m = vm;
+  // the warp's maximum becomes that of vm where it is larger: seldom after a few
+  // steps, since the warp's lanes share it
+  auto raise = [&](float vm) {
+    if (!__any_sync(0xffffffffu, !(vm <= m))) return;
+    const float to = max_nan(m, warp_max(vm));
+    const Sums x = refer({m, s2.x, u2.x}, to, c), y = refer({m, s2.y, u2.y}, to, c);
+    s2 = {x.s, y.s};
+    u2 = {x.u, y.u};
+    m = to;
   };
   TopList top;
-  float floor = -INFINITY;   // the CTA's top_k-th logit so far
+  // a logit is looked at unless it is <= pass: the list's last one, since later
+  // steps have higher indices and an equal logit comes after, or just below the
+  // CTA's top_k-th so far, since against other warps it may come before
+  float pass = -INFINITY;
+  uint32_t floor = 0;        // order_key of the CTA's top_k-th logit so far
+  auto set_pass = [&](bool equals) {
+    const uint32_t own = (uint32_t)(top.last >> 32);
+    uint32_t k = max(own - (equals && own ? 1 : 0), floor ? floor - 1 : 0);
+    if (k == 0x7FFFFFFFu) k--;   // -0, which compares equal to the 0 above it
+    pass = k ? order_value(k) : __uint_as_float(0x7FC00000u);   // NaN: everything passes
+  };
 
   // the elements before the first and past the last whole vector: `edges`, at the
   // end, by the first CTA's first warp
@@ -250,20 +275,26 @@ __global__ void __launch_bounds__(kScoreThreads) token_score_kernel(const ScoreA
     asm volatile("cp.async.wait_group %0;" ::"n"(kScoreStages - 1) : "memory");
     float v[kScoreVecs][N], vmax[kScoreVecs];
 #pragma unroll
-    for (int j = 0; j < kScoreVecs; j++) {
+    for (int j = 0; j < kScoreVecs; j++)
       Lanes<T>::unpack(ring[it % kScoreStages][j][threadIdx.x], v[j]);
-      if (i + j * 32 >= v1) {
+    if (it + 1 == n_steps) {
 #pragma unroll
-        for (int e = 0; e < N; e++) v[j][e] = -INFINITY;
-      }
-      vmax[j] = v[j][0];
+      for (int j = 0; j < kScoreVecs; j++)
+        if (i + j * 32 >= v1) {
 #pragma unroll
-      for (int e = 1; e < N; e++) vmax[j] = max_nan(vmax[j], v[j][e]);
+          for (int e = 0; e < N; e++) v[j][e] = -INFINITY;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < kScoreVecs; j++) {
+      vmax[j] = max_nan(v[j][0], v[j][1]);
+#pragma unroll
+      for (int e = 2; e < N; e += 2) vmax[j] = max_nan(vmax[j], v[j][e], v[j][e + 1]);
     }
     float vm = vmax[0];
 #pragma unroll
     for (int j = 1; j < kScoreVecs; j++) vm = max_nan(vm, vmax[j]);
-    if (!(vm <= m)) raise(vm);
+    raise(vm);
     const float ref = m == -INFINITY ? 0.0f : m;
     const float2 neg = {-ref, -ref}, c2 = {c, c};
 #pragma unroll
@@ -294,36 +325,32 @@ __global__ void __launch_bounds__(kScoreThreads) token_score_kernel(const ScoreA
           }
       top.start(i < v1 ? entry(vm, own) : 0, a.top_k);
     }
-    // later steps have higher indices, so a logit equal to the list's last comes
-    // after it; within the first step, and against other warps, it may come before
-    const bool first = it == 0;
-    float seen = top.last ? order_value((uint32_t)(top.last >> 32)) : -INFINITY;
-    auto passes = [&](float y) {
-      return (!(y <= seen) || (y == seen && (first || top.last == 0))) && !(y < floor);
-    };
-    if (__any_sync(0xffffffffu, passes(vm))) {
+    if (it == 0) set_pass(true);
+    if (__any_sync(0xffffffffu, !(vm <= pass))) {
 #pragma unroll
       for (int j = 0; j < kScoreVecs; j++) {
-        if (!__any_sync(0xffffffffu, passes(vmax[j]))) continue;
+        if (!__any_sync(0xffffffffu, !(vmax[j] <= pass))) continue;
+        const bool valid = i + j * 32 < v1;
 #pragma unroll
         for (int e = 0; e < N; e++) {
           const uint32_t at = at0 + 32 * N * j + e;
-          const bool in = i + j * 32 < v1 && at != own && passes(v[j][e]);
+          const bool in = valid && at != own && !(v[j][e] <= pass);
           if (__any_sync(0xffffffffu, in)) {
             top.offer(in ? entry(v[j][e], at) : 0, a.top_k);
-            seen = top.last ? order_value((uint32_t)(top.last >> 32)) : -INFINITY;
+            set_pass(it == 0);
           }
         }
       }
     }
+    if (it == 0) set_pass(false);
     if (it + 1 == refresh && it + 1 < n_steps) {
       refresh *= 4;
       if (lane < a.top_k) lists[w * a.top_k + lane] = top.mine;
       __syncthreads();
       rank_entries(lists, kScoreWarps * a.top_k, a.top_k, best);
       __syncthreads();
-      const uint64_t kth = best[a.top_k - 1];
-      floor = kth ? order_value((uint32_t)(kth >> 32)) : -INFINITY;
+      floor = (uint32_t)(best[a.top_k - 1] >> 32);
+      set_pass(false);
     }
   }
   if (rank == 0 && w == 0) {
@@ -331,7 +358,7 @@ __global__ void __launch_bounds__(kScoreThreads) token_score_kernel(const ScoreA
     const bool is = lane < 16 ? lane < lead : tail < a.vocab;
     const int at = lane < 16 ? lane : tail;
     const float y = is ? Lanes<T>::one(x + at) : -INFINITY;
-    if (!(y <= m)) raise(y);
+    raise(y);
     const float d = max_nan((y - (m == -INFINITY ? 0.0f : m)) * c, -1e4f), p = fast_exp2(d);
     s2.x += p;
     u2.x = fmaf(p, d, u2.x);
@@ -339,29 +366,23 @@ __global__ void __launch_bounds__(kScoreThreads) token_score_kernel(const ScoreA
   }
 
   // the warp's, the CTA's, the row's
-  Sums acc = {m, s2.x + s2.y, u2.x + u2.y};
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Sums b = {__shfl_xor_sync(0xffffffffu, acc.m, o), __shfl_xor_sync(0xffffffffu, acc.s, o),
-              __shfl_xor_sync(0xffffffffu, acc.u, o)};
-    acc = join(acc, b, c);
-  }
+  Sums acc = join_lanes({m, s2.x + s2.y, u2.x + u2.y}, c);
   if (lane == 0) sums[w] = acc;
   if (TOP && lane < a.top_k) lists[w * a.top_k + lane] = top.mine;
   __syncthreads();
   if (w == 0) {
-    for (int i = 1; i < kScoreWarps; i++) acc = join(acc, sums[i], c);
+    acc = join_lanes(lane < kScoreWarps ? sums[lane] : Sums{-INFINITY, 0.0f, 0.0f}, c);
     if (lane == 0) cta_sums = acc;
   }
   if (TOP) rank_entries(lists, kScoreWarps * a.top_k, a.top_k, n_ctas > 1 ? cta_list : best);
   if (n_ctas > 1) {
     score_cluster_sync();
     if (rank == 0) {
-      if (w == 0)
-        for (int r = 1; r < n_ctas; r++) {
-          const uint32_t p = cluster_peer(&cta_sums, r);
-          acc = join(acc, Sums{peer_f32(p), peer_f32(p + 4), peer_f32(p + 8)}, c);
-        }
+      if (w == 0) {
+        const uint32_t p = cluster_peer(&cta_sums, lane < n_ctas ? lane : 0);
+        acc = {peer_f32(p), peer_f32(p + 4), peer_f32(p + 8)};
+        acc = join_lanes(lane < n_ctas ? acc : Sums{-INFINITY, 0.0f, 0.0f}, c);
+      }
       if (TOP) {
         if (threadIdx.x < n_ctas * a.top_k) {
           const int r = threadIdx.x / a.top_k;
