@@ -87,46 +87,6 @@ __device__ __forceinline__ Sums join_lanes(Sums x, float c) {
   return x;
 }
 
-// The warp's best entries, one a lane, best first; the first top_k count.
-struct TopList {
-  uint64_t mine = 0;   // this lane's entry
-  uint64_t last = 0;   // entry top_k - 1: what a newcomer has to beat
-
-  // each lane's x, sorted: the list's first contents
-  __device__ __forceinline__ void start(uint64_t x, int top_k) {
-    const int lane = lane_id();
-#pragma unroll
-    for (int k = 2; k <= 32; k <<= 1)
-#pragma unroll
-      for (int j = k >> 1; j > 0; j >>= 1) {
-        const uint64_t y = __shfl_xor_sync(0xffffffffu, x, j);
-        const bool keep_max = ((lane & k) == 0) == ((lane & j) == 0);
-        x = keep_max == (x > y) ? x : y;
-      }
-    mine = x;
-    last = __shfl_sync(0xffffffffu, mine, top_k - 1);
-  }
-  // x (the same in all lanes) takes its place
-  __device__ __forceinline__ void insert(uint64_t x, int top_k) {
-    const int lane = lane_id();
-    const uint64_t up = __shfl_up_sync(0xffffffffu, mine, 1);
-    const int at = __popc(__ballot_sync(0xffffffffu, mine > x));
-    if (lane == at) mine = x;
-    if (lane > at) mine = up;
-    last = __shfl_sync(0xffffffffu, mine, top_k - 1);
-  }
-  // each lane's x where it beats the list
-  __device__ __forceinline__ void offer(uint64_t x, int top_k) {
-    uint32_t who = __ballot_sync(0xffffffffu, x > last);
-    while (who) {
-      const int from = __ffs(who) - 1;
-      insert(__shfl_sync(0xffffffffu, x, from), top_k);
-      who &= who - 1;
-      who &= __ballot_sync(0xffffffffu, x > last);
-    }
-  }
-};
-
 template <typename T>
 struct Lanes;
 template <>
@@ -176,51 +136,193 @@ __device__ __forceinline__ void score_cluster_sync() {
                ::: "memory");
 }
 
-// The first top_k of n entries (n <= kScoreThreads, distinct but for 0) in order:
-// every thread counts the entries above its own. Called by the whole CTA.
-__device__ __forceinline__ void rank_entries(const uint64_t* from, int n, int top_k,
-                                             uint64_t* to) {
-  const int t = threadIdx.x;
-  if (t < n) {
-    const uint64_t x = from[t];
-    int rank = 0;
-#pragma unroll 8
-    for (int i = 0; i < n; i++) rank += from[i] > x;
-    if (x && rank < top_k) to[rank] = x;
+constexpr int kCandidates = 768;
+
+// A CTA's candidates for the alternatives, in no order, and the best of them.
+struct Candidates {
+  uint64_t list[kCandidates];
+  uint64_t best[kScoreMaxTop];
+  uint64_t part[kScoreWarps];
+  uint32_t sorted[kScoreWarps][32];   // each warp's largest logits, descending
+  uint32_t reach;                     // the top_k-th largest of them: top_k reach it
+  int n, n_owners;
+  uint8_t owners[kScoreThreads];      // threads whose largest logit reaches it
+};
+
+// Sets c.reach from each thread's largest logit (its order_key; 0: it has none), and
+// c.owners. Called by every thread, after a barrier; ends with one.
+__device__ __forceinline__ void find_reach(Candidates& c, uint32_t key, int top_k) {
+  const int lane = lane_id(), w = warp_id();
+  int r = 0;
+#pragma unroll
+  for (int j = 0; j < 32; j++) {
+    const uint32_t y = __shfl_sync(0xffffffffu, key, j);
+    r += y > key || (y == key && j < lane);
   }
+  c.sorted[w][r] = key;
+  __syncthreads();
+  int above = 0;   // largest logits above this one, by a search in each warp's
+#pragma unroll
+  for (int u = 0; u < kScoreWarps; u++) {
+    int at = 0;
+#pragma unroll
+    for (int step = 16; step > 0; step >>= 1)
+      if (c.sorted[u][at + step - 1] > key) at += step;
+    above += at + (c.sorted[u][at] > key ? 1 : 0);
+  }
+  if (above < top_k) atomicMin(&c.reach, key);
+  __syncthreads();
+  if (key && key >= c.reach) c.owners[atomicAdd(&c.n_owners, 1)] = (uint8_t)threadIdx.x;
+  __syncthreads();
+}
+static_assert(kScoreThreads <= 256, "a thread's number is kept in a byte");
+
+// The first top_k of c.list's n <= kCandidates entries (distinct but for 0) to c.best,
+// 0 past their number: an entry's place is the number of entries above it. Called by
+// every thread, after a barrier; ends with one.
+__device__ __forceinline__ void rank_candidates(Candidates& c, int n, int top_k) {
+  if (threadIdx.x < kScoreMaxTop) c.best[threadIdx.x] = 0;
+  __syncthreads();
+#pragma unroll 1
+  for (int i = threadIdx.x; i < n; i += kScoreThreads) {
+    const uint64_t e = c.list[i];
+    int r = 0;
+#pragma unroll 8
+    for (int j = 0; j < n; j++) r += c.list[j] > e;
+    if (e && r < top_k) c.best[r] = e;
+  }
+  __syncthreads();
+}
+
+// A CTA's vectors of a row: thread t's are i(it, j) + 32 j for each step it.
+template <typename T>
+struct Slice {
+  const uint4* vec;
+  int lead, v0, v1, n_steps;
+  static constexpr int kStep = kScoreThreads * kScoreVecs;
+  static __device__ __forceinline__ int at(int step, int j, int t) {
+    return step * kStep + (t >> 5) * 32 * kScoreVecs + j * 32 + (t & 31);
+  }
+};
+
+// The largest entry below `bar` among thread t's vectors, found by t's whole warp
+// (each lane gets it).
+template <typename T>
+__device__ __forceinline__ uint64_t best_below(const Slice<T>& s, int t, uint64_t bar) {
+  constexpr int N = Lanes<T>::N;
+  uint64_t mx = 0;
+  for (int i = lane_id(); i < s.n_steps * kScoreVecs; i += 32) {
+    const int k = s.v0 + Slice<T>::at(i / kScoreVecs, i % kScoreVecs, t);
+    if (k >= s.v1) continue;
+    float v[N];
+    Lanes<T>::unpack(__ldg(s.vec + k), v);
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+      const uint64_t y = entry(v[e], (uint32_t)(s.lead + k * N + e));
+      if (y < bar && y > mx) mx = y;
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const uint64_t y = __shfl_xor_sync(0xffffffffu, mx, o);
+    mx = y > mx ? y : mx;
+  }
+  return mx;
+}
+
+// c.best by taking the largest entry top_k times, for rows where too many logits
+// reach the threshold (most tokens masked, long runs of equal logits): `edge` is
+// an entry of the thread's own besides its vectors, or 0.
+template <typename T>
+__device__ __noinline__ void take_best(const Slice<T>& s, Candidates& c, int top_k,
+                                       uint64_t edge) {
+  const int lane = lane_id(), w = warp_id();
+  uint64_t mine = 0;   // the thread's largest vector entry not yet taken
+  for (int l = 0; l < 32; l++) {
+    const uint64_t y = best_below(s, w * 32 + l, ~0ull);
+    if (l == lane) mine = y;
+  }
+  for (int r = 0; r < top_k; r++) {
+    const uint64_t own = edge > mine ? edge : mine;
+    uint64_t mx = own;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const uint64_t y = __shfl_xor_sync(0xffffffffu, mx, o);
+      mx = y > mx ? y : mx;
+    }
+    if (lane == 0) c.part[w] = mx;
+    __syncthreads();
+    uint64_t all = 0;
+    for (int u = 0; u < kScoreWarps; u++) all = c.part[u] > all ? c.part[u] : all;
+    if (threadIdx.x == 0) c.best[r] = all;
+    __syncthreads();
+    if (all && mx == all) {   // this warp's: the lane that holds it looks for its next
+      const uint32_t who = __ballot_sync(0xffffffffu, own == all && edge != all);
+      if (edge == all) edge = 0;
+      if (who) {
+        const int l = __ffs(who) - 1;
+        const uint64_t y = best_below(s, w * 32 + l, all);
+        if (l == lane) mine = y;
+      }
+    }
+  }
+  __syncthreads();
 }
 
 // Row blockIdx.y by a cluster of gridDim.x CTAs, each a contiguous part of it.
 //
 // A thread takes kScoreVecs 16-byte vectors a step, copied kScoreStages - 1 steps
-// ahead into shared memory, and rescales its sums when its
-// own maximum moves. A warp's list starts as its lanes' first maxima, sorted. From
-// then on a vector is looked into only if its largest logit passes the list's last
-// one and is not below `bound`, the CTA's top_k-th logit so far, which the lists
-// are joined for after steps 1, 4, 16 and so on: about top_k logits of a row pass
-// each time the logits seen have grown fourfold. The parts are joined in shared
-// memory, then over the cluster's, the lists by counting ranks.
+// ahead into shared memory; the warp shares the reference of its sums. For the
+// alternatives the pass keeps each thread's largest logit and nothing else. The
+// top_k-th of these is a logit that top_k reach, so the alternatives are among the
+// logits of the few threads whose largest reaches it: these are gone over again
+// (from shared memory or L2), and those that reach it are listed and put in order
+// by counting ranks. The parts are joined in shared memory, then over the cluster's.
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kScoreThreads) token_score_kernel(const ScoreArgs a) {
   constexpr int N = Lanes<T>::N;
   __shared__ Sums sums[kScoreWarps];
   __shared__ Sums cta_sums;
-  __shared__ uint64_t lists[kScoreThreads];   // of kScoreWarps warps or kScoreMaxCtas CTAs
-  __shared__ uint64_t cta_list[kScoreMaxTop], best[kScoreMaxTop];
   __shared__ uint4 ring[kScoreStages][kScoreVecs][kScoreThreads];
-  static_assert(kScoreMaxCtas * kScoreMaxTop <= kScoreThreads && kScoreMaxCtas <= 32, "");
+  __shared__ Candidates cand;
   const int lane = lane_id(), w = warp_id();
   const int rank = blockIdx.x, n_ctas = gridDim.x;
   const int64_t row = blockIdx.y;
   const T* x = static_cast<const T*>(a.logits) + row * a.ld;
   const float c = 1.4426950408889634f * a.inv_t;
-  if (TOP) {
-    if (threadIdx.x < kScoreMaxTop) cta_list[threadIdx.x] = best[threadIdx.x] = 0;
-    __syncthreads();
+
+  // the elements before the first and past the last whole vector are left for the
+  // end
+  Slice<T> s;
+  s.lead = (int)min(a.vocab, (int64_t)(((16 - ((uintptr_t)x & 15)) & 15) / sizeof(T)));
+  const int n_vec = (int)((a.vocab - s.lead) / N);
+  s.vec = reinterpret_cast<const uint4*>(x + s.lead);
+  s.v0 = (int)((int64_t)n_vec * rank / n_ctas);
+  s.v1 = (int)((int64_t)n_vec * (rank + 1) / n_ctas);
+  s.n_steps = (s.v1 - s.v0 + Slice<T>::kStep - 1) / Slice<T>::kStep;
+  // each thread copies its vectors ahead into slots that only it reads
+  auto fetch = [&](int it) {
+#pragma unroll
+    for (int j = 0; j < kScoreVecs; j++) {
+      const int i = s.v0 + Slice<T>::at(it, j, threadIdx.x);
+      if (i < s.v1)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                         smem_u32(&ring[it % kScoreStages][j][threadIdx.x])),
+                     "l"(s.vec + i)
+                     : "memory");
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int it = 0; it < kScoreStages - 1; it++) fetch(it);
+  if (TOP && threadIdx.x == 0) {
+    cand.reach = 0xFFFFFFFFu;
+    cand.n = cand.n_owners = 0;
   }
 
   float m = -INFINITY;
   float2 s2 = {0.0f, 0.0f}, u2 = {0.0f, 0.0f};
+  float largest = -INFINITY;   // the thread's
   // the warp's maximum becomes that of vm where it is larger: seldom after a few
   // steps, since the warp's lanes share it
   auto raise = [&](float vm) {
@@ -231,69 +333,29 @@ __global__ void __launch_bounds__(kScoreThreads) token_score_kernel(const ScoreA
     u2 = {x.u, y.u};
     m = to;
   };
-  TopList top;
-  // a logit is looked at unless it is <= pass: the list's last one, since later
-  // steps have higher indices and an equal logit comes after, or just below the
-  // CTA's top_k-th so far, since against other warps it may come before
-  float pass = -INFINITY;
-  uint32_t floor = 0;        // order_key of the CTA's top_k-th logit so far
-  auto set_pass = [&](bool equals) {
-    const uint32_t own = (uint32_t)(top.last >> 32);
-    uint32_t k = max(own - (equals && own ? 1 : 0), floor ? floor - 1 : 0);
-    if (k == 0x7FFFFFFFu) k--;   // -0, which compares equal to the 0 above it
-    pass = k ? order_value(k) : __uint_as_float(0x7FC00000u);   // NaN: everything passes
-  };
 
-  // the elements before the first and past the last whole vector: `edges`, at the
-  // end, by the first CTA's first warp
-  const int lead = (int)min(a.vocab, (int64_t)(((16 - ((uintptr_t)x & 15)) & 15) / sizeof(T)));
-  const int n_vec = (int)((a.vocab - lead) / N);
-  const uint4* xv = reinterpret_cast<const uint4*>(x + lead);
-  const int v0 = (int)((int64_t)n_vec * rank / n_ctas);
-  const int v1 = (int)((int64_t)n_vec * (rank + 1) / n_ctas);
-  constexpr int kStep = kScoreThreads * kScoreVecs;
-  const int n_steps = (v1 - v0 + kStep - 1) / kStep;
-  // each thread copies its vectors ahead into slots that only it reads
-  auto fetch = [&](int it) {
-    const int i = v0 + it * kStep + w * 32 * kScoreVecs + lane;
-#pragma unroll
-    for (int j = 0; j < kScoreVecs; j++)
-      if (i + j * 32 < v1)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                         smem_u32(&ring[it % kScoreStages][j][threadIdx.x])),
-                     "l"(xv + i + j * 32)
-                     : "memory");
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-#pragma unroll
-  for (int it = 0; it < kScoreStages - 1; it++) fetch(it);
-  int refresh = 1;
-  for (int it = 0; it < n_steps; it++) {
-    // a warp's vectors of a step lie side by side, so its indices only grow
-    const int i = v0 + it * kStep + w * 32 * kScoreVecs + lane;
+#pragma unroll 1
+  for (int it = 0; it < s.n_steps; it++) {
     fetch(it + kScoreStages - 1);
     asm volatile("cp.async.wait_group %0;" ::"n"(kScoreStages - 1) : "memory");
-    float v[kScoreVecs][N], vmax[kScoreVecs];
+    float v[kScoreVecs][N];
 #pragma unroll
     for (int j = 0; j < kScoreVecs; j++)
       Lanes<T>::unpack(ring[it % kScoreStages][j][threadIdx.x], v[j]);
-    if (it + 1 == n_steps) {
+    if (it + 1 == s.n_steps) {
 #pragma unroll
       for (int j = 0; j < kScoreVecs; j++)
-        if (i + j * 32 >= v1) {
+        if (s.v0 + Slice<T>::at(it, j, threadIdx.x) >= s.v1) {
 #pragma unroll
           for (int e = 0; e < N; e++) v[j][e] = -INFINITY;
         }
     }
+    float vm = v[0][0];
 #pragma unroll
-    for (int j = 0; j < kScoreVecs; j++) {
-      vmax[j] = max_nan(v[j][0], v[j][1]);
+    for (int j = 0; j < kScoreVecs; j++)
 #pragma unroll
-      for (int e = 2; e < N; e += 2) vmax[j] = max_nan(vmax[j], v[j][e], v[j][e + 1]);
-    }
-    float vm = vmax[0];
-#pragma unroll
-    for (int j = 1; j < kScoreVecs; j++) vm = max_nan(vm, vmax[j]);
+      for (int e = 0; e < N; e += 2) vm = max_nan(vm, v[j][e], v[j][e + 1]);
+    if (TOP) largest = max_nan(largest, vm);
     raise(vm);
     const float ref = m == -INFINITY ? 0.0f : m;
     const float2 neg = {-ref, -ref}, c2 = {c, c};
@@ -309,72 +371,60 @@ __global__ void __launch_bounds__(kScoreThreads) token_score_kernel(const ScoreA
         s2 = __fadd2_rn(s2, p);
         u2 = __ffma2_rn(p, d, u2);
       }
-    if (!TOP) continue;
-
-    const uint32_t at0 = (uint32_t)lead + (uint32_t)i * N;   // vector j: + 32 N j
-    uint32_t own = 0xFFFFFFFFu;   // the lane's entry of the list's start
-    if (it == 0) {
-      bool got = false;
-#pragma unroll
-      for (int j = 0; j < kScoreVecs; j++)
-#pragma unroll
-        for (int e = 0; e < N; e++)
-          if (!got && (v[j][e] == vm || v[j][e] != v[j][e])) {
-            got = true;
-            own = at0 + 32 * N * j + e;
-          }
-      top.start(i < v1 ? entry(vm, own) : 0, a.top_k);
-    }
-    if (it == 0) set_pass(true);
-    if (__any_sync(0xffffffffu, !(vm <= pass))) {
-#pragma unroll
-      for (int j = 0; j < kScoreVecs; j++) {
-        if (!__any_sync(0xffffffffu, !(vmax[j] <= pass))) continue;
-        const bool valid = i + j * 32 < v1;
-#pragma unroll
-        for (int e = 0; e < N; e++) {
-          const uint32_t at = at0 + 32 * N * j + e;
-          const bool in = valid && at != own && !(v[j][e] <= pass);
-          if (__any_sync(0xffffffffu, in)) {
-            top.offer(in ? entry(v[j][e], at) : 0, a.top_k);
-            set_pass(it == 0);
-          }
-        }
-      }
-    }
-    if (it == 0) set_pass(false);
-    if (it + 1 == refresh && it + 1 < n_steps) {
-      refresh *= 4;
-      if (lane < a.top_k) lists[w * a.top_k + lane] = top.mine;
-      __syncthreads();
-      rank_entries(lists, kScoreWarps * a.top_k, a.top_k, best);
-      __syncthreads();
-      floor = (uint32_t)(best[a.top_k - 1] >> 32);
-      set_pass(false);
-    }
   }
+  // the row's edges
+  uint64_t edge = 0;
   if (rank == 0 && w == 0) {
-    const int tail = lead + n_vec * N + lane - 16;
-    const bool is = lane < 16 ? lane < lead : tail < a.vocab;
+    const int tail = s.lead + n_vec * N + lane - 16;
+    const bool is = lane < 16 ? lane < s.lead : tail < a.vocab;
     const int at = lane < 16 ? lane : tail;
     const float y = is ? Lanes<T>::one(x + at) : -INFINITY;
     raise(y);
     const float d = max_nan((y - (m == -INFINITY ? 0.0f : m)) * c, -1e4f), p = fast_exp2(d);
     s2.x += p;
     u2.x = fmaf(p, d, u2.x);
-    if (TOP) top.offer(is ? entry(y, (uint32_t)at) : 0, a.top_k);
+    if (is) edge = entry(y, (uint32_t)at);
   }
 
   // the warp's, the CTA's, the row's
   Sums acc = join_lanes({m, s2.x + s2.y, u2.x + u2.y}, c);
   if (lane == 0) sums[w] = acc;
-  if (TOP && lane < a.top_k) lists[w * a.top_k + lane] = top.mine;
-  __syncthreads();
+  __syncthreads();   // reach, n and n_owners are set too
   if (w == 0) {
     acc = join_lanes(lane < kScoreWarps ? sums[lane] : Sums{-INFINITY, 0.0f, 0.0f}, c);
     if (lane == 0) cta_sums = acc;
   }
-  if (TOP) rank_entries(lists, kScoreWarps * a.top_k, a.top_k, n_ctas > 1 ? cta_list : best);
+  if (TOP) {
+    const bool has = s.v0 + Slice<T>::at(0, 0, threadIdx.x) < s.v1;
+    find_reach(cand, has ? order_key(largest) : 0, a.top_k);
+    const uint32_t reach = cand.reach;
+    auto list = [&](uint64_t e) {
+      const int at = atomicAdd(&cand.n, 1);
+      if (at < kCandidates) cand.list[at] = e;
+    };
+    if (edge && (uint32_t)(edge >> 32) >= reach) list(edge);
+    // the owners' vectors, dealt out over the CTA; what is left in the ring is there
+    const int per = s.n_steps * kScoreVecs, n = cand.n_owners * per;
+    const bool in_ring = s.n_steps <= kScoreStages;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n; i += kScoreThreads) {
+      const int t = cand.owners[i / per], f = i % per, it = f / kScoreVecs, j = f % kScoreVecs;
+      const int k = s.v0 + Slice<T>::at(it, j, t);
+      if (k >= s.v1) continue;
+      float v[N];
+      Lanes<T>::unpack(in_ring ? ring[it][j][t] : __ldg(s.vec + k), v);
+#pragma unroll
+      for (int e = 0; e < N; e++) {
+        const uint32_t y = order_key(v[e]);
+        if (y >= reach) list(((uint64_t)y << 32) | ~(uint32_t)(s.lead + k * N + e));
+      }
+    }
+    __syncthreads();
+    if (cand.n <= kCandidates)
+      rank_candidates(cand, cand.n, a.top_k);
+    else
+      take_best(s, cand, a.top_k, edge);
+  }
   if (n_ctas > 1) {
     score_cluster_sync();
     if (rank == 0) {
@@ -383,19 +433,15 @@ __global__ void __launch_bounds__(kScoreThreads) token_score_kernel(const ScoreA
         acc = {peer_f32(p), peer_f32(p + 4), peer_f32(p + 8)};
         acc = join_lanes(lane < n_ctas ? acc : Sums{-INFINITY, 0.0f, 0.0f}, c);
       }
-      if (TOP) {
-        if (threadIdx.x < n_ctas * a.top_k) {
-          const int r = threadIdx.x / a.top_k;
-          lists[threadIdx.x] =
-              peer_u64(cluster_peer(cta_list + (threadIdx.x - r * a.top_k), r));
-        }
-        __syncthreads();
-        rank_entries(lists, n_ctas * a.top_k, a.top_k, best);
-      }
+      // CTA u's list by warp u
+      if (TOP && w < n_ctas && lane < a.top_k)
+        cand.list[w * a.top_k + lane] = peer_u64(cluster_peer(cand.best + lane, w));
     }
-    score_cluster_sync();   // a CTA's shared memory outlives its readers
-  } else if (TOP) {
-    __syncthreads();
+    // a CTA's shared memory outlives its readers: nothing is handed over
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;"
+                 ::: "memory");
+    if (rank != 0) return;
+    if (TOP) rank_candidates(cand, n_ctas * a.top_k, a.top_k);
   }
   if (rank != 0 || w != 0) return;
 
@@ -411,11 +457,13 @@ __global__ void __launch_bounds__(kScoreThreads) token_score_kernel(const ScoreA
       a.entropy[row] = empty ? 0.0f : log_s - 0.6931471805599453f * (acc.u / acc.s);
   }
   if (TOP && lane < a.top_k) {
-    const uint64_t e = best[lane];
+    const uint64_t e = cand.best[lane];
     a.top_logprob[row * a.top_k + lane] = logprob(order_value((uint32_t)(e >> 32)));
     a.top_index[row * a.top_k + lane] = (int32_t)~(uint32_t)e;
   }
 }
+static_assert(kScoreMaxCtas <= kScoreWarps, "a CTA's list for each warp of the first");
+static_assert(kScoreMaxCtas * kScoreMaxTop <= kCandidates, "");
 
 template <typename T, bool TOP>
 static cudaError_t launch_score(const ScoreArgs& a, int ctas, int64_t rows, cudaStream_t st) {
