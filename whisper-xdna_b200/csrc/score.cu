@@ -18,7 +18,7 @@ constexpr int kScoreThreads = 256, kScoreWarps = kScoreThreads / 32;
 constexpr int kScoreMaxCtas = 8;    // CTAs (one cluster) on a row
 constexpr int kScoreMaxTop = 32;    // one lane each
 constexpr int kScoreVecs = 2;       // 16-byte vectors of a thread's step
-constexpr int kScoreStages = 5;     // steps in flight
+constexpr int kScoreStages = 4;     // steps in flight
 
 struct ScoreArgs {
   const void* logits;
@@ -279,7 +279,7 @@ __device__ __noinline__ void take_best(const Slice<T>& s, Candidates& c, int top
 // (from shared memory or L2), and those that reach it are listed and put in order
 // by counting ranks. The parts are joined in shared memory, then over the cluster's.
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kScoreThreads) token_score_kernel(const ScoreArgs a) {
+__global__ void __launch_bounds__(kScoreThreads, 4) token_score_kernel(const ScoreArgs a) {
   constexpr int N = Lanes<T>::N;
   __shared__ Sums sums[kScoreWarps];
   __shared__ Sums cta_sums;
@@ -413,6 +413,10 @@ __global__ void __launch_bounds__(kScoreThreads) token_score_kernel(const ScoreA
       if (k >= s.v1) continue;
       float v[N];
       Lanes<T>::unpack(in_ring ? ring[it][j][t] : __ldg(s.vec + k), v);
+      float vm = v[0];
+#pragma unroll
+      for (int e = 0; e < N; e += 2) vm = max_nan(vm, v[e], v[e + 1]);
+      if (order_key(vm) < reach) continue;
 #pragma unroll
       for (int e = 0; e < N; e++) {
         const uint32_t y = order_key(v[e]);
