@@ -64,144 +64,17 @@ __device__ __forceinline__ void key_range(const PagedArgs& a, int seq, int* firs
 constexpr int kPagedThreads = 128;
 constexpr int kPagedWarps = kPagedThreads / 32;
 
-// GT query rows of one (sequence, head) against the keys of one split, fp32:
-// products on the FMA pipe, which keeps all of their bits. Each group of `lanes` lanes holds a key row (16 bytes a
-// lane); the groups of the CTA take tokens in turn, keep sums of their own and
-// are joined at the end.
-template <int HD, int GT>
-__global__ void __launch_bounds__(kPagedThreads) paged_attention_fma_kernel(const PagedArgs a) {
-  constexpr int N = 4, kLanes = HD / N;     // lanes on a row
-  constexpr int kRows = 32 / kLanes;                 // rows a warp reads at once
-  constexpr int kStreams = kPagedWarps * kRows;      // token streams of the CTA
-  constexpr int U = 4;                               // tokens of a stream in flight
-  static_assert(kLanes <= 32 && 32 % kLanes == 0, "");
-  __shared__ float sh_o[kStreams][GT][HD];
-  __shared__ float sh_m[kStreams][GT], sh_l[kStreams][GT];
-  pdl_launch_dependents();   // the join waits for this kernel's end
-
-  const int tiles = (a.group + GT - 1) / GT;
-  const int split = blockIdx.x / tiles, tile = blockIdx.x - split * tiles;
-  const int head = blockIdx.y, seq = blockIdx.z;
-  const int g0 = tile * GT, g_n = min(GT, a.group - g0);
-  int first, end;
-  key_range(a, seq, &first, &end);
-  const int c0 = max(first, split * a.chunk), c1 = min(end, (split + 1) * a.chunk);
-  if (c0 >= c1 && a.splits > 1) return;   // the join skips it too
-
-  const int lane = lane_id(), sub = lane % kLanes;
-  const int stream = warp_id() * kRows + lane / kLanes;
-  const float* q = static_cast<const float*>(a.q) + seq * a.q_seq + head * a.q_head;
-  const float* kp = static_cast<const float*>(a.k) + head * a.head_stride + sub * N;
-  const float* vp = static_cast<const float*>(a.v) + head * a.head_stride + sub * N;
-  const int32_t* row = a.table + seq * a.ld_table;
-
-  float qr[GT][N], o[GT][N], m[GT], l[GT];
-#pragma unroll
-  for (int g = 0; g < GT; g++) {
-    m[g] = -INFINITY;
-    l[g] = 0.0f;
-#pragma unroll
-    for (int e = 0; e < N; e++) {
-      o[g][e] = 0.0f;
-      qr[g][e] = g < g_n ? q[(g0 + g) * a.q_group + sub * N + e] * a.scale_log2 : 0.0f;
-    }
+// Where key t of the sequence with this row of the table is, in elements from the
+// head's first; -1: on no page.
+__device__ __forceinline__ int64_t key_at(const PagedArgs& a, const int32_t* row, int t) {
+  const int slot = page_slot(a, t);
+  const int page = __ldg(row + slot);
+  if (page < 0 || page >= a.n_pages) {
+    atomicOr(&g_attend_err, WX_DEVERR_PAGE);
+    return -1;
   }
-  for (int t0 = c0 + stream; t0 - stream < c1; t0 += kStreams * U) {
-    float4 kw[U], vw[U];
-    bool ok[U];
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-      const int t = t0 + u * kStreams;
-      ok[u] = t < c1;
-      kw[u] = vw[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (ok[u]) {
-        const int slot = page_slot(a, t);
-        const int page = row[slot];
-        if (page < 0 || page >= a.n_pages) {
-          atomicOr(&g_attend_err, WX_DEVERR_PAGE);
-          ok[u] = false;
-        } else {
-          const int64_t at = page * a.page_stride + (t - slot * a.page_size) * a.tok_stride;
-          kw[u] = *reinterpret_cast<const float4*>(kp + at);
-          vw[u] = *reinterpret_cast<const float4*>(vp + at);
-        }
-      }
-    }
-    float s[U][GT];
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-      const float kf[N] = {kw[u].x, kw[u].y, kw[u].z, kw[u].w};
-#pragma unroll
-      for (int g = 0; g < GT; g++) {
-        float x = 0.0f;
-#pragma unroll
-        for (int e = 0; e < N; e++) x = fmaf(qr[g][e], kf[e], x);
-#pragma unroll
-        for (int w = kLanes / 2; w > 0; w >>= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
-        s[u][g] = ok[u] ? x : -INFINITY;
-      }
-    }
-#pragma unroll
-    for (int g = 0; g < GT; g++) {
-      float mx = m[g];
-#pragma unroll
-      for (int u = 0; u < U; u++) mx = fmaxf(mx, s[u][g]);
-      const float mu = mx == -INFINITY ? 0.0f : mx;
-      const float f = fast_exp2(m[g] - mu);
-      m[g] = mx;
-      l[g] *= f;
-#pragma unroll
-      for (int e = 0; e < N; e++) o[g][e] *= f;
-#pragma unroll
-      for (int u = 0; u < U; u++) {
-        s[u][g] = fast_exp2(s[u][g] - mu);
-        l[g] += s[u][g];
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-      const float vf[N] = {vw[u].x, vw[u].y, vw[u].z, vw[u].w};
-#pragma unroll
-      for (int g = 0; g < GT; g++)
-#pragma unroll
-        for (int e = 0; e < N; e++) o[g][e] = fmaf(s[u][g], vf[e], o[g][e]);
-    }
-  }
-#pragma unroll
-  for (int g = 0; g < GT; g++) {
-#pragma unroll
-    for (int e = 0; e < N; e++) sh_o[stream][g][sub * N + e] = o[g][e];
-    if (sub == 0) {
-      sh_m[stream][g] = m[g];
-      sh_l[stream][g] = l[g];
-    }
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < g_n * HD; i += kPagedThreads) {
-    const int g = i / HD, d = i - g * HD;
-    float mx = -INFINITY;
-    for (int w = 0; w < kStreams; w++) mx = fmaxf(mx, sh_m[w][g]);
-    const float mu = mx == -INFINITY ? 0.0f : mx;
-    float sum = 0.0f, x = 0.0f;
-    for (int w = 0; w < kStreams; w++) {
-      const float f = fast_exp2(sh_m[w][g] - mu);
-      sum = fmaf(sh_l[w][g], f, sum);
-      x = fmaf(sh_o[w][g][d], f, x);
-    }
-    const int64_t r = ((int64_t)seq * a.n_heads + head) * a.group + g0 + g;
-    if (a.splits > 1) {
-      a.part_o[(r * a.splits + split) * HD + d] = x;
-      if (d == 0) a.part_ml[r * a.splits + split] = make_float2(mx, sum);
-    } else {
-      float* out = static_cast<float*>(a.out) + seq * a.o_seq + head * a.o_head + (g0 + g) * a.o_group;
-      out[d] = sum == 0.0f ? 0.0f : x / sum;
-      if (d == 0 && a.lse)
-        a.lse[r] = sum == 0.0f ? -INFINITY : (mx + log2f(sum)) * 0.6931471805599453f;
-    }
-  }
+  return page * a.page_stride + (t - slot * a.page_size) * a.tok_stride;
 }
-
-// ---------------------------------------------------------------- tensor cores
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
   // src_size 0 reads nothing and writes zeros
@@ -216,6 +89,254 @@ template <int N>
 __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
+
+// The warps' parts of ROWS query rows, (maximum, sum, o) in shared memory, joined
+// and written: the result where the cache's length is not split, else a part.
+template <typename T, int HD, int ROWS>
+__device__ __forceinline__ void join_warps(const PagedArgs& a, const float* part,
+                                           const float (&sh_m)[kPagedWarps][ROWS],
+                                           const float (&sh_l)[kPagedWarps][ROWS], int seq,
+                                           int head, int split, int g0, int g_n) {
+  for (int i = threadIdx.x; i < g_n * HD; i += kPagedThreads) {
+    const int g = i / HD, d = i - g * HD;
+    float mx = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < kPagedWarps; u++) mx = fmaxf(mx, sh_m[u][g]);
+    const float mu = mx == -INFINITY ? 0.0f : mx;
+    float sum = 0.0f, x = 0.0f;
+#pragma unroll
+    for (int u = 0; u < kPagedWarps; u++) {
+      const float f = fast_exp2(sh_m[u][g] - mu);
+      sum = fmaf(sh_l[u][g], f, sum);
+      x = fmaf(part[(u * ROWS + g) * HD + d], f, x);
+    }
+    const int64_t r = ((int64_t)seq * a.n_heads + head) * a.group + g0 + g;
+    if (a.splits > 1) {
+      a.part_o[(r * a.splits + split) * HD + d] = x;
+      if (d == 0) a.part_ml[r * a.splits + split] = make_float2(mx, sum);
+    } else {
+      T* out = static_cast<T*>(a.out) + seq * a.o_seq + head * a.o_head + (g0 + g) * a.o_group;
+      store_out(out + d, sum == 0.0f ? 0.0f : x / sum);
+      if (d == 0 && a.lse)
+        a.lse[r] = sum == 0.0f ? -INFINITY : (mx + log2f(sum)) * 0.6931471805599453f;
+    }
+  }
+}
+
+// ---------------------------------------------------------------- fp32
+
+// Values x[0 .. NV) summed over groups of L lanes, NV <= L: lane i of a group gets
+// the sum of x[i / (L / NV)]. Each round halves the values that a lane keeps and
+// hands its partner the rest, so NV sums cost NV - 1 shuffles and log2(L / NV) more.
+template <int L, int NV>
+__device__ __forceinline__ float sum_lanes(float (&x)[NV]) {
+  const int lane = lane_id();
+#pragma unroll
+  for (int n = NV, d = L / 2; n > 1; n >>= 1, d >>= 1) {
+    const bool up = lane & d;
+#pragma unroll
+    for (int i = 0; i < n / 2; i++) {
+      const float keep = up ? x[n / 2 + i] : x[i], give = up ? x[i] : x[n / 2 + i];
+      x[i] = keep + __shfl_xor_sync(0xffffffffu, give, d);
+    }
+  }
+#pragma unroll
+  for (int d = L / NV / 2; d > 0; d >>= 1) x[0] += __shfl_xor_sync(0xffffffffu, x[0], d);
+  return x[0];
+}
+
+template <int HD>
+struct FmaCfg {
+  static constexpr int kTok = 4;                           // keys of one tile
+  static constexpr int kStages = HD == 64 ? 6 : 4;
+  static constexpr int kTileBytes = kTok * HD * 4;         // K or V of one tile
+  static constexpr int kWarpBytes = kStages * 2 * kTileBytes;
+  static constexpr int kSmem = kPagedWarps * kWarpBytes;
+};
+
+// GT query rows of one (sequence, head) against the keys of one split, fp32:
+// products on the FMA pipe, which keeps all of their bits. Each warp takes tiles of
+// four keys through a ring of its own, as the bf16 kernel does. A group of HD / 4
+// lanes holds a key row, 16 bytes a lane: HD = 64 makes two groups, which take two
+// keys of a tile each. A tile's scores are summed over the lanes so that each lane
+// ends with one (key, query row) and takes one exponential; the weights come back
+// to all lanes through shared memory.
+template <int HD, int GT>
+__global__ void __launch_bounds__(kPagedThreads) paged_attention_fma_kernel(const PagedArgs a) {
+  using Cfg = FmaCfg<HD>;
+  constexpr int kLanes = HD / 4, kGroups = 32 / kLanes;
+  constexpr int kKeys = Cfg::kTok / kGroups;         // of a group
+  constexpr int NV = kKeys * GT, kDup = kLanes / NV; // lanes with the same score
+  static_assert(NV <= kLanes, "");
+  extern __shared__ __align__(128) char smem[];
+  __shared__ float sh_m[kPagedWarps][GT], sh_l[kPagedWarps][GT];
+  __shared__ __align__(16) float sh_p[kPagedWarps][Cfg::kTok * GT];
+  pdl_launch_dependents();   // the join waits for this kernel's end
+
+  const int tiles = (a.group + GT - 1) / GT;
+  const int split = blockIdx.x / tiles, g0 = (blockIdx.x - split * tiles) * GT;
+  const int g_n = min(GT, a.group - g0);
+  const int head = blockIdx.y, seq = blockIdx.z;
+  int first, end;
+  key_range(a, seq, &first, &end);
+  const int c0 = max(first, split * a.chunk), c1 = min(end, (split + 1) * a.chunk);
+  if (c0 >= c1 && a.splits > 1) return;   // the join skips it too
+
+  const int lane = lane_id(), w = warp_id(), sub = lane % kLanes, grp = lane / kLanes;
+  const float* kp = static_cast<const float*>(a.k) + head * a.head_stride;
+  const float* vp = static_cast<const float*>(a.v) + head * a.head_stride;
+  const int32_t* row = a.table + seq * a.ld_table;
+  char* ring = smem + w * Cfg::kWarpBytes;
+  const uint32_t ring_at = smem_u32(ring);
+
+  constexpr int kTurn = kPagedWarps * Cfg::kTok;   // keys of one turn of the warps
+  const int base = c0 + w * Cfg::kTok;
+  const int n_mine = base < c1 ? (c1 - base + kTurn - 1) / kTurn : 0;
+  // where key (tile i, lane % kTok) is, -1: nowhere
+  auto locate = [&](int i) -> int64_t {
+    const int t = base + i * kTurn + lane % Cfg::kTok;
+    return t < c1 ? key_at(a, row, t) : -1;
+  };
+  auto fetch = [&](int i, int64_t where) {
+    const uint32_t slot = ring_at + (i % Cfg::kStages) * 2 * Cfg::kTileBytes;
+#pragma unroll
+    for (int j = 0; j < kKeys; j++) {
+      const int r = j * kGroups + grp;
+      const int64_t at = __shfl_sync(0xffffffffu, where, r);
+      const uint32_t dst = slot + r * HD * 4 + sub * 16;
+      const int64_t from = at < 0 ? 0 : at + sub * 4;
+      cp_async16(dst, kp + from, at >= 0);
+      cp_async16(dst + Cfg::kTileBytes, vp + from, at >= 0);
+    }
+  };
+  int64_t next = n_mine > 0 ? locate(0) : -1;
+  uint32_t live[Cfg::kStages];   // bit r: key r of the tile in this slot is one
+#pragma unroll
+  for (int i = 0; i < Cfg::kStages - 1; i++) {
+    live[i] = __ballot_sync(0xffffffffu, next >= 0);
+    if (i < n_mine) fetch(i, next);
+    cp_async_commit();
+    next = i + 1 < n_mine ? locate(i + 1) : -1;
+  }
+
+  const float* q = static_cast<const float*>(a.q) + seq * a.q_seq + head * a.q_head;
+  float qr[GT][4], o[GT][4];
+#pragma unroll
+  for (int g = 0; g < GT; g++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      o[g][e] = 0.0f;
+      qr[g][e] = g < g_n ? q[(g0 + g) * a.q_group + sub * 4 + e] * a.scale_log2 : 0.0f;
+    }
+  // this lane's score: key my_r of the tile (r counts as the ring's rows), row my_g
+  const int my = sub / kDup, my_g = my % GT, my_r = my / GT * kGroups + grp;
+  float m = -INFINITY, l = 0.0f;   // of row my_g: the warp's reference, this lane's sum
+
+#pragma unroll 1
+  for (int i = 0; i < n_mine; i++) {
+    {
+      const int f = i + Cfg::kStages - 1;
+      __syncwarp();   // every lane has read the slot that is filled now
+      const uint32_t bits = __ballot_sync(0xffffffffu, next >= 0);
+      if (f < n_mine) fetch(f, next);
+      cp_async_commit();
+      next = f + 1 < n_mine ? locate(f + 1) : -1;
+      live[Cfg::kStages - 1] = bits;
+    }
+    cp_async_wait<Cfg::kStages - 1>();
+    __syncwarp();
+    const float4* kt = reinterpret_cast<const float4*>(
+        ring + (i % Cfg::kStages) * 2 * Cfg::kTileBytes);
+    const float4* vt = kt + Cfg::kTileBytes / 16;
+
+    float s[NV];
+#pragma unroll
+    for (int u = 0; u < kKeys; u++) {
+      const float4 k = kt[(u * kGroups + grp) * kLanes + sub];
+#pragma unroll
+      for (int g = 0; g < GT; g++)
+        s[u * GT + g] = fmaf(qr[g][3], k.w, fmaf(qr[g][2], k.z, fmaf(qr[g][1], k.y,
+                                                                    qr[g][0] * k.x)));
+    }
+    float x = sum_lanes<kLanes, NV>(s);
+    if (!(live[0] >> my_r & 1)) x = -INFINITY;
+    if (__any_sync(0xffffffffu, x > m + 8.0f)) {
+      // a new reference: the row's largest score so far, over keys and groups
+      float y = x;
+#pragma unroll
+      for (int d = kLanes / 2; d >= GT * kDup; d >>= 1)
+        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, d));
+      if (kGroups == 2) y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 16));
+      y = fmaxf(y, m);
+      const float f = m == -INFINITY ? 0.0f : fast_exp2(m - y);
+      m = y;
+      l *= f;
+#pragma unroll
+      for (int g = 0; g < GT; g++) {
+        const float fg = __shfl_sync(0xffffffffu, f, g * kDup);
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[g][e] *= fg;
+      }
+    }
+    x = fast_exp2(x - (m == -INFINITY ? 0.0f : m));
+    l += x;
+    if (kDup == 1 || sub % kDup == 0) sh_p[w][my_r * GT + my_g] = x;
+    __syncwarp();
+#pragma unroll
+    for (int u = 0; u < kKeys; u++) {
+      const int r = u * kGroups + grp;
+      const float4 v = vt[r * kLanes + sub];
+      float p[GT];
+      if constexpr (GT >= 4) {
+#pragma unroll
+        for (int g = 0; g < GT; g += 4)
+          *reinterpret_cast<float4*>(p + g) =
+              *reinterpret_cast<const float4*>(&sh_p[w][r * GT + g]);
+      } else {
+#pragma unroll
+        for (int g = 0; g < GT; g++) p[g] = sh_p[w][r * GT + g];
+      }
+#pragma unroll
+      for (int g = 0; g < GT; g++) {
+        o[g][0] = fmaf(p[g], v.x, o[g][0]);
+        o[g][1] = fmaf(p[g], v.y, o[g][1]);
+        o[g][2] = fmaf(p[g], v.z, o[g][2]);
+        o[g][3] = fmaf(p[g], v.w, o[g][3]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j + 1 < Cfg::kStages; j++) live[j] = live[j + 1];
+  }
+  // the row's sum over its keys' lanes and the groups
+#pragma unroll
+  for (int d = kLanes / 2; d >= GT * kDup; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+  if (kGroups == 2) {
+    l += __shfl_xor_sync(0xffffffffu, l, 16);
+#pragma unroll
+    for (int g = 0; g < GT; g++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) o[g][e] += __shfl_xor_sync(0xffffffffu, o[g][e], 16);
+  }
+  cp_async_wait<0>();
+  __syncthreads();   // the rings become the warps' parts of o
+
+  float* part = reinterpret_cast<float*>(smem);   // [warp][row][HD]
+  if (lane < kLanes) {
+#pragma unroll
+    for (int g = 0; g < GT; g++)
+      *reinterpret_cast<float4*>(part + (w * GT + g) * HD + sub * 4) =
+          make_float4(o[g][0], o[g][1], o[g][2], o[g][3]);
+    if (my_r == 0 && sub % kDup == 0) {
+      sh_m[w][my_g] = m;
+      sh_l[w][my_g] = l;
+    }
+  }
+  __syncthreads();
+  join_warps<float, HD, GT>(a, part, sh_m, sh_l, seq, head, split, g0, g_n);
+}
+
+// ---------------------------------------------------------------- tensor cores
+
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -248,7 +369,7 @@ constexpr int kTok = 16;   // keys of one tile
 
 template <int HD>
 struct MmaCfg {
-  static constexpr int kStages = HD == 64 ? 4 : 3;
+  static constexpr int kStages = 2;
   static constexpr int kTileBytes = kTok * HD * 2;               // K or V of one tile
   static constexpr int kWarpBytes = kStages * 2 * kTileBytes;
   static constexpr int kSmem = kPagedWarps * kWarpBytes;
@@ -297,14 +418,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_mma_kernel(cons
   // where key (tile i, lane % 16) is, -1: nowhere
   auto locate = [&](int i) -> int64_t {
     const int t = base + i * kPagedWarps * kTok + (lane & 15);
-    if (t < c0 || t >= c1) return -1;
-    const int slot = page_slot(a, t);
-    const int page = __ldg(row + slot);
-    if (page < 0 || page >= a.n_pages) {
-      atomicOr(&g_attend_err, WX_DEVERR_PAGE);
-      return -1;
-    }
-    return page * a.page_stride + (t - slot * a.page_size) * a.tok_stride;
+    return t >= c0 && t < c1 ? key_at(a, row, t) : -1;
   };
   // copies tile i (its keys at `where`) into its slot of the ring; returns which
   // keys have none
@@ -477,65 +591,73 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_mma_kernel(cons
       }
     }
   __syncthreads();
-  for (int i = threadIdx.x; i < g_n * HD; i += kPagedThreads) {
-    const int g = i / HD, d = i - g * HD;
-    float mx = -INFINITY;
-#pragma unroll
-    for (int u = 0; u < kPagedWarps; u++) mx = fmaxf(mx, sh_m[u][g]);
-    const float mu = mx == -INFINITY ? 0.0f : mx;
-    float sum = 0.0f, x = 0.0f;
-#pragma unroll
-    for (int u = 0; u < kPagedWarps; u++) {
-      const float f = fast_exp2(sh_m[u][g] - mu);
-      sum = fmaf(sh_l[u][g], f, sum);
-      x = fmaf(part[(u * kRows + g) * HD + d], f, x);
-    }
-    const int64_t r = ((int64_t)seq * a.n_heads + head) * a.group + g0 + g;
-    if (a.splits > 1) {
-      a.part_o[(r * a.splits + split) * HD + d] = x;
-      if (d == 0) a.part_ml[r * a.splits + split] = make_float2(mx, sum);
-    } else {
-      uint16_t* out = static_cast<uint16_t*>(a.out) + seq * a.o_seq + head * a.o_head +
-                      (g0 + g) * a.o_group;
-      out[d] = (uint16_t)bf16_bits<RND_RNE>(sum == 0.0f ? 0.0f : x / sum);
-      if (d == 0 && a.lse)
-        a.lse[r] = sum == 0.0f ? -INFINITY : (mx + log2f(sum)) * 0.6931471805599453f;
-    }
-  }
+  join_warps<uint16_t, HD, kRows>(a, part, sh_m, sh_l, seq, head, split, g0, g_n);
 }
 
-// One warp a query row: the parts of the splits that held keys, joined in order.
+constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32;
+
+// One CTA a query row: the parts of the splits that held keys, each warp's share of
+// them in turn, then the warps' in order.
 template <typename T, int HD>
-__global__ void __launch_bounds__(kPagedThreads) paged_attention_join_kernel(const PagedArgs a,
-                                                                             int64_t rows) {
-  pdl_wait();
-  const int64_t r = (int64_t)blockIdx.x * kPagedWarps + warp_id();
-  if (r >= rows) return;
+__global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(const PagedArgs a) {
   constexpr int N = HD / 32;
-  const int lane = lane_id();
+  __shared__ float sh[kJoinWarps], sh_o[kJoinWarps][HD];
+  const int64_t r = blockIdx.x;
+  const int lane = lane_id(), w = warp_id();
   const int g = (int)(r % a.group);
-  const int64_t sh = r / a.group;
-  const int head = (int)(sh % a.n_heads), seq = (int)(sh / a.n_heads);
+  const int64_t sh_row = r / a.group;
+  const int head = (int)(sh_row % a.n_heads), seq = (int)(sh_row / a.n_heads);
   int first, end;
   key_range(a, seq, &first, &end);
   const int s0 = first / a.chunk, s1 = first < end ? (end + a.chunk - 1) / a.chunk : s0;
+  const float2* ml = a.part_ml + r * a.splits;
+  pdl_wait();
+  auto over_warps = [&](float x, bool max) {   // every thread gets it
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+      const float y = __shfl_xor_sync(0xffffffffu, x, d);
+      x = max ? fmaxf(x, y) : x + y;
+    }
+    if (lane == 0) sh[w] = x;
+    __syncthreads();
+    x = sh[0];
+#pragma unroll
+    for (int u = 1; u < kJoinWarps; u++) x = max ? fmaxf(x, sh[u]) : x + sh[u];
+    __syncthreads();
+    return x;
+  };
   float mx = -INFINITY;
-  for (int s = s0; s < s1; s++) mx = fmaxf(mx, a.part_ml[r * a.splits + s].x);
+  for (int s = s0 + threadIdx.x; s < s1; s += kJoinThreads) mx = fmaxf(mx, ml[s].x);
+  mx = over_warps(mx, true);
   const float mu = mx == -INFINITY ? 0.0f : mx;
-  float sum = 0.0f, x[N] = {};
-  for (int s = s0; s < s1; s++) {
-    const float2 ml = a.part_ml[r * a.splits + s];
-    const float f = fast_exp2(ml.x - mu);
-    sum = fmaf(ml.y, f, sum);
-    const float* p = a.part_o + (r * a.splits + s) * HD;
+  float sum = 0.0f;
+  for (int s = s0 + threadIdx.x; s < s1; s += kJoinThreads)
+    sum = fmaf(ml[s].y, fast_exp2(ml[s].x - mu), sum);
+  sum = over_warps(sum, false);
+  float x[N] = {};
+  const float* p = a.part_o + r * a.splits * HD + lane * N;
+#pragma unroll 4
+  for (int s = s0 + w; s < s1; s += kJoinWarps) {
+    const float f = fast_exp2(ml[s].x - mu);
+    float y[N];
+    if constexpr (N == 4)
+      *reinterpret_cast<float4*>(y) = *reinterpret_cast<const float4*>(p + (int64_t)s * HD);
+    else
+      *reinterpret_cast<float2*>(y) = *reinterpret_cast<const float2*>(p + (int64_t)s * HD);
 #pragma unroll
-    for (int e = 0; e < N; e++) x[e] = fmaf(p[e * 32 + lane], f, x[e]);
+    for (int e = 0; e < N; e++) x[e] = fmaf(y[e], f, x[e]);
   }
-  T* out = static_cast<T*>(a.out) + seq * a.o_seq + head * a.o_head + g * a.o_group;
 #pragma unroll
-  for (int e = 0; e < N; e++)
-    store_out(out + e * 32 + lane, sum == 0.0f ? 0.0f : x[e] / sum);
-  if (lane == 0 && a.lse)
+  for (int e = 0; e < N; e++) sh_o[w][lane * N + e] = x[e];
+  __syncthreads();
+  if (threadIdx.x < HD) {
+    float y = 0.0f;
+#pragma unroll
+    for (int u = 0; u < kJoinWarps; u++) y += sh_o[u][threadIdx.x];
+    T* out = static_cast<T*>(a.out) + seq * a.o_seq + head * a.o_head + g * a.o_group;
+    store_out(out + threadIdx.x, sum == 0.0f ? 0.0f : y / sum);
+  }
+  if (threadIdx.x == 0 && a.lse)
     a.lse[r] = sum == 0.0f ? -INFINITY : (mx + log2f(sum)) * 0.6931471805599453f;
 }
 
@@ -569,30 +691,37 @@ static int64_t paged_space(int64_t rows, const PagedCut& c, int64_t head_dim) {
   return c.splits > 1 ? rows * c.splits * (head_dim * 4 + 8) : 0;
 }
 
-template <int HD, int NT>
-static cudaError_t run_mma(const PagedArgs& a, dim3 grid, cudaStream_t st) {
-  static std::atomic<uint64_t> done{0};   // bit: a device whose limit has been raised
+// Launches a kernel with `smem` bytes of dynamic shared memory, its limit raised on
+// the first call on each device.
+template <void (*kernel)(const PagedArgs)>
+static cudaError_t launch_paged(const PagedArgs& a, dim3 grid, int smem, cudaStream_t st) {
+  static std::atomic<uint64_t> done{0};   // a bit a device
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev >= 64 || !(done.load(std::memory_order_acquire) >> dev & 1)) {
-    e = cudaFuncSetAttribute(paged_attention_mma_kernel<HD, NT>,
-                             cudaFuncAttributeMaxDynamicSharedMemorySize, MmaCfg<HD>::kSmem);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
   }
-  return launch_k(paged_attention_mma_kernel<HD, NT>, grid, dim3(kPagedThreads),
-                  MmaCfg<HD>::kSmem, st, a);
+  return launch_k(kernel, grid, dim3(kPagedThreads), smem, st, a);
+}
+
+template <int HD>
+static cudaError_t run_mma(const PagedArgs& a, int tile, dim3 grid, cudaStream_t st) {
+  constexpr int smem = MmaCfg<HD>::kSmem;
+  return tile == 8 ? launch_paged<paged_attention_mma_kernel<HD, 1>>(a, grid, smem, st)
+                   : launch_paged<paged_attention_mma_kernel<HD, 2>>(a, grid, smem, st);
 }
 
 template <int HD>
 static cudaError_t run_fma(const PagedArgs& a, int tile, dim3 grid, cudaStream_t st) {
-  const dim3 block(kPagedThreads);
+  constexpr int smem = FmaCfg<HD>::kSmem;
   switch (tile) {
-    case 1: return launch_k(paged_attention_fma_kernel<HD, 1>, grid, block, 0, st, a);
-    case 2: return launch_k(paged_attention_fma_kernel<HD, 2>, grid, block, 0, st, a);
-    case 4: return launch_k(paged_attention_fma_kernel<HD, 4>, grid, block, 0, st, a);
-    default: return launch_k(paged_attention_fma_kernel<HD, 8>, grid, block, 0, st, a);
+    case 1: return launch_paged<paged_attention_fma_kernel<HD, 1>>(a, grid, smem, st);
+    case 2: return launch_paged<paged_attention_fma_kernel<HD, 2>>(a, grid, smem, st);
+    case 4: return launch_paged<paged_attention_fma_kernel<HD, 4>>(a, grid, smem, st);
+    default: return launch_paged<paged_attention_fma_kernel<HD, 8>>(a, grid, smem, st);
   }
 }
 
@@ -603,21 +732,21 @@ static cudaError_t run_paged(const PagedArgs& a, const PagedCut& c, int64_t n_se
   const dim3 grid((unsigned)(c.splits * tiles), (unsigned)a.n_heads, (unsigned)n_seqs);
   cudaError_t e;
   if constexpr (sizeof(T) == 2)
-    e = c.tile == 8 ? run_mma<HD, 1>(a, grid, st) : run_mma<HD, 2>(a, grid, st);
+    e = run_mma<HD>(a, c.tile, grid, st);
   else
     e = run_fma<HD>(a, c.tile, grid, st);
   if (e != cudaSuccess || c.splits == 1) return e;
   const int64_t rows = n_seqs * a.n_heads * a.group;
   PdlScope pdl(true);
   return launch_k(paged_attention_join_kernel<T, HD>,
-                  dim3((unsigned)((rows + kPagedWarps - 1) / kPagedWarps)), dim3(kPagedThreads),
-                  0, st, a, rows);
+                  dim3((unsigned)rows), dim3(kJoinThreads), 0, st, a);
 }
 
 static int check_cut(const char* what, int64_t n_seqs, int64_t n_heads, int64_t group,
                      int64_t head_dim, int64_t max_len) {
   if (n_seqs < 0 || n_seqs > 65535 || n_heads < 1 || n_heads > 65535 || group < 1 ||
-      group > 65535 || max_len < 0 || max_len > (1 << 30))
+      group > 65535 || n_seqs * n_heads * group > 0x7fffffff || max_len < 0 ||
+      max_len > (1 << 30))
     return fail(WX_ERR_INVALID,
                 "%s: bad shape: %lld sequences, %lld heads, group %lld, max_len %lld", what,
                 (long long)n_seqs, (long long)n_heads, (long long)group, (long long)max_len);
