@@ -1,4 +1,5 @@
-"""Build libwxb200.so from csrc/ for sm_100a, in the source tree.
+"""Build libwxb200.so from csrc/ for sm_100a, and the Python binding of its decoder
+operators (_decoder.so), in the source tree.
 
     python -m wxb200._build          (with whisper-xdna_b200/ on sys.path)
 
@@ -10,6 +11,7 @@ cudaGetDriverEntryPoint, so the library loads on machines without a GPU.
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -18,6 +20,7 @@ CSRC = PKG.parent / "csrc"
 ROOT = PKG.parents[1]
 BUILD = ROOT / "_build"
 LIB = PKG / "libwxb200.so"
+BINDING = PKG / "_decoder.so"
 SOURCES = ["capi.cu", "rowops.cu", "gemm.cu", "attention.cu", "encoder.cu", "noalloc.cu",
            "mel.cu", "quant.cu", "kvcache.cu", "paged_attention.cu", "score.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3",
@@ -66,11 +69,35 @@ def build(verbose=False, force=False):
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    build_binding(force)
     if verbose:
         for _, log in results:
             if log:
                 print(log)
     return LIB
+
+
+def build_binding(force=False):
+    """_decoder.so: csrc/decoder_binding.cpp against torch's headers, linked with
+    libwxb200.so beside it."""
+    src = CSRC / "decoder_binding.cpp"
+    newest = max(src.stat().st_mtime, (ROOT / "include" / "wxb200.h").stat().st_mtime)
+    if not force and BINDING.exists() and BINDING.stat().st_mtime > newest:
+        return
+    import torch
+    torch_dir = Path(torch.__file__).resolve().parent
+    cuda = Path(_nvcc()).resolve().parents[1] if os.path.isabs(_nvcc()) else Path("/usr/local/cuda")
+    includes = [torch_dir / "include", torch_dir / "include" / "torch" / "csrc" / "api" / "include",
+                cuda / "include", sysconfig.get_paths()["include"]]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++20", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           *(f"-I{p}" for p in includes), str(src), "-o", str(BINDING),
+           f"-L{LIB.parent}", f"-l:{LIB.name}", "-Wl,-rpath,$ORIGIN",
+           f"-L{torch_dir / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-lc10",
+           "-lc10_cuda"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on {src.name}:\n{r.stdout}\n{r.stderr}")
 
 
 if __name__ == "__main__":

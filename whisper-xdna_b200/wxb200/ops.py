@@ -7,7 +7,6 @@ buffers are accepted as they are -- the banded outputs of src/rowops.py:80-88
 and the per-head slices of a fused QKV buffer.
 """
 import ctypes
-import functools
 
 import torch
 
@@ -280,62 +279,21 @@ def log_mel(audio, n_mels=80, out=None):
 # ---------------------------------------------------------------- decoder operators
 # Paged key-value cache: pools of shape (pages, page, heads, head_dim) for a
 # layer, (layers, pages, page, heads, head_dim) for a whole cache, any strides
-# with head_dim contiguous (a head-major pool is passed transposed). The page
-# table is (n_seqs, width) int32, -1 past a sequence's last page.
-
-_KV_DTYPES = {torch.bfloat16: L.WX_DTYPE_BF16, torch.float32: L.WX_DTYPE_F32}
-
-# a decoder step calls these operators for every layer, so their checks are kept
-# to a few microseconds
-_raw_stream = torch._C._cuda_getCurrentRawStream
+# with head_dim contiguous (a head-major pool is passed transposed), bf16 or fp32.
+# The page table is (n_seqs, width) int32, -1 past a sequence's last page.
+# Arguments are checked, and outputs allocated, in _decoder.so.
 
 
-def _on(dev, name, t, dtype, shape):
-    """The address of t: on device `dev`, of dtype, contiguous, of the shape given."""
-    if (isinstance(t, torch.Tensor) and t.get_device() == dev and t.dtype is dtype
-            and t.shape == shape and t.is_contiguous()):
-        return t.data_ptr()
-    if not isinstance(t, torch.Tensor) or t.get_device() != dev:
-        raise ValueError(f"{name} must be a CUDA tensor on the device of the others")
-    raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)}, got "
-                     f"{t.dtype}, {tuple(t.shape)}, strides {t.stride()}")
+class _Unbuilt:
+    def __getattr__(self, name):
+        raise RuntimeError(f"wxb200/_decoder.so cannot be loaded ({_why}): build it with "
+                           "__graft_entry__.build() or `python -m wxb200._build`.")
 
 
-def _pools(k_cache, v_cache, dim):
-    """Checks a cache's two pools; returns (device, dtype code, shape, strides)."""
-    for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
-            raise ValueError(f"{name} must be a CUDA tensor")
-    dtype, shape, strides = k_cache.dtype, k_cache.shape, k_cache.stride()
-    if len(shape) != dim:
-        raise ValueError(f"the cache must have {dim} dimensions, got {len(shape)}")
-    if v_cache.dtype is not dtype or v_cache.shape != shape or v_cache.stride() != strides:
-        raise ValueError("k_cache and v_cache must have the same dtype, shape and strides")
-    code = _KV_DTYPES.get(dtype)
-    if code is None:
-        raise ValueError(f"cache dtype {dtype} not in {list(_KV_DTYPES)}")
-    if strides[-1] != 1:
-        raise ValueError("the cache's head_dim must be contiguous")
-    dev = k_cache.get_device()
-    if v_cache.get_device() != dev or dev != torch.cuda.current_device():
-        raise ValueError("the cache must be on the current CUDA device")
-    return dev, code, shape, strides
-
-
-def _rows(dev, table):
-    """(sequences, width, address) of a page table."""
-    shape = table.shape if isinstance(table, torch.Tensor) else ()
-    if len(shape) != 2 or shape[1] == 0:
-        raise ValueError("table must be a (n_seqs, width) tensor")
-    return shape[0], shape[1], _on(dev, "table", table, torch.int32, shape)
-
-
-@functools.lru_cache(maxsize=1024)
-def _attend_space(n_seqs, n_heads, group, head_dim, max_len, dtype):
-    n = L.lib().wx_paged_attention_workspace(n_seqs, n_heads, group, head_dim, max_len, dtype)
-    if n < 0:
-        L.check(n)
-    return n
+try:
+    from . import _decoder
+except ImportError as e:
+    _why, _decoder = e, _Unbuilt()
 
 
 def paged_attention(q, k_cache, v_cache, table, lens, scale=None, starts=None, max_len=None,
@@ -347,52 +305,11 @@ def paged_attention(q, k_cache, v_cache, table, lens, scale=None, starts=None, m
     (n_seqs, cache heads, group, head_dim) with any strides -- for beams over one
     clip's keys, x.view(clips, beams, heads, hd).transpose(1, 2). scale: default
     head_dim ** -0.5. max_len: an upper bound of lens, by default what the table
-    holds; a close one makes a better split. Returns out (q's shape and strides,
-    q's dtype), with return_lse also log sum_j e^(scale q.k_j), fp32, q's shape
-    without head_dim. A row without keys gives 0 and -inf."""
-    dev, dt, shape, st = _pools(k_cache, v_cache, 4)
-    n_pages, page, n_heads, hd = shape
-    n, width, table_p = _rows(dev, table)
-    lens_p = _on(dev, "lens", lens, torch.int32, (n,))
-    if not isinstance(q, torch.Tensor) or q.get_device() != dev or q.dtype is not k_cache.dtype:
-        raise ValueError("q must be a CUDA tensor on the cache's device, of its dtype")
-    qs, qt = q.shape, q.stride()
-    if len(qs) == 3:
-        group, rest = divmod(qs[1], n_heads)
-        if rest:
-            raise ValueError(f"{qs[1]} query heads are no multiple of {n_heads} cache heads")
-    elif len(qs) == 4:
-        group = qs[2]
-        if qs[1] != n_heads:
-            raise ValueError(f"q has {qs[1]} cache heads, the cache {n_heads}")
-    else:
-        raise ValueError("q must have 3 or 4 dimensions")
-    if qs[0] != n or qs[-1] != hd or qt[-1] != 1:
-        raise ValueError(f"q of shape {tuple(qs)} does not fit {n} sequences of head_dim {hd} "
-                         "(contiguous)")
-    if out is None:
-        out = torch.empty_like(q)
-    elif (out.shape != qs or out.dtype is not q.dtype or out.get_device() != dev
-          or out.stride(-1) != 1):
-        raise ValueError("out must be like q, with a contiguous head_dim")
-    ot = out.stride()
-    if len(qs) == 3:
-        qt, ot = (qt[0], qt[1] * group, qt[1]), (ot[0], ot[1] * group, ot[1])
-    if max_len is None:
-        max_len = width * page
-    starts_p = None if starts is None else _on(dev, "starts", starts, torch.int32, (n,))
-    lse = torch.empty(qs[:-1], dtype=torch.float32, device=q.device) if return_lse else None
-    space = _attend_space(n, n_heads, group, hd, max_len, dt)
-    ws = torch.empty(space, dtype=torch.uint8, device=q.device) if space else None
-    status = L.lib().wx_paged_attention(
-        q.data_ptr(), qt[0], qt[1], qt[2], k_cache.data_ptr(), v_cache.data_ptr(), st[0], st[1],
-        st[2], table_p, width, lens_p, starts_p, out.data_ptr(), ot[0], ot[1], ot[2],
-        lse.data_ptr() if return_lse else None, n, n_heads, group, hd, n_pages, page, max_len,
-        hd ** -0.5 if scale is None else float(scale), dt, ws.data_ptr() if space else None,
-        space, _raw_stream(dev))
-    if status:
-        L.check(status)
-    return (out, lse) if return_lse else out
+    holds. Returns out (q's shape, strides and dtype), with return_lse also
+    log sum_j e^(scale q.k_j), fp32, q's shape without head_dim. A row without keys
+    gives 0 and -inf."""
+    return _decoder.paged_attention(q, k_cache, v_cache, table, lens, scale, starts, max_len, out,
+                                    return_lse)
 
 
 def kv_append(k, v, k_cache, v_cache, table, lens, counts=None):
@@ -400,32 +317,7 @@ def kv_append(k, v, k_cache, v_cache, table, lens, counts=None):
     heads, head_dim) or, for one token each, (n_seqs, heads, head_dim), of the
     cache's dtype; row t < counts[i] (all if None) of sequence i goes to position
     lens[i] - counts[i] + t."""
-    dev, dt, shape, st = _pools(k_cache, v_cache, 4)
-    n_pages, page, n_heads, hd = shape
-    n, width, table_p = _rows(dev, table)
-    lens_p = _on(dev, "lens", lens, torch.int32, (n,))
-    for t, name in ((k, "k"), (v, "v")):
-        if (not isinstance(t, torch.Tensor) or t.get_device() != dev
-                or t.dtype is not k_cache.dtype):
-            raise ValueError(f"{name} must be a CUDA tensor on the cache's device, of its dtype")
-    ks, kt = k.shape, k.stride()
-    if v.shape != ks or v.stride() != kt:
-        raise ValueError("k and v must have the same shape and strides")
-    if len(ks) == 3:
-        ks, kt = (ks[0], 1, ks[1], ks[2]), (kt[0], 0, kt[1], kt[2])
-    if len(ks) != 4 or ks[0] != n or ks[2] != n_heads or ks[3] != hd or kt[3] != 1:
-        raise ValueError(f"k of shape {tuple(k.shape)} does not fit {n} sequences of {n_heads} "
-                         f"heads of {hd} (contiguous)")
-    counts_p = _on(dev, "counts", counts, torch.int32, (n,)) if counts is not None else None
-    L.check(L.lib().wx_kv_append(
-        k.data_ptr(), v.data_ptr(), kt[0], kt[1], kt[2], k_cache.data_ptr(), v_cache.data_ptr(),
-        st[0], st[1], st[2], table_p, width, lens_p, counts_p, n, ks[1], n_heads, hd, n_pages,
-        page, dt, _raw_stream(dev)))
-
-
-@functools.lru_cache(maxsize=1024)
-def _plan_space(n_seqs, n_pages):
-    return L.lib().wx_kv_workspace(n_seqs, n_pages)
+    _decoder.kv_append(k, v, k_cache, v_cache, table, lens, counts)
 
 
 def kv_fork(k_cache, v_cache, table, lens, refs, parents=None, grow=None):
@@ -438,43 +330,14 @@ def kv_fork(k_cache, v_cache, table, lens, refs, parents=None, grow=None):
     Returns new int32 tensors (table, lens, refs, grown, status): lens counts the
     tokens granted (grown), status is (pages left free, pages short). A sequence
     whose pages the pool does not hold is not grown."""
-    dev, dt, shape, st = _pools(k_cache, v_cache, 5)
-    n_layers, n_pages, page, n_heads, hd = shape
-    n, width, table_p = _rows(dev, table)
-    lens_p = _on(dev, "lens", lens, torch.int32, (n,))
-    refs_p = _on(dev, "refs", refs, torch.int32, (n_pages,))
-    parents_p = _on(dev, "parents", parents, torch.int32, (n,)) if parents is not None else None
-    grow_p = _on(dev, "grow", grow, torch.int32, (n,)) if grow is not None else None
-    space = _plan_space(n, n_pages)
-    on = table.device
-    new = (torch.empty_like(table), torch.empty_like(lens), torch.empty_like(refs),
-           torch.empty_like(lens), torch.empty(2, dtype=torch.int32, device=on))
-    ws = torch.empty(space, dtype=torch.uint8, device=on)
-    L.check(L.lib().wx_kv_fork(
-        k_cache.data_ptr(), v_cache.data_ptr(), n_layers, st[0], st[1], st[2], st[3], n_heads, hd,
-        n_pages, page, dt, table_p, lens_p, refs_p, parents_p, grow_p, n, width,
-        *(t.data_ptr() for t in new), ws.data_ptr(), space, _raw_stream(dev)))
-    return new
+    return _decoder.kv_fork(k_cache, v_cache, table, lens, refs, parents, grow)
 
 
 def kv_compact(k_cache, v_cache, table, refs):
     """Moves the pages in use to the front of the pool in all layers of a cache,
     with the fewest moves. Returns new int32 tensors (table, refs, status), status
     being (pages in use, pages moved)."""
-    dev, dt, shape, st = _pools(k_cache, v_cache, 5)
-    n_layers, n_pages, page, n_heads, hd = shape
-    n, width, table_p = _rows(dev, table)
-    refs_p = _on(dev, "refs", refs, torch.int32, (n_pages,))
-    space = _plan_space(n, n_pages)
-    on = table.device
-    new = (torch.empty_like(table), torch.empty_like(refs),
-           torch.empty(2, dtype=torch.int32, device=on))
-    ws = torch.empty(space, dtype=torch.uint8, device=on)
-    L.check(L.lib().wx_kv_compact(
-        k_cache.data_ptr(), v_cache.data_ptr(), n_layers, st[0], st[1], st[2], st[3], n_heads, hd,
-        n_pages, page, dt, table_p, refs_p, n, width, *(t.data_ptr() for t in new),
-        ws.data_ptr(), space, _raw_stream(dev)))
-    return new
+    return _decoder.kv_compact(k_cache, v_cache, table, refs)
 
 
 def token_logprobs(logits, tokens, top_k=0, temperature=1.0):
@@ -485,24 +348,4 @@ def token_logprobs(logits, tokens, top_k=0, temperature=1.0):
     likeliest tokens with their log probabilities, (rows, top_k) fp32 and int32,
     equal logits by the lowest token. A row that is all -inf scores -inf, with
     entropy 0."""
-    _mat(logits, "logits", (torch.bfloat16, torch.float32))
-    rows, vocab = logits.shape
-    dev = logits.get_device()
-    if dev != torch.cuda.current_device():
-        raise ValueError("logits must be on the current CUDA device")
-    tokens_p = _on(dev, "tokens", tokens, torch.int64, (rows,))
-    if not 0 <= top_k <= min(32, vocab):
-        raise ValueError(f"top_k {top_k} not in [0, min(32, vocabulary {vocab})]")
-    on = logits.device
-    logprob = torch.empty(rows, dtype=torch.float32, device=on)
-    entropy = torch.empty_like(logprob)
-    top = torch.empty((rows, top_k), dtype=torch.float32, device=on)
-    index = torch.empty_like(top, dtype=torch.int32)
-    status = L.lib().wx_token_logprobs(
-        logits.data_ptr(), _KV_DTYPES[logits.dtype], rows, vocab, logits.stride(0), tokens_p,
-        top_k, float(temperature), logprob.data_ptr(), entropy.data_ptr(),
-        top.data_ptr() if top_k else None, index.data_ptr() if top_k else None,
-        _raw_stream(dev))
-    if status:
-        L.check(status)
-    return logprob, entropy, top, index
+    return _decoder.token_logprobs(logits, tokens, top_k, temperature)
