@@ -7,6 +7,7 @@
 // A cache is two pools (K and V) of n_pages pages of page_size tokens for each
 // layer; a row of the page table names a sequence's pages in order, -1 past the
 // last. refs[p] counts the table entries that name page p; 0 is free.
+#include <atomic>
 #include <cstdint>
 
 #include "common.cuh"
@@ -41,14 +42,17 @@ struct AppendArgs {
   const int32_t* lens;
   const int32_t* counts;
   int n_tokens, n_heads, row_units;   // units of sizeof(U) bytes in one head's row
-  int page_size, width;
+  Div by_token, by_row, by_page;      // units of a token, units of a row, page_size
+  int width;
   int64_t n_pages;
 };
 
-// One thread moves units of sizeof(U) bytes: (token, head, unit) of sequence
-// blockIdx.y, K or V by blockIdx.z. Consecutive threads take consecutive units
-// of a row, so both sides are full lines. Bound by latency for one token (a
-// launch), by the memory's bandwidth for a prompt's or a clip's worth.
+constexpr int kAppendUnroll = 4;
+
+// A thread moves units of sizeof(U) bytes, kAppendUnroll of them in flight: (token,
+// head, unit) of sequence blockIdx.y, K or V by blockIdx.z. Consecutive threads take
+// consecutive units of a row, so both sides are full lines. Bound by latency for one
+// token (a launch), by the memory's bandwidth for a prompt's or a clip's worth.
 template <typename U>
 __global__ void __launch_bounds__(256) kv_append_kernel(const AppendArgs a) {
   const int seq = blockIdx.y;
@@ -60,23 +64,31 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const AppendArgs a) {
   const char* src = a.src[blockIdx.z] + seq * a.s_seq;
   char* dst = a.dst[blockIdx.z];
   const int32_t* row = a.table + seq * a.ld_table;
-  for (uint32_t i = blockIdx.x * blockDim.x + threadIdx.x; i < total;
-       i += gridDim.x * blockDim.x) {
-    const int t = (int)(i / per_token);
-    const int r = (int)(i - (uint32_t)t * per_token);
-    const int h = r / a.row_units, u = r - h * a.row_units;
-    const int pos = len - count + t;
-    const int slot = pos / a.page_size;
-    const int page = pos >= 0 && slot < a.width ? row[slot] : -1;
-    if (page < 0 || page >= a.n_pages) {
-      kv_error();
-      continue;
+  for (uint32_t i0 = blockIdx.x * blockDim.x * kAppendUnroll + threadIdx.x; i0 < total;
+       i0 += gridDim.x * blockDim.x * kAppendUnroll) {
+    U x[kAppendUnroll];
+    int64_t to[kAppendUnroll];
+#pragma unroll
+    for (int j = 0; j < kAppendUnroll; j++) {
+      const uint32_t i = i0 + j * blockDim.x;
+      to[j] = -1;
+      if (i >= total) continue;
+      const int t = a.by_token((int)i), r = (int)(i - (uint32_t)t * per_token);
+      const int h = a.by_row(r), u = r - h * a.row_units;
+      x[j] = *reinterpret_cast<const U*>(src + t * a.s_tok + h * a.s_head +
+                                         u * (int64_t)sizeof(U));
+      const int pos = len - count + t;
+      const int slot = a.by_page(max(pos, 0));
+      const int page = pos >= 0 && slot < a.width ? row[slot] : -1;
+      if (page < 0 || page >= a.n_pages)
+        kv_error();
+      else
+        to[j] = page * a.page_stride + (pos - slot * (int)a.by_page.d) * a.tok_stride +
+                h * a.head_stride + u * (int64_t)sizeof(U);
     }
-    const int in_page = pos - slot * a.page_size;
-    const U x = *reinterpret_cast<const U*>(src + t * a.s_tok + h * a.s_head +
-                                            u * (int64_t)sizeof(U));
-    *reinterpret_cast<U*>(dst + page * a.page_stride + in_page * a.tok_stride +
-                          h * a.head_stride + u * (int64_t)sizeof(U)) = x;
+#pragma unroll
+    for (int j = 0; j < kAppendUnroll; j++)
+      if (to[j] >= 0) *reinterpret_cast<U*>(dst + to[j]) = x[j];
   }
 }
 
@@ -93,26 +105,31 @@ __device__ __forceinline__ void cluster_sync() {
 }
 
 // Inclusive scan over the CTA's kPlanThreads values; *total gets their sum.
-// Every thread calls it; `part` is 32 words of shared memory.
+// Every thread calls it; `part` is 33 words of shared memory.
 __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* part, int64_t* total) {
   const int lane = lane_id(), w = warp_id();
+  auto warp_scan = [&](int64_t x) {
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += u;
-  }
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t u = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += u;
+    }
+    return x;
+  };
+  v = warp_scan(v);
   __syncthreads();   // the previous call's readers are done with part
-  if (lane == 31) part[w] = v;
+  if (lane == 31) part[w + 1] = v;
   __syncthreads();
-  int64_t before = 0, all = 0;
-  for (int i = 0; i < kPlanThreads / 32; i++) {
-    const int64_t p = part[i];
-    if (i < w) before += p;
-    all += p;
+  if (w == 0) {
+    const int64_t x = warp_scan(part[lane + 1]);
+    part[lane + 1] = x;
+    if (lane == 0) part[0] = 0;
   }
-  *total = all;
-  return v + before;
+  __syncthreads();
+  *total = part[32];
+  return v + part[w];
 }
+static_assert(kPlanThreads == 1024, "block_scan: a warp scans the warps' sums");
 
 // One page copy: the first n_tok tokens of page src, every layer and head.
 struct PageCopy {
@@ -124,6 +141,9 @@ struct PlanSpace {
   PageCopy* copies;     // max(n_seqs, n_pages)
   int32_t* list;        // n_pages: free pages or holes, ascending
   int32_t* remap;       // n_pages: where compaction moves a page
+  unsigned long long* keeper;   // n_pages: the longest sharer of a page to be written
+  int32_t* sharers;     // n_pages: how many share it, 0 before
+  int32_t* column;      // n_pages: its column + 1, 0: not to be written
   int64_t* scan;        // n_seqs: pages and copies asked for before this sequence
   int32_t* need;        // n_seqs: pages asked for, bit 30: one of them is a copy
   int32_t* seg;         // 3 * kPlanCtas counts
@@ -147,6 +167,9 @@ static int64_t plan_space(PlanSpace* p, void* base, int64_t n_seqs, int64_t n_pa
       take((int64_t)sizeof(PageCopy) * (n_seqs > n_pages ? n_seqs : n_pages)));
   s.list = reinterpret_cast<int32_t*>(take(4 * n_pages));
   s.remap = reinterpret_cast<int32_t*>(take(4 * n_pages));
+  s.keeper = reinterpret_cast<unsigned long long*>(take(8 * n_pages));
+  s.sharers = reinterpret_cast<int32_t*>(take(4 * n_pages));
+  s.column = reinterpret_cast<int32_t*>(take(4 * n_pages));
   s.scan = reinterpret_cast<int64_t*>(take(8 * n_seqs));
   s.need = reinterpret_cast<int32_t*>(take(4 * n_seqs));
   if (p) *p = s;
@@ -158,26 +181,73 @@ struct ForkArgs {
   int32_t *table_out, *lens_out, *refs_out, *grown, *status;
   PlanSpace ws;
   int n_seqs, width, page_size, n_pages;
+  Div by_page, by_width;   // page_size, width
 };
 
 constexpr int kNeedsCopy = 1 << 30;
+
+// The steps of a fork for one sequence or table entry, shared by its two forms.
+
+// sequence i's parent, -1: none
+__device__ __forceinline__ int fork_parent(const ForkArgs& a, int i) {
+  const int par = a.parents ? a.parents[i] : i;
+  if (par >= a.n_seqs) {
+    kv_error();
+    return -1;
+  }
+  return par < 0 ? -1 : par;
+}
+// the length it goes on from
+__device__ __forceinline__ int fork_length(const ForkArgs& a, int par) {
+  const int n = par < 0 ? 0 : a.lens[par];
+  const int64_t most = (int64_t)a.width * a.page_size;
+  if (n < 0 || n > most) {
+    kv_error();
+    return n < 0 ? 0 : (int)most;
+  }
+  return n;
+}
+// a row's entry in column c, `from` standing in the parent's row
+__device__ __forceinline__ int fork_entry(const ForkArgs& a, int from, int c, int now) {
+  if (c * a.page_size >= now) return -1;
+  if (from < 0 || from >= a.n_pages) {
+    kv_error();
+    return -1;
+  }
+  return from;
+}
+__device__ __forceinline__ void fork_refs(const ForkArgs& a, int32_t* refs, int was, int is) {
+  if (was == is) return;
+  if (was >= 0 && was < a.n_pages) atomicSub(refs + was, 1);
+  if (is >= 0) atomicAdd(refs + is, 1);
+}
+// the tokens that sequence i is to grow by, as far as its row has room
+__device__ __forceinline__ int fork_grow(const ForkArgs& a, int i, int now) {
+  const int g = a.grow ? a.grow[i] : 0;
+  return g > 0 && (int64_t)now + g <= (int64_t)a.width * a.page_size ? g : 0;
+}
+__device__ __forceinline__ unsigned long long keeper_rank(int now, int i) {
+  return ((unsigned long long)(uint32_t)now << 32) | (uint32_t)~i;
+}
 
 // Sequence i goes on as parents[i] did, with room for grow[i] more tokens:
 //   1 the lengths, and the reference counts as they were
 //   2 the rows of the page table; references given back and taken (integer
 //     atomics: the counts do not depend on their order)
-//   3 what each sequence asks for: pages for its new tokens, and one more where
-//     its last page is partly filled and another sequence refers to it too. Of
-//     the sequences that share such a page the longest (the first among equals)
-//     keeps it: what it writes lies past the others' lengths. The rest copy it.
-//     A page stands at the same place in the rows of all sequences that share
-//     it, so the sharers are found by comparing one column.
-//   4 the free pages in ascending order, and the running sum of the requests
-//   5 the k-th page asked for is the k-th free page; sequences past the pool's
+//   3 the partly filled last pages that are to be written and are shared
+//   4 their sharers: the longest (the first among equals) keeps the page, since
+//     what it writes lies past the others' lengths. A page stands at the same place
+//     in the rows of all sequences that share it.
+//   5 what each sequence asks for: pages for its new tokens, and one more where it
+//     has to copy a shared page
+//   6 the free pages in ascending order, and the running sum of the requests
+//   7 the k-th page asked for is the k-th free page; sequences past the pool's
 //     end are not grown
-// Integer work of a few bytes a page, bound by the latency of its phases.
+// Integer work of a few bytes a page, bound by the latency of its phases. This form
+// keeps its arrays in global memory, parted by a cluster's barrier: for tables that
+// do not fit one CTA's shared memory.
 __global__ void __launch_bounds__(kPlanThreads, 1) kv_fork_kernel(const ForkArgs a) {
-  __shared__ int64_t part[32];
+  __shared__ int64_t part[33];
   pdl_launch_dependents();
   const int cta = blockIdx.x;
   const int tid = cta * kPlanThreads + threadIdx.x;
@@ -185,79 +255,68 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_fork_kernel(const ForkArgs
   const int lane = lane_id(), gw = tid >> 5;
   constexpr int kWarps = kAll / 32;
   const int ps = a.page_size;
-  const int64_t capacity = (int64_t)a.width * ps;
 
   // 1
-  for (int p = tid; p < a.n_pages; p += kAll) a.refs_out[p] = a.refs[p];
-  for (int i = tid; i < a.n_seqs; i += kAll) {
-    const int par = a.parents ? a.parents[i] : i;
-    int now = 0;
-    if (par >= 0 && par < a.n_seqs) {
-      now = a.lens[par];
-      if (now < 0 || now > capacity) {
-        kv_error();
-        now = now < 0 ? 0 : (int)capacity;
-      }
-    } else if (par >= a.n_seqs) {
-      kv_error();
-    }
-    a.lens_out[i] = now;
+  for (int p = tid; p < a.n_pages; p += kAll) {
+    a.refs_out[p] = a.refs[p];
+    a.ws.keeper[p] = 0;
+    a.ws.sharers[p] = a.ws.column[p] = 0;
   }
+  for (int i = tid; i < a.n_seqs; i += kAll) a.lens_out[i] = fork_length(a, fork_parent(a, i));
   if (tid == 0) *a.ws.n_copies = 0;
   cluster_sync();
 
   // 2
   for (int i = gw; i < a.n_seqs; i += kWarps) {
-    const int par = a.parents ? a.parents[i] : i;
-    const int held = (__ldcg(a.lens_out + i) + ps - 1) / ps;
+    const int par = a.parents ? a.parents[i] : i, now = __ldcg(a.lens_out + i);
     const int32_t* from = a.table + (int64_t)(par >= 0 && par < a.n_seqs ? par : i) * a.width;
     const int32_t* old = a.table + (int64_t)i * a.width;
     int32_t* to = a.table_out + (int64_t)i * a.width;
     for (int c = lane; c < a.width; c += 32) {
-      const int was = old[c];
-      int is = c < held ? from[c] : -1;
-      if (is >= a.n_pages || (is < 0 && c < held)) {
-        kv_error();
-        is = -1;
-      }
+      const int is = fork_entry(a, from[c], c, now);
       to[c] = is;
-      if (was != is) {
-        if (was >= 0 && was < a.n_pages) atomicSub(a.refs_out + was, 1);
-        if (is >= 0) atomicAdd(a.refs_out + is, 1);
-      }
+      fork_refs(a, a.refs_out, old[c], is);
     }
   }
   cluster_sync();
 
   // 3
+  for (int i = tid; i < a.n_seqs; i += kAll) {
+    const int now = __ldcg(a.lens_out + i);
+    const int col = a.by_page(now);
+    if (now == col * ps || !fork_grow(a, i, now)) continue;
+    const int page = __ldcg(a.table_out + (int64_t)i * a.width + col);
+    if (page >= 0 && __ldcg(a.refs_out + page) > 1) atomicMax(a.ws.column + page, col + 1);
+  }
+  cluster_sync();
+
+  // 4
   for (int i = gw; i < a.n_seqs; i += kWarps) {
     const int now = __ldcg(a.lens_out + i);
-    const int grow = a.grow ? max(a.grow[i], 0) : 0;
-    const bool wants = grow > 0 && (int64_t)now + grow <= capacity;
-    int need = 0;
-    if (wants) {
-      const int col = now / ps;
-      need = (int)(((int64_t)now + grow + ps - 1) / ps) - (now + ps - 1) / ps;
-      if (now % ps) {
-        const int page = __ldcg(a.table_out + (int64_t)i * a.width + col);
-        const int refs = page >= 0 ? __ldcg(a.refs_out + page) : 0;
-        if (refs > 1) {
-          int mates = 0;
-          bool better = false;
-          for (int j = lane; j < a.n_seqs; j += 32) {
-            const int nj = __ldcg(a.lens_out + j);
-            if (nj > col * ps && __ldcg(a.table_out + (int64_t)j * a.width + col) == page) {
-              mates++;
-              better |= nj > now || (nj == now && j < i);
-            }
-          }
-          mates = __reduce_add_sync(0xffffffffu, mates);
-          better = __any_sync(0xffffffffu, better);
-          if (better || mates != refs) need = (need + 1) | kNeedsCopy;
-        }
-      }
+    for (int c = lane; c * ps < now; c += 32) {
+      const int page = __ldcg(a.table_out + (int64_t)i * a.width + c);
+      if (page < 0 || __ldcg(a.ws.column + page) != c + 1) continue;
+      atomicMax(a.ws.keeper + page, keeper_rank(now, i));
+      atomicAdd(a.ws.sharers + page, 1);
     }
-    if (lane == 0) a.ws.need[i] = need;
+  }
+  cluster_sync();
+
+  // 5
+  for (int i = tid; i < a.n_seqs; i += kAll) {
+    const int now = __ldcg(a.lens_out + i), grow = fork_grow(a, i, now);
+    int need = 0;
+    if (grow) {
+      const int col = a.by_page(now);
+      need = a.by_page(now + grow - 1) - a.by_page(now + ps - 1) + 1;
+      const int page = now != col * ps ? __ldcg(a.table_out + (int64_t)i * a.width + col) : -1;
+      const int refs = page >= 0 ? __ldcg(a.refs_out + page) : 0;
+      if (refs > 1 && (__ldcg(a.ws.keeper + page) != keeper_rank(now, i) ||
+                       __ldcg(a.ws.sharers + page) != refs ||
+                       __ldcg(a.ws.column + page) != col + 1))
+        need = (need + 1) | kNeedsCopy;
+    }
+    a.ws.need[i] = need;
   }
   const int seg = (a.n_pages + kPlanCtas - 1) / kPlanCtas;
   const int p0 = min(a.n_pages, cta * seg), p1 = min(a.n_pages, p0 + seg);
@@ -270,7 +329,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_fork_kernel(const ForkArgs
   }
   cluster_sync();
 
-  // 4
+  // 6
   int n_free = 0, base = 0;
   for (int c = 0; c < kPlanCtas; c++) {
     const int n = __ldcg(a.ws.seg + c);
@@ -297,21 +356,17 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_fork_kernel(const ForkArgs
     if (threadIdx.x == 0) {
       const int64_t asked = run >> 32;
       a.status[1] = (int)(asked > n_free ? asked - n_free : 0);
-      a.status[0] = n_free;   // less what phase 5 takes
+      a.status[0] = n_free;   // less what phase 7 takes
     }
   }
   cluster_sync();
 
-  // 5
+  // 7
   for (int i = gw; i < a.n_seqs; i += kWarps) {
-    const int now = __ldcg(a.lens_out + i);
-    const int grow = a.grow ? max(a.grow[i], 0) : 0;
-    const bool wants = grow > 0 && (int64_t)now + grow <= capacity;
-    const int asked = __ldcg(a.ws.need + i);
-    const int need = asked & ~kNeedsCopy;
-    const int64_t scan = __ldcg(a.ws.scan + i);
-    const int64_t before = scan >> 32;
-    const bool granted = wants && (need == 0 || before + need <= n_free);
+    const int now = __ldcg(a.lens_out + i), grow = fork_grow(a, i, now);
+    const int asked = __ldcg(a.ws.need + i), need = asked & ~kNeedsCopy;
+    const int64_t scan = __ldcg(a.ws.scan + i), before = scan >> 32;
+    const bool granted = grow && (need == 0 || before + need <= n_free);
     __syncwarp();
     if (lane == 0) {
       a.lens_out[i] = granted ? now + grow : now;
@@ -322,24 +377,162 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_fork_kernel(const ForkArgs
     int32_t* row = a.table_out + (int64_t)i * a.width;
     int64_t next = before;
     if (asked & kNeedsCopy) {
-      const int col = now / ps;
+      const int col = a.by_page(now);
       if (lane == 0) {
         const int src = __ldcg(row + col), dst = __ldcg(a.ws.list + next);
         atomicSub(a.refs_out + src, 1);
         a.refs_out[dst] = 1;
         row[col] = dst;
-        a.ws.copies[(int32_t)scan] = {src, dst, now % ps, 0};
+        a.ws.copies[(int32_t)scan] = {src, dst, now - col * ps, 0};
         atomicAdd(a.ws.n_copies, 1);
       }
       next++;
     }
     const int fresh = need - (asked & kNeedsCopy ? 1 : 0);
-    const int held = (now + ps - 1) / ps;
+    const int held = a.by_page(now + ps - 1);
     for (int c = lane; c < fresh; c += 32) {
       const int page = __ldcg(a.ws.list + next + c);
       row[held + c] = page;
       a.refs_out[page] = 1;
     }
+  }
+}
+
+// Words of shared memory that the one-CTA form of a fork takes.
+__host__ __device__ constexpr int64_t fork_words(int64_t n_seqs, int64_t width, int64_t n_pages) {
+  return 2 * n_seqs * width + 6 * n_pages + 4 * n_seqs + 2;
+}
+
+// The same plan by one CTA, its arrays in shared memory: a phase costs a barrier and
+// not a trip through L2.
+__global__ void __launch_bounds__(kPlanThreads, 1) kv_fork_cta_kernel(const ForkArgs a) {
+  extern __shared__ __align__(16) int32_t words[];
+  __shared__ int64_t part[33];
+  __shared__ int n_copies, taken;
+  pdl_launch_dependents();
+  const int tid = threadIdx.x;
+  const int n_entries = a.n_seqs * a.width, ps = a.page_size;
+  unsigned long long* keeper = reinterpret_cast<unsigned long long*>(words);   // n_pages
+  int32_t* refs = words + 2 * a.n_pages;
+  int32_t *sharers = refs + a.n_pages, *column = sharers + a.n_pages, *list = column + a.n_pages;
+  int32_t *is = list + a.n_pages, *was = is + n_entries;      // rows after and before
+  int32_t *len = was + n_entries, *need = len + a.n_seqs;
+  int32_t *pages_before = need + a.n_seqs, *copies_before = pages_before + a.n_seqs;
+
+  // 1: parents' rows as they stand, lengths, counts
+#pragma unroll 4
+  for (int e = tid; e < n_entries; e += kPlanThreads) {
+    const int i = a.by_width(e), par = a.parents ? a.parents[i] : i;
+    is[e] = a.table[par < 0 || par >= a.n_seqs ? e : e + (par - i) * a.width];
+    was[e] = a.table[e];
+  }
+#pragma unroll 4
+  for (int p = tid; p < a.n_pages; p += kPlanThreads) {
+    refs[p] = a.refs[p];
+    keeper[p] = 0;
+    sharers[p] = column[p] = 0;
+  }
+  for (int i = tid; i < a.n_seqs; i += kPlanThreads) len[i] = fork_length(a, fork_parent(a, i));
+  if (tid == 0) n_copies = taken = 0;
+  __syncthreads();
+
+  // 2
+  for (int e = tid; e < n_entries; e += kPlanThreads) {
+    const int i = a.by_width(e), page = fork_entry(a, is[e], e - i * a.width, len[i]);
+    is[e] = page;
+    fork_refs(a, refs, was[e], page);
+  }
+  __syncthreads();
+
+  // 3
+  for (int i = tid; i < a.n_seqs; i += kPlanThreads) {
+    const int now = len[i], col = a.by_page(now);
+    if (now == col * ps || !fork_grow(a, i, now)) continue;
+    const int page = is[i * a.width + col];
+    if (page >= 0 && refs[page] > 1) atomicMax(column + page, col + 1);
+  }
+  __syncthreads();
+
+  // 4
+  for (int e = tid; e < n_entries; e += kPlanThreads) {
+    const int page = is[e];
+    if (page < 0 || column[page] == 0) continue;
+    const int i = a.by_width(e);
+    if (column[page] != e - i * a.width + 1) continue;
+    atomicMax(keeper + page, keeper_rank(len[i], i));
+    atomicAdd(sharers + page, 1);
+  }
+  __syncthreads();
+
+  // 5 and 6: each thread a run of sequences and of pages
+  const int per = (a.n_seqs + kPlanThreads - 1) / kPlanThreads;
+  const int i0 = min(a.n_seqs, tid * per), i1 = min(a.n_seqs, i0 + per);
+  int64_t asked = 0;   // pages, and the copies among them in the low half
+  for (int i = i0; i < i1; i++) {
+    const int now = len[i], grow = fork_grow(a, i, now);
+    int n = 0;
+    if (grow) {
+      const int col = a.by_page(now);
+      n = a.by_page(now + grow - 1) - a.by_page(now + ps - 1) + 1;
+      const int page = now != col * ps ? is[i * a.width + col] : -1;
+      if (page >= 0 && refs[page] > 1 &&
+          (keeper[page] != keeper_rank(now, i) || sharers[page] != refs[page] ||
+           column[page] != col + 1))
+        n = (n + 1) | kNeedsCopy;
+    }
+    need[i] = n;
+    asked += ((int64_t)(n & ~kNeedsCopy) << 32) | (n & kNeedsCopy ? 1 : 0);
+  }
+  const int per_p = (a.n_pages + kPlanThreads - 1) / kPlanThreads;
+  const int p0 = min(a.n_pages, tid * per_p), p1 = min(a.n_pages, p0 + per_p);
+  int free = 0;
+  for (int p = p0; p < p1; p++) free += refs[p] == 0;
+  int64_t total, n_free;
+  int64_t at = block_scan(asked, part, &total) - asked;
+  for (int i = i0; i < i1; i++) {
+    pages_before[i] = (int)min(at >> 32, (int64_t)0x7fffffff);
+    copies_before[i] = (int)at;
+    at += ((int64_t)(need[i] & ~kNeedsCopy) << 32) | (need[i] & kNeedsCopy ? 1 : 0);
+  }
+  at = block_scan(free, part, &n_free) - free;
+  for (int p = p0; p < p1; p++)
+    if (refs[p] == 0) list[at++] = p;
+  __syncthreads();
+
+  // 7
+  for (int i = tid; i < a.n_seqs; i += kPlanThreads) {
+    const int now = len[i], grow = fork_grow(a, i, now);
+    const int n = need[i] & ~kNeedsCopy, copy = need[i] & kNeedsCopy ? 1 : 0;
+    const int before = pages_before[i];
+    const bool granted = grow && (n == 0 || (int64_t)before + n <= n_free);
+    a.lens_out[i] = granted ? now + grow : now;
+    if (a.grown) a.grown[i] = granted ? grow : 0;
+    if (!granted || n == 0) continue;
+    atomicAdd(&taken, n);
+    int32_t* row = is + i * a.width;
+    if (copy) {
+      const int col = a.by_page(now), src = row[col], dst = list[before];
+      atomicSub(refs + src, 1);
+      refs[dst] = 1;
+      row[col] = dst;
+      a.ws.copies[copies_before[i]] = {src, dst, now - col * ps, 0};
+      atomicAdd(&n_copies, 1);
+    }
+    const int held = a.by_page(now + ps - 1);
+    for (int c = 0; c < n - copy; c++) {
+      const int page = list[before + copy + c];
+      row[held + c] = page;
+      refs[page] = 1;
+    }
+  }
+  __syncthreads();
+  for (int e = tid; e < n_entries; e += kPlanThreads) a.table_out[e] = is[e];
+  for (int p = tid; p < a.n_pages; p += kPlanThreads) a.refs_out[p] = refs[p];
+  if (tid == 0) {
+    const int64_t pages = total >> 32;
+    *a.ws.n_copies = n_copies;
+    a.status[0] = (int)n_free - taken;
+    a.status[1] = (int)(pages > n_free ? pages - n_free : 0);
   }
 }
 
@@ -352,9 +545,10 @@ struct CompactArgs {
 };
 
 // The used pages past the first n_used go to the free ones among them, both in
-// ascending order: the fewest moves that leave the pool dense.
+// ascending order: the fewest moves that leave the pool dense. This form keeps its
+// arrays in global memory, for pools that do not fit one CTA's shared memory.
 __global__ void __launch_bounds__(kPlanThreads, 1) kv_compact_kernel(const CompactArgs a) {
-  __shared__ int64_t part[32];
+  __shared__ int64_t part[33];
   pdl_launch_dependents();
   const int cta = blockIdx.x;
   const int64_t tid = cta * kPlanThreads + threadIdx.x;
@@ -437,6 +631,70 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_compact_kernel(const Compa
   }
 }
 
+// Words of shared memory that the one-CTA form of a compaction takes.
+__host__ __device__ constexpr int64_t compact_words(int64_t n_pages) { return 4 * n_pages; }
+
+// The same by one CTA, its arrays in shared memory.
+__global__ void __launch_bounds__(kPlanThreads, 1) kv_compact_cta_kernel(const CompactArgs a) {
+  extern __shared__ __align__(16) int32_t words[];
+  __shared__ int64_t part[33];
+  pdl_launch_dependents();
+  const int tid = threadIdx.x;
+  int32_t *refs = words, *holes = refs + a.n_pages, *movers = holes + a.n_pages,
+          *remap = movers + a.n_pages;
+#pragma unroll 4
+  for (int p = tid; p < a.n_pages; p += kPlanThreads) refs[p] = a.refs[p];
+  __syncthreads();
+  // each thread a run of pages
+  const int per = (a.n_pages + kPlanThreads - 1) / kPlanThreads;
+  const int p0 = min(a.n_pages, tid * per), p1 = min(a.n_pages, p0 + per);
+  int n = 0;
+  for (int p = p0; p < p1; p++) n += refs[p] > 0;
+  int64_t total;
+  block_scan(n, part, &total);
+  const int n_used = (int)total;
+  int64_t both = 0;   // holes, and movers in the low half
+  for (int p = p0; p < p1; p++) {
+    if (p < n_used && refs[p] <= 0) both += 1ll << 32;
+    if (p >= n_used && refs[p] > 0) both += 1;
+  }
+  int64_t at = block_scan(both, part, &total) - both;
+  const int n_movers = (int)total;
+  for (int p = p0; p < p1; p++) {
+    if (p < n_used && refs[p] <= 0) {
+      holes[at >> 32] = p;
+      at += 1ll << 32;
+    }
+    if (p >= n_used && refs[p] > 0) movers[(int)at++] = p;
+  }
+  __syncthreads();
+  for (int m = tid; m < n_movers; m += kPlanThreads) {
+    const int src = movers[m], dst = holes[m];
+    a.ws.copies[m] = {src, dst, a.page_size, 0};
+    remap[src] = dst;
+    refs[dst] = refs[src];
+  }
+  if (tid == 0) {
+    a.status[0] = n_used;
+    a.status[1] = n_movers;
+    *a.ws.n_copies = n_movers;
+  }
+  __syncthreads();
+  for (int p = tid; p < a.n_pages; p += kPlanThreads)
+    a.refs_out[p] = p < n_used ? max(refs[p], 0) : 0;
+#pragma unroll 4
+  for (int64_t i = tid; i < a.n_entries; i += kPlanThreads) {
+    int page = a.table[i];
+    if (page >= a.n_pages || (page >= n_used && refs[page] <= 0)) {
+      kv_error();   // not a page, or one that the counts call free
+      page = -1;
+    } else if (page >= n_used) {
+      page = remap[page];
+    }
+    a.table_out[i] = page;
+  }
+}
+
 // ---------------------------------------------------------------- page copies
 
 struct CopyArgs {
@@ -445,6 +703,9 @@ struct CopyArgs {
   const int32_t* n_copies;
   int64_t layer_stride, page_stride, tok_stride, head_stride;   // bytes
   int n_layers, n_heads, row_chunks;   // 16-byte chunks of one head's row
+  Div by_row, by_head;                 // row_chunks, n_heads
+  int run;                             // a page's first `run` tokens are one run of memory,
+                                       // or any number of tokens if it is 1
   bool head_major;                     // a page is stored head by head
 };
 
@@ -466,23 +727,26 @@ __global__ void __launch_bounds__(kCopyThreads) kv_copy_kernel(const CopyArgs a)
     const char* src = pool + c.src * a.page_stride;
     char* dst = pool + c.dst * a.page_stride;
     const int n = c.n_tok * a.n_heads * a.row_chunks;
-    for (int i0 = 0; i0 < n; i0 += kCopyThreads * kCopyUnroll) {
+    const bool run = a.run == 1 || a.run == c.n_tok;
+    for (int i0 = threadIdx.x; i0 < n; i0 += kCopyThreads * kCopyUnroll) {
       uint4 x[kCopyUnroll];
       int64_t at[kCopyUnroll];
 #pragma unroll
       for (int j = 0; j < kCopyUnroll; j++) {
-        const int i = i0 + j * kCopyThreads + threadIdx.x;
-        const int r = i / a.row_chunks, k = i - r * a.row_chunks;
-        const int inner = a.head_major ? c.n_tok : a.n_heads;
-        const int hi = r / inner, lo = r - hi * inner;
-        const int t = a.head_major ? lo : hi, h = a.head_major ? hi : lo;
-        at[j] = t * a.tok_stride + h * a.head_stride + k * 16;
+        const int i = i0 + j * kCopyThreads;
+        at[j] = (int64_t)i * 16;
+        if (!run) {
+          const int r = a.by_row(i), k = i - r * a.row_chunks;
+          const int hi = a.head_major ? r / c.n_tok : a.by_head(r);
+          const int lo = r - hi * (a.head_major ? c.n_tok : a.n_heads);
+          const int t = a.head_major ? lo : hi, h = a.head_major ? hi : lo;
+          at[j] = t * a.tok_stride + h * a.head_stride + k * 16;
+        }
         if (i < n) x[j] = *reinterpret_cast<const uint4*>(src + at[j]);
       }
 #pragma unroll
       for (int j = 0; j < kCopyUnroll; j++)
-        if (i0 + j * kCopyThreads + (int)threadIdx.x < n)
-          *reinterpret_cast<uint4*>(dst + at[j]) = x[j];
+        if (i0 + j * kCopyThreads < n) *reinterpret_cast<uint4*>(dst + at[j]) = x[j];
     }
   }
 }
@@ -529,9 +793,30 @@ static cudaError_t launch_cluster(void (*kernel)(Args), const Args& a, cudaStrea
   return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
+// The one-CTA forms' bound: what one CTA reads before a cluster of eight overtakes it,
+// within its shared memory.
+constexpr int64_t kCtaEntries = 16384;
+constexpr int64_t kCtaWords = 220 * 1024 / 4;
+
+template <typename Args>
+static cudaError_t launch_cta(void (*kernel)(Args), std::atomic<uint64_t>& done, const Args& a,
+                              int64_t words, cudaStream_t st) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 64 || !(done.load(std::memory_order_acquire) >> dev & 1)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)(kCtaWords * 4));
+    if (e != cudaSuccess) return e;
+    if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
+  }
+  return launch_k(kernel, dim3(1), dim3(kPlanThreads), (size_t)words * 4, st, a);
+}
+
 struct Pool {
   void *k, *v;
-  int64_t n_layers, layer_stride, page_stride, tok_stride, head_stride, n_heads, head_dim;
+  int64_t n_layers, layer_stride, page_stride, tok_stride, head_stride, n_heads, head_dim,
+      page_size;
   int dtype;
 };
 
@@ -552,7 +837,14 @@ static int launch_copies(const char* what, const Pool& p, const PlanSpace& ws,
   a.n_layers = (int)p.n_layers;
   a.n_heads = (int)p.n_heads;
   a.row_chunks = (int)(p.head_dim * es / 16);
+  a.by_row = Div((uint32_t)a.row_chunks);
+  a.by_head = Div((uint32_t)a.n_heads);
   a.head_major = p.tok_stride < p.head_stride;
+  a.run = 0;
+  if (p.head_stride == p.head_dim && p.tok_stride == p.n_heads * p.head_dim)
+    a.run = 1;
+  else if (p.tok_stride == p.head_dim && p.head_stride == p.page_size * p.head_dim)
+    a.run = (int)p.page_size;
   const int64_t units = max_copies * p.n_layers * 2, most = (int64_t)sm_count() * 8;
   PdlScope pdl(true);
   WX_CUDA_TRY(launch_k(kv_copy_kernel, dim3((unsigned)(units < most ? units : most)),
@@ -616,7 +908,7 @@ int wx_kv_append(const void* k, const void* v, int64_t src_seq_stride, int64_t s
   a.counts = counts;
   a.n_tokens = (int)n_tokens;
   a.n_heads = (int)n_heads;
-  a.page_size = (int)page_size;
+  a.by_page = Div((uint32_t)page_size);
   a.width = (int)(ld_table < 0x7fffffff ? ld_table : 0x7fffffff);
   a.n_pages = n_pages;
   // 16 bytes a thread where the source rows allow it, else one element
@@ -624,8 +916,10 @@ int wx_kv_append(const void* k, const void* v, int64_t src_seq_stride, int64_t s
                       (int64_t)(uintptr_t)v) & 15);
   const int64_t unit = vec ? 16 : es;
   a.row_units = (int)(head_dim * es / unit);
+  a.by_row = Div((uint32_t)a.row_units);
+  a.by_token = Div((uint32_t)(a.row_units * a.n_heads));
   const int64_t units = n_tokens * n_heads * a.row_units;
-  const int64_t blocks = (units + 255) / 256;
+  const int64_t blocks = (units + 256 * kAppendUnroll - 1) / (256 * kAppendUnroll);
   const dim3 grid((unsigned)(blocks < 65536 ? blocks : 65536), (unsigned)n_seqs, 2);
   cudaStream_t st = as_stream(stream);
   if (vec)
@@ -658,8 +952,8 @@ int wx_kv_fork(void* k_cache, void* v_cache, int64_t n_layers, int64_t layer_str
     return fail(WX_ERR_INVALID, "kv_fork: NULL argument");
   if (table == table_out || lens == lens_out || refs == refs_out)
     return fail(WX_ERR_INVALID, "kv_fork: the new page table cannot be written over the old one");
-  if (n_heads * head_dim * page_size > 0x7fffffff || width * page_size > 0x7fffffff)
-    return fail(WX_ERR_INVALID, "kv_fork: a page or a sequence of over 2^31 - 1 elements or tokens");
+  if (n_heads * head_dim * page_size > 0x7fffffff || width * page_size > (1 << 30))
+    return fail(WX_ERR_INVALID, "kv_fork: a page of over 2^31 - 1 elements or a row of over 2^30 tokens");
   ForkArgs a = {};
   a.table = table;
   a.lens = lens;
@@ -676,12 +970,19 @@ int wx_kv_fork(void* k_cache, void* v_cache, int64_t n_layers, int64_t layer_str
   a.width = (int)width;
   a.page_size = (int)page_size;
   a.n_pages = (int)n_pages;
+  a.by_page = Div((uint32_t)page_size);
+  a.by_width = Div((uint32_t)width);
   cudaStream_t st = as_stream(stream);
-  WX_CUDA_TRY(launch_cluster(kv_fork_kernel, a, st));
+  const int64_t words = fork_words(n_seqs, width, n_pages);
+  static std::atomic<uint64_t> ready{0};
+  if (n_seqs * width <= kCtaEntries && words <= kCtaWords)
+    WX_CUDA_TRY(launch_cta(kv_fork_cta_kernel, ready, a, words, st));
+  else
+    WX_CUDA_TRY(launch_cluster(kv_fork_kernel, a, st));
   WX_TRY(check_launch("kv_fork"));
   if (!grow) return WX_OK;   // nothing is written, so nothing is copied
   const Pool p = {k_cache, v_cache, n_layers, layer_stride, page_stride, tok_stride,
-                  head_stride, n_heads, head_dim, dtype};
+                  head_stride, n_heads, head_dim, page_size, dtype};
   return launch_copies("kv_fork copies", p, a.ws, n_seqs, st);
 }
 
@@ -713,10 +1014,15 @@ int wx_kv_compact(void* k_cache, void* v_cache, int64_t n_layers, int64_t layer_
   a.page_size = (int)page_size;
   a.n_pages = (int)n_pages;
   cudaStream_t st = as_stream(stream);
-  WX_CUDA_TRY(launch_cluster(kv_compact_kernel, a, st));
+  const int64_t words = compact_words(n_pages);
+  static std::atomic<uint64_t> ready{0};
+  if (a.n_entries <= kCtaEntries && words <= kCtaWords)
+    WX_CUDA_TRY(launch_cta(kv_compact_cta_kernel, ready, a, words, st));
+  else
+    WX_CUDA_TRY(launch_cluster(kv_compact_kernel, a, st));
   WX_TRY(check_launch("kv_compact"));
   const Pool p = {k_cache, v_cache, n_layers, layer_stride, page_stride, tok_stride,
-                  head_stride, n_heads, head_dim, dtype};
+                  head_stride, n_heads, head_dim, page_size, dtype};
   return launch_copies("kv_compact copies", p, a.ws, n_pages / 2 + 1, st);
 }
 

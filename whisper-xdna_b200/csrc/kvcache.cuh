@@ -4,6 +4,23 @@
 
 namespace wx {
 
+// Division of n < 2^31 by an invariant d (Granlund and Montgomery, "Division by
+// invariant integers using multiplication", 1994): a multiply, an add and a shift
+// where the hardware's division takes some twenty instructions.
+struct Div {
+  uint32_t d, mul, shift;
+  Div() = default;
+  explicit Div(uint32_t by) : d(by), shift(0) {
+    while ((1ull << shift) < by) shift++;
+    mul = (uint32_t)((((1ull << shift) - by) << 32) / by + 1);
+  }
+#ifdef __CUDACC__
+  __device__ __forceinline__ int operator()(int n) const {
+    return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift);
+  }
+#endif
+};
+
 // Checks a pool's types, sizes, strides (elements) and alignment.
 int check_pool(const char* what, const void* k, const void* v, int64_t page_stride,
                int64_t tok_stride, int64_t head_stride, int64_t n_heads, int64_t head_dim,

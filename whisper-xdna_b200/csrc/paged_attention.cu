@@ -37,13 +37,9 @@ struct PagedArgs {
   int64_t page_stride, tok_stride, head_stride, ld_table;
   int64_t n_pages;
   int n_heads, group, page_size, max_len, splits, chunk;
-  uint32_t div_mul, div_shift;   // t / page_size = (umulhi(t, mul) + t) >> shift
+  Div by_page;            // page_size
   float scale_log2;       // scale * log2(e)
 };
-
-__device__ __forceinline__ int page_slot(const PagedArgs& a, int t) {
-  return (int)((__umulhi((uint32_t)t, a.div_mul) + (uint32_t)t) >> a.div_shift);
-}
 
 __device__ __forceinline__ void store_out(float* p, float x) { *p = x; }
 __device__ __forceinline__ void store_out(uint16_t* p, float x) {
@@ -67,7 +63,7 @@ constexpr int kPagedWarps = kPagedThreads / 32;
 // Where key t of the sequence with this row of the table is, in elements from the
 // head's first; -1: on no page.
 __device__ __forceinline__ int64_t key_at(const PagedArgs& a, const int32_t* row, int t) {
-  const int slot = page_slot(a, t);
+  const int slot = a.by_page(t);
   const int page = __ldg(row + slot);
   if (page < 0 || page >= a.n_pages) {
     atomicOr(&g_attend_err, WX_DEVERR_PAGE);
@@ -825,10 +821,7 @@ int wx_paged_attention(const void* q, int64_t q_seq_stride, int64_t q_head_strid
   a.max_len = (int)max_len;
   a.splits = c.splits;
   a.chunk = c.chunk;
-  // Granlund and Montgomery's division by an invariant, for t < 2^31
-  a.div_shift = 0;
-  while ((1ll << a.div_shift) < page_size) a.div_shift++;
-  a.div_mul = (uint32_t)((((1ull << a.div_shift) - page_size) << 32) / page_size + 1);
+  a.by_page = Div((uint32_t)page_size);
   a.scale_log2 = scale * 1.4426950408889634f;
   cudaStream_t st = as_stream(stream);
   if (dtype == WX_DTYPE_BF16)
