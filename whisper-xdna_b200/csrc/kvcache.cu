@@ -7,6 +7,7 @@
 // A cache is two pools (K and V) of n_pages pages of page_size tokens for each
 // layer; a row of the page table names a sequence's pages in order, -1 past the
 // last. refs[p] counts the table entries that name page p; 0 is free.
+#include <algorithm>
 #include <atomic>
 #include <cstdint>
 
@@ -703,51 +704,54 @@ struct CopyArgs {
   const int32_t* n_copies;
   int64_t layer_stride, page_stride, tok_stride, head_stride;   // bytes
   int n_layers, n_heads, row_chunks;   // 16-byte chunks of one head's row
-  Div by_row, by_head;                 // row_chunks, n_heads
+  int n_parts;                         // parts of kCopyPart chunks in a whole page
+  Div by_row, by_head, by_part;        // row_chunks, n_heads, n_parts
   int run;                             // a page's first `run` tokens are one run of memory,
                                        // or any number of tokens if it is 1
   bool head_major;                     // a page is stored head by head
 };
 
-constexpr int kCopyThreads = 256, kCopyUnroll = 4;
+constexpr int kCopyThreads = 256, kCopyUnroll = 8;
+constexpr int kCopyResident = 4;   // CTAs on an SM (registers)
 
-// One CTA a (copy, layer, K or V) at a time: the tokens of a page, 16 bytes a
-// thread, kCopyUnroll loads in flight before their stores. Source and target
-// pages are never the same page, nor is a target another copy's source: plans
-// copy pages in use to free ones. Bound by the memory's bandwidth, read + write.
-__global__ void __launch_bounds__(kCopyThreads) kv_copy_kernel(const CopyArgs a) {
+constexpr int kCopyPart = kCopyThreads * kCopyUnroll;   // 16-byte chunks
+
+// One CTA a part of a copy at a time, K or V of layer blockIdx.y / 2: 32 KiB of the page's tokens, 16
+// bytes a thread, kCopyUnroll loads in flight before their stores. Source and target
+// pages are never the same page, nor is a target another copy's source: plans copy
+// pages in use to free ones. Bound by the memory's bandwidth, read + write; whole
+// pages a CTA (20 to 64 KB) left a last round that few CTAs ran.
+__global__ void __launch_bounds__(kCopyThreads, kCopyResident) kv_copy_kernel(const CopyArgs a) {
   pdl_wait();   // the plan
-  const int64_t units = (int64_t)*a.n_copies * a.n_layers * 2;
-  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
-    const int which = (int)(u & 1);
-    const int64_t v = u >> 1;
-    const int layer = (int)(v % a.n_layers);
-    const PageCopy c = a.copies[v / a.n_layers];
+  const int which = blockIdx.y & 1, layer = blockIdx.y >> 1;
+  const int units = *a.n_copies * a.n_parts;   // at most the pool's pages * n_parts
+  for (int u = blockIdx.x; u < units; u += gridDim.x) {
+    const int item = a.by_part(u);
+    const PageCopy c = a.copies[item];
+    const int n = c.n_tok * a.n_heads * a.row_chunks;
+    const int i0 = (u - item * a.n_parts) * kCopyPart + threadIdx.x;
     char* pool = (which ? a.v : a.k) + layer * a.layer_stride;
     const char* src = pool + c.src * a.page_stride;
     char* dst = pool + c.dst * a.page_stride;
-    const int n = c.n_tok * a.n_heads * a.row_chunks;
     const bool run = a.run == 1 || a.run == c.n_tok;
-    for (int i0 = threadIdx.x; i0 < n; i0 += kCopyThreads * kCopyUnroll) {
-      uint4 x[kCopyUnroll];
-      int64_t at[kCopyUnroll];
+    uint4 x[kCopyUnroll];
+    int64_t at[kCopyUnroll];
 #pragma unroll
-      for (int j = 0; j < kCopyUnroll; j++) {
-        const int i = i0 + j * kCopyThreads;
-        at[j] = (int64_t)i * 16;
-        if (!run) {
-          const int r = a.by_row(i), k = i - r * a.row_chunks;
-          const int hi = a.head_major ? r / c.n_tok : a.by_head(r);
-          const int lo = r - hi * (a.head_major ? c.n_tok : a.n_heads);
-          const int t = a.head_major ? lo : hi, h = a.head_major ? hi : lo;
-          at[j] = t * a.tok_stride + h * a.head_stride + k * 16;
-        }
-        if (i < n) x[j] = *reinterpret_cast<const uint4*>(src + at[j]);
+    for (int j = 0; j < kCopyUnroll; j++) {
+      const int i = i0 + j * kCopyThreads;
+      at[j] = (int64_t)i * 16;
+      if (!run) {
+        const int r = a.by_row(i), k = i - r * a.row_chunks;
+        const int hi = a.head_major ? r / c.n_tok : a.by_head(r);
+        const int lo = r - hi * (a.head_major ? c.n_tok : a.n_heads);
+        const int t = a.head_major ? lo : hi, h = a.head_major ? hi : lo;
+        at[j] = t * a.tok_stride + h * a.head_stride + k * 16;
       }
-#pragma unroll
-      for (int j = 0; j < kCopyUnroll; j++)
-        if (i0 + j * kCopyThreads < n) *reinterpret_cast<uint4*>(dst + at[j]) = x[j];
+      if (i < n) x[j] = *reinterpret_cast<const uint4*>(src + at[j]);
     }
+#pragma unroll
+    for (int j = 0; j < kCopyUnroll; j++)
+      if (i0 + j * kCopyThreads < n) *reinterpret_cast<uint4*>(dst + at[j]) = x[j];
   }
 }
 
@@ -845,9 +849,13 @@ static int launch_copies(const char* what, const Pool& p, const PlanSpace& ws,
     a.run = 1;
   else if (p.tok_stride == p.head_dim && p.head_stride == p.page_size * p.head_dim)
     a.run = (int)p.page_size;
-  const int64_t units = max_copies * p.n_layers * 2, most = (int64_t)sm_count() * 8;
+  const int64_t chunks = p.page_size * p.n_heads * a.row_chunks;
+  a.n_parts = (int)((chunks + kCopyPart - 1) / kCopyPart);
+  a.by_part = Div((uint32_t)a.n_parts);
+  const int64_t units = max_copies * a.n_parts, y = 2 * p.n_layers;
+  const int64_t most = std::max<int64_t>(1, (int64_t)sm_count() * kCopyResident / y);
   PdlScope pdl(true);
-  WX_CUDA_TRY(launch_k(kv_copy_kernel, dim3((unsigned)(units < most ? units : most)),
+  WX_CUDA_TRY(launch_k(kv_copy_kernel, dim3((unsigned)std::min(units, most), (unsigned)y),
                        dim3(kCopyThreads), 0, st, a));
   return check_launch(what);
 }
@@ -855,7 +863,7 @@ static int launch_copies(const char* what, const Pool& p, const PlanSpace& ws,
 static int check_plan(const char* what, int64_t n_layers, int64_t layer_stride, int64_t es,
                       int64_t n_seqs, int64_t width, const void* ws, int64_t ws_bytes,
                       int64_t n_pages) {
-  if (n_layers < 1 || n_layers > 65536 || layer_stride < 0 || layer_stride * es % 16)
+  if (n_layers < 1 || n_layers > 32767 || layer_stride < 0 || layer_stride * es % 16)
     return fail(WX_ERR_INVALID, "%s: bad layers: %lld, stride %lld", what, (long long)n_layers,
                 (long long)layer_stride);
   if (n_seqs < 1 || n_seqs > (1 << 20) || width < 1 || width > 0x7fffffff)
