@@ -30,13 +30,17 @@ struct PagedArgs {
   const void *q, *k, *v;
   void* out;
   float* lse;             // (sequences, heads, group) or NULL
-  float* part_o;          // (rows, splits, head_dim): parts, where splits > 1
+  float* part_o;          // (rows, splits, head_dim): parts, where chunk > 0
   float2* part_ml;        // (rows, splits): maximum (log2 units) and sum
   const int32_t *table, *lens, *starts;
   int64_t q_seq, q_head, q_group, o_seq, o_head, o_group;   // elements
   int64_t page_stride, tok_stride, head_stride, ld_table;
   int64_t n_pages;
-  int n_heads, group, page_size, max_len, splits, chunk;
+  int n_seqs, n_heads, group, page_size, max_len, tiles;   // tiles: of a group's rows
+  // how the cache's length is split: chunk > 0: in chunks of that many keys, their
+  // parts joined by another kernel; else in `splits` even parts of each sequence's
+  // keys, by the CTAs of a cluster
+  int splits, chunk;
   Div by_page;            // page_size
   float scale_log2;       // scale * log2(e)
 };
@@ -86,36 +90,133 @@ __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// The warps' parts of ROWS query rows, (maximum, sum, o) in shared memory, joined
-// and written: the result where the cache's length is not split, else a part.
-template <typename T, int HD, int ROWS>
-__device__ __forceinline__ void join_warps(const PagedArgs& a, const float* part,
-                                           const float (&sh_m)[kPagedWarps][ROWS],
-                                           const float (&sh_l)[kPagedWarps][ROWS], int seq,
-                                           int head, int split, int g0, int g_n) {
-  for (int i = threadIdx.x; i < g_n * HD; i += kPagedThreads) {
+// What a CTA (WPI = 4: its four warps share an item) or a warp (WPI = 1: each has an
+// item of its own) works on: query rows [g0, g0 + g_n) of a (sequence, head), keys
+// [c0, c1).
+struct PagedItem {
+  int seq, head, split, g0, g_n, c0, c1;
+  bool any;   // false: there is no such item
+};
+
+template <int WPI, int ROWS, int TOK>
+__device__ __forceinline__ PagedItem paged_item(const PagedArgs& a) {
+  PagedItem t;
+  int tile;
+  if constexpr (WPI == 1) {
+    const int64_t i = (int64_t)blockIdx.x * kPagedWarps + warp_id();
+    const int64_t row = i / a.tiles;
+    tile = (int)(i - row * a.tiles);
+    t.seq = (int)(row / a.n_heads);
+    t.head = (int)(row - (int64_t)t.seq * a.n_heads);
+    t.split = 0;
+    t.any = t.seq < a.n_seqs;
+    if (!t.any) return t;
+  } else {
+    tile = blockIdx.x / a.splits;
+    t.split = blockIdx.x - tile * a.splits;
+    t.head = blockIdx.y;
+    t.seq = blockIdx.z;
+    t.any = true;
+  }
+  t.g0 = tile * ROWS;
+  t.g_n = min(ROWS, a.group - t.g0);
+  int first, end;
+  key_range(a, t.seq, &first, &end);
+  if (a.chunk > 0) {
+    t.c0 = max(first, t.split * a.chunk);
+    t.c1 = min(end, (t.split + 1) * a.chunk);
+  } else {
+    const int from = first / TOK * TOK;
+    const int n = max(end - from, 0);
+    const int per = ((n + TOK - 1) / TOK + a.splits - 1) / a.splits * TOK;
+    t.c0 = max(first, from + t.split * per);
+    t.c1 = min(end, from + (t.split + 1) * per);
+  }
+  return t;
+}
+
+template <int WPI>
+__device__ __forceinline__ void item_sync() {
+  if constexpr (WPI == 1)
+    __syncwarp();
+  else
+    __syncthreads();
+}
+
+__device__ __forceinline__ float peer_f32(const float* p, int rank) {
+  uint32_t r;
+  float v;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(r) : "memory");
+  return v;
+}
+
+// Parts of one query row's element joined: (maximum, sum, o) of `n` parts.
+struct Joined {
+  float m, l, o;
+  template <typename M, typename L, typename O>
+  __device__ __forceinline__ Joined(int n, M ms, L ls, O os) : m(-INFINITY), l(0.0f), o(0.0f) {
+#pragma unroll
+    for (int u = 0; u < n; u++) m = fmaxf(m, ms(u));
+    const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int u = 0; u < n; u++) {
+      const float f = fast_exp2(ms(u) - ref);
+      l = fmaf(ls(u), f, l);
+      o = fmaf(os(u), f, o);
+    }
+  }
+};
+
+// The item's warps' parts in shared memory, o as (warp, row, HD), joined and written:
+// as the result, as a part for the joining kernel, or over the cluster's CTAs. `mine`
+// (ROWS * (HD + 2) floats) is the CTA's own part in a cluster.
+template <typename T, int HD, int ROWS, int WPI>
+__device__ __forceinline__ void finish_item(const PagedArgs& a, const PagedItem& t,
+                                            const float* part, const float (*sh_m)[ROWS],
+                                            const float (*sh_l)[ROWS], float* mine) {
+  const int tid = threadIdx.x % (32 * WPI);
+  const int64_t row0 = ((int64_t)t.seq * a.n_heads + t.head) * a.group + t.g0;
+  T* out = static_cast<T*>(a.out) + t.seq * a.o_seq + t.head * a.o_head + t.g0 * a.o_group;
+  auto write = [&](int g, int d, const Joined& j) {
+    store_out(out + g * a.o_group + d, j.l == 0.0f ? 0.0f : j.o / j.l);
+    if (d == 0 && a.lse)
+      a.lse[row0 + g] = j.l == 0.0f ? -INFINITY : (j.m + log2f(j.l)) * 0.6931471805599453f;
+  };
+  for (int i = tid; i < t.g_n * HD; i += 32 * WPI) {
     const int g = i / HD, d = i - g * HD;
-    float mx = -INFINITY;
-#pragma unroll
-    for (int u = 0; u < kPagedWarps; u++) mx = fmaxf(mx, sh_m[u][g]);
-    const float mu = mx == -INFINITY ? 0.0f : mx;
-    float sum = 0.0f, x = 0.0f;
-#pragma unroll
-    for (int u = 0; u < kPagedWarps; u++) {
-      const float f = fast_exp2(sh_m[u][g] - mu);
-      sum = fmaf(sh_l[u][g], f, sum);
-      x = fmaf(part[(u * ROWS + g) * HD + d], f, x);
-    }
-    const int64_t r = ((int64_t)seq * a.n_heads + head) * a.group + g0 + g;
-    if (a.splits > 1) {
-      a.part_o[(r * a.splits + split) * HD + d] = x;
-      if (d == 0) a.part_ml[r * a.splits + split] = make_float2(mx, sum);
+    const Joined j(
+        WPI, [&](int u) { return sh_m[u][g]; }, [&](int u) { return sh_l[u][g]; },
+        [&](int u) { return part[(u * ROWS + g) * HD + d]; });
+    if (a.chunk > 0) {
+      a.part_o[((row0 + g) * a.splits + t.split) * HD + d] = j.o;
+      if (d == 0) a.part_ml[(row0 + g) * a.splits + t.split] = make_float2(j.m, j.l);
+    } else if (WPI > 1 && a.splits > 1) {
+      mine[g * HD + d] = j.o;
+      if (d == 0) {
+        mine[ROWS * HD + g] = j.m;
+        mine[ROWS * (HD + 1) + g] = j.l;
+      }
     } else {
-      T* out = static_cast<T*>(a.out) + seq * a.o_seq + head * a.o_head + (g0 + g) * a.o_group;
-      store_out(out + d, sum == 0.0f ? 0.0f : x / sum);
-      if (d == 0 && a.lse)
-        a.lse[r] = sum == 0.0f ? -INFINITY : (mx + log2f(sum)) * 0.6931471805599453f;
+      write(g, d, j);
     }
+  }
+  if (WPI > 1 && a.chunk == 0 && a.splits > 1) {
+    asm volatile(
+        "barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
+            : "memory");
+    // each CTA writes its share of the rows
+    for (int i = t.split * kPagedThreads + tid; i < t.g_n * HD; i += a.splits * kPagedThreads) {
+      const int g = i / HD, d = i - g * HD;
+      write(g, d,
+            Joined(
+                a.splits, [&](int u) { return peer_f32(mine + ROWS * HD + g, u); },
+                [&](int u) { return peer_f32(mine + ROWS * (HD + 1) + g, u); },
+                [&](int u) { return peer_f32(mine + g * HD + d, u); }));
+    }
+    // a CTA's shared memory outlives its readers: nothing is handed over
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::
+                     : "memory");
   }
 }
 
@@ -157,7 +258,7 @@ struct FmaCfg {
 // keys of a tile each. A tile's scores are summed over the lanes so that each lane
 // ends with one (key, query row) and takes one exponential; the weights come back
 // to all lanes through shared memory.
-template <int HD, int GT>
+template <int HD, int GT, int WPI>
 __global__ void __launch_bounds__(kPagedThreads) paged_attention_fma_kernel(const PagedArgs a) {
   using Cfg = FmaCfg<HD>;
   constexpr int kLanes = HD / 4, kGroups = 32 / kLanes;
@@ -169,14 +270,10 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_fma_kernel(cons
   __shared__ __align__(16) float sh_p[kPagedWarps][Cfg::kTok * GT];
   pdl_launch_dependents();   // the join waits for this kernel's end
 
-  const int tiles = (a.group + GT - 1) / GT;
-  const int split = blockIdx.x / tiles, g0 = (blockIdx.x - split * tiles) * GT;
-  const int g_n = min(GT, a.group - g0);
-  const int head = blockIdx.y, seq = blockIdx.z;
-  int first, end;
-  key_range(a, seq, &first, &end);
-  const int c0 = max(first, split * a.chunk), c1 = min(end, (split + 1) * a.chunk);
-  if (c0 >= c1 && a.splits > 1) return;   // the join skips it too
+  const PagedItem it = paged_item<WPI, GT, Cfg::kTok>(a);
+  // nothing to do; in a cluster the others still wait for this CTA
+  if (!it.any || (it.c0 >= it.c1 && a.chunk > 0)) return;
+  const int seq = it.seq, head = it.head, g0 = it.g0, g_n = it.g_n, c0 = it.c0, c1 = it.c1;
 
   const int lane = lane_id(), w = warp_id(), sub = lane % kLanes, grp = lane / kLanes;
   const float* kp = static_cast<const float*>(a.k) + head * a.head_stride;
@@ -185,8 +282,8 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_fma_kernel(cons
   char* ring = smem + w * Cfg::kWarpBytes;
   const uint32_t ring_at = smem_u32(ring);
 
-  constexpr int kTurn = kPagedWarps * Cfg::kTok;   // keys of one turn of the warps
-  const int base = c0 + w * Cfg::kTok;
+  constexpr int kTurn = WPI * Cfg::kTok;   // keys of one turn of the item's warps
+  const int base = c0 + w % WPI * Cfg::kTok;
   const int n_mine = base < c1 ? (c1 - base + kTurn - 1) / kTurn : 0;
   // where key (tile i, lane % kTok) is, -1: nowhere
   auto locate = [&](int i) -> int64_t {
@@ -314,21 +411,23 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_fma_kernel(cons
       for (int e = 0; e < 4; e++) o[g][e] += __shfl_xor_sync(0xffffffffu, o[g][e], 16);
   }
   cp_async_wait<0>();
-  __syncthreads();   // the rings become the warps' parts of o
+  item_sync<WPI>();   // the item's rings become its warps' parts of o
 
-  float* part = reinterpret_cast<float*>(smem);   // [warp][row][HD]
+  float* part = reinterpret_cast<float*>(smem + (WPI == 1 ? w * Cfg::kWarpBytes : 0));
+  float* my_part = part + w % WPI * GT * HD;
   if (lane < kLanes) {
 #pragma unroll
     for (int g = 0; g < GT; g++)
-      *reinterpret_cast<float4*>(part + (w * GT + g) * HD + sub * 4) =
+      *reinterpret_cast<float4*>(my_part + g * HD + sub * 4) =
           make_float4(o[g][0], o[g][1], o[g][2], o[g][3]);
     if (my_r == 0 && sub % kDup == 0) {
       sh_m[w][my_g] = m;
       sh_l[w][my_g] = l;
     }
   }
-  __syncthreads();
-  join_warps<float, HD, GT>(a, part, sh_m, sh_l, seq, head, split, g0, g_n);
+  item_sync<WPI>();
+  const int w0 = WPI == 1 ? w : 0;
+  finish_item<float, HD, GT, WPI>(a, it, part, sh_m + w0, sh_l + w0, part + WPI * GT * HD);
 }
 
 // ---------------------------------------------------------------- tensor cores
@@ -383,7 +482,7 @@ struct MmaCfg {
 // the four warps' parts are joined at the end. The rows' reference maximum moves
 // only when a score passes it by more than 2^8, so weights stay below 2^8 and
 // the rescaling is rare.
-template <int HD, int NT>
+template <int HD, int NT, int WPI>
 __global__ void __launch_bounds__(kPagedThreads) paged_attention_mma_kernel(const PagedArgs a) {
   using Cfg = MmaCfg<HD>;
   constexpr int kRows = 8 * NT, kSteps = HD / 16, kCpr = HD / 8;   // 16-byte chunks of a row
@@ -392,14 +491,10 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_mma_kernel(cons
   __shared__ float sh_m[kPagedWarps][kRows], sh_l[kPagedWarps][kRows];
   pdl_launch_dependents();   // the join waits for this kernel's end
 
-  const int tiles = (a.group + kRows - 1) / kRows;
-  const int split = blockIdx.x / tiles, g0 = (blockIdx.x - split * tiles) * kRows;
-  const int g_n = min(kRows, a.group - g0);
-  const int head = blockIdx.y, seq = blockIdx.z;
-  int first, end;
-  key_range(a, seq, &first, &end);
-  const int c0 = max(first, split * a.chunk), c1 = min(end, (split + 1) * a.chunk);
-  if (c0 >= c1 && a.splits > 1) return;   // the join skips it too
+  const PagedItem it = paged_item<WPI, kRows, kTok>(a);
+  // nothing to do; in a cluster the others still wait for this CTA
+  if (!it.any || (it.c0 >= it.c1 && a.chunk > 0)) return;
+  const int seq = it.seq, head = it.head, g0 = it.g0, g_n = it.g_n, c0 = it.c0, c1 = it.c1;
 
   const int lane = lane_id(), w = warp_id();
   const uint16_t* kp = static_cast<const uint16_t*>(a.k) + head * a.head_stride;
@@ -407,13 +502,14 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_mma_kernel(cons
   const int32_t* row = a.table + seq * a.ld_table;
   const uint32_t ring = smem_u32(smem) + w * Cfg::kWarpBytes;
 
-  // the warp's tiles: kTok keys from base + 4 kTok i on
-  const int base = c0 / kTok * kTok + w * kTok;
-  const int n_mine = base < c1 ? (c1 - base + kPagedWarps * kTok - 1) / (kPagedWarps * kTok) : 0;
+  // the warp's tiles: kTok keys from base + kTurn i on
+  constexpr int kTurn = WPI * kTok;
+  const int base = c0 / kTok * kTok + w % WPI * kTok;
+  const int n_mine = base < c1 ? (c1 - base + kTurn - 1) / kTurn : 0;
 
   // where key (tile i, lane % 16) is, -1: nowhere
   auto locate = [&](int i) -> int64_t {
-    const int t = base + i * kPagedWarps * kTok + (lane & 15);
+    const int t = base + i * kTurn + (lane & 15);
     return t >= c0 && t < c1 ? key_at(a, row, t) : -1;
   };
   // copies tile i (its keys at `where`) into its slot of the ring; returns which
@@ -564,9 +660,9 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_mma_kernel(cons
     for (int j = 0; j + 1 < Cfg::kStages; j++) live[j] = live[j + 1];
   }
   cp_async_wait<0>();
-  __syncthreads();   // the rings become the warps' parts of o
+  item_sync<WPI>();   // the item's rings become its warps' parts of o
 
-  float* part = reinterpret_cast<float*>(smem);   // [warp][row][HD]
+  float* part = reinterpret_cast<float*>(smem + (WPI == 1 ? w * Cfg::kWarpBytes : 0));
 #pragma unroll
   for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -579,21 +675,69 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_mma_kernel(cons
         sh_m[w][g] = m[n][h];
         sh_l[w][g] = sum;
       }
-      float* p = part + (w * kRows + g) * HD + (lane >> 2);
+      float* p = part + (w % WPI * kRows + g) * HD + (lane >> 2);
 #pragma unroll
       for (int k = 0; k < kSteps; k++) {
         p[k * 16] = o[n][k][h];
         p[k * 16 + 8] = o[n][k][2 + h];
       }
     }
-  __syncthreads();
-  join_warps<uint16_t, HD, kRows>(a, part, sh_m, sh_l, seq, head, split, g0, g_n);
+  item_sync<WPI>();
+  const int w0 = WPI == 1 ? w : 0;
+  finish_item<uint16_t, HD, kRows, WPI>(a, it, part, sh_m + w0, sh_l + w0,
+                                        part + WPI * kRows * HD);
 }
 
+// One warp a query row, for few splits: the parts of those that held keys, in order.
+template <typename T, int HD>
+__global__ void __launch_bounds__(kPagedThreads) paged_attention_join_few_kernel(
+    const PagedArgs a, int64_t rows) {
+  constexpr int N = HD / 32;
+  const int64_t r = (int64_t)blockIdx.x * kPagedWarps + warp_id();
+  if (r >= rows) return;
+  const int lane = lane_id();
+  const int g = (int)(r % a.group);
+  const int64_t sh_row = r / a.group;
+  const int head = (int)(sh_row % a.n_heads), seq = (int)(sh_row / a.n_heads);
+  int first, end;
+  key_range(a, seq, &first, &end);
+  const int s0 = first / a.chunk, s1 = first < end ? (end + a.chunk - 1) / a.chunk : s0;
+  const float2* ml = a.part_ml + r * a.splits;
+  pdl_wait();
+  // lane s - s0 holds split s (at most 32 of them)
+  const float2 my = s0 + lane < s1 ? ml[s0 + lane] : make_float2(-INFINITY, 0.0f);
+  float mx = my.x;
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+  const float f = fast_exp2(my.x - (mx == -INFINITY ? 0.0f : mx));
+  float sum = my.y * f;
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  float x[N] = {};
+  const float* p = a.part_o + r * a.splits * HD + lane * N;
+#pragma unroll 4
+  for (int s = s0; s < s1; s++) {
+    const float fs = __shfl_sync(0xffffffffu, f, s - s0);
+    float y[N];
+    if constexpr (N == 4)
+      *reinterpret_cast<float4*>(y) = *reinterpret_cast<const float4*>(p + (int64_t)s * HD);
+    else
+      *reinterpret_cast<float2*>(y) = *reinterpret_cast<const float2*>(p + (int64_t)s * HD);
+#pragma unroll
+    for (int e = 0; e < N; e++) x[e] = fmaf(y[e], fs, x[e]);
+  }
+  T* out = static_cast<T*>(a.out) + seq * a.o_seq + head * a.o_head + g * a.o_group + lane * N;
+#pragma unroll
+  for (int e = 0; e < N; e++) store_out(out + e, sum == 0.0f ? 0.0f : x[e] / sum);
+  if (lane == 0 && a.lse)
+    a.lse[r] = sum == 0.0f ? -INFINITY : (mx + log2f(sum)) * 0.6931471805599453f;
+}
+
+constexpr int kJoinFew = 32;   // splits that the warp form takes
 constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32;
 
-// One CTA a query row: the parts of the splits that held keys, each warp's share of
-// them in turn, then the warps' in order.
+// One CTA a query row, for many splits: each warp's share of them in turn, then the
+// warps' in order.
 template <typename T, int HD>
 __global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(const PagedArgs a) {
   constexpr int N = HD / 32;
@@ -657,85 +801,136 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(cons
     a.lse[r] = sum == 0.0f ? -INFINITY : (mx + log2f(sum)) * 0.6931471805599453f;
 }
 
-// How a call's work is cut: query rows a CTA takes, splits of the cache's length
-// and the tokens of one.
+// How a call's work is cut: query rows of a tile, warps on an item (1 or 4), and for
+// long caches chunks of keys that a second kernel joins. In between, a launch splits
+// an item over a cluster where that keeps every CTA in the first wave (launch_paged).
+//
+// Measured (B200): 6400 items of up to 224 keys, a warp each 27.8 us, a CTA each 34.7.
+// 320 items of 1500 keys, a cluster of 1, 2, 4, 8 for each: 27.3, 25.8, 31.0, 38.4 us
+// (two waves from 4 on; 3 CTAs, which divide no GPC: 33.0); 20 such items 20.3, 13.3,
+// 8.7, 7.3. 64 sequences to 16384 keys, chunks of at most 512, 1024, 2048: 98, 91, 95.
 struct PagedCut {
-  int tile, splits, chunk;
+  int tile, warps, splits, chunk;
 };
+constexpr int64_t kShortKeys = 256, kShortItems = 8 * 148;
+constexpr int64_t kClusterKeys = 4096;
+constexpr int64_t kMinChunk = 128, kMaxChunk = 1024, kChunkCtas = 4 * 148;
 
-static PagedCut paged_cut(int64_t n_seqs, int64_t n_heads, int64_t group, int64_t max_len,
-                          int dtype) {
-  PagedCut c;
+static PagedCut paged_cut(int64_t n_seqs, int64_t n_heads, int64_t group, int64_t head_dim,
+                          int64_t max_len, int dtype) {
+  PagedCut c = {};
   if (dtype == WX_DTYPE_BF16) {
     c.tile = group <= 8 ? 8 : 16;
   } else {
     c.tile = 1;
     while (c.tile < 8 && c.tile < group) c.tile *= 2;
   }
+  c.splits = 1;
+  c.warps = 4;
   const int64_t items = n_seqs * n_heads * ((group + c.tile - 1) / c.tile);
-  const int64_t want = 4 * 148;      // CTAs
-  int64_t chunk = max_len * items / want;
-  chunk = chunk < 128 ? 128 : chunk > 1024 ? 1024 : chunk;
-  chunk = (chunk + 63) / 64 * 64;
-  c.chunk = (int)chunk;
-  c.splits = (int)((max_len + chunk - 1) / chunk);
-  if (c.splits < 1) c.splits = 1;
+  if (max_len <= kShortKeys && items >= kShortItems) {
+    c.warps = 1;
+  } else if (max_len > kClusterKeys) {
+    int64_t chunk = max_len * items / kChunkCtas;
+    chunk = chunk < kMinChunk ? kMinChunk : chunk > kMaxChunk ? kMaxChunk : chunk;
+    chunk = (chunk + 63) / 64 * 64;
+    c.chunk = (int)chunk;
+    c.splits = (int)((max_len + chunk - 1) / chunk);
+  }
   return c;
 }
 
 static int64_t paged_space(int64_t rows, const PagedCut& c, int64_t head_dim) {
-  return c.splits > 1 ? rows * c.splits * (head_dim * 4 + 8) : 0;
+  return c.chunk > 0 ? rows * c.splits * (head_dim * 4 + 8) : 0;
 }
 
-// Launches a kernel with `smem` bytes of dynamic shared memory, its limit raised on
-// the first call on each device.
-template <void (*kernel)(const PagedArgs)>
-static cudaError_t launch_paged(const PagedArgs& a, dim3 grid, int smem, cudaStream_t st) {
-  static std::atomic<uint64_t> done{0};   // a bit a device
-  int dev = 0;
+// What a kernel needs to know of a device before its first launch there: its dynamic
+// shared memory's limit is raised, and the CTAs that are resident at once counted.
+static cudaError_t prepare_paged(std::atomic<int> (&resident)[64], const void* kernel, int smem,
+                                 int* ctas) {
+  int dev = 0, n = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  if (dev >= 64 || !(done.load(std::memory_order_acquire) >> dev & 1)) {
+  if (dev < 64) n = resident[dev].load(std::memory_order_acquire);
+  if (n == 0) {
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kPagedThreads, smem);
+    if (e != cudaSuccess) return e;
+    n = (n < 1 ? 1 : n) * sm_count();
+    if (dev < 64) resident[dev].store(n, std::memory_order_release);
   }
-  return launch_k(kernel, grid, dim3(kPagedThreads), smem, st, a);
+  *ctas = n;
+  return cudaSuccess;
+}
+
+template <void (*kernel)(const PagedArgs)>
+static cudaError_t launch_paged(PagedArgs a, const PagedCut& c, int smem, cudaStream_t st) {
+  static std::atomic<int> resident[64] = {};
+  int ctas = 0;
+  cudaError_t e = prepare_paged(resident, reinterpret_cast<const void*>(kernel), smem, &ctas);
+  if (e != cudaSuccess) return e;
+  const int64_t n_items = (int64_t)a.n_seqs * a.n_heads * a.tiles;
+  if (c.chunk == 0 && c.warps > 1)
+    while (a.splits < 8 && n_items * a.splits * 2 <= ctas && a.max_len >= 128 * a.splits)
+      a.splits *= 2;
+  if (c.warps == 1) {
+    return launch_k(kernel, dim3((unsigned)((n_items + kPagedWarps - 1) / kPagedWarps)),
+                    dim3(kPagedThreads), smem, st, a);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.splits * a.tiles), (unsigned)a.n_heads, (unsigned)a.n_seqs);
+  cfg.blockDim = dim3(kPagedThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  if (c.chunk == 0 && a.splits > 1) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)a.splits;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+  }
+  return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
 template <int HD>
-static cudaError_t run_mma(const PagedArgs& a, int tile, dim3 grid, cudaStream_t st) {
+static cudaError_t run_mma(const PagedArgs& a, const PagedCut& c, cudaStream_t st) {
   constexpr int smem = MmaCfg<HD>::kSmem;
-  return tile == 8 ? launch_paged<paged_attention_mma_kernel<HD, 1>>(a, grid, smem, st)
-                   : launch_paged<paged_attention_mma_kernel<HD, 2>>(a, grid, smem, st);
+  if (c.warps == 1)
+    return c.tile == 8 ? launch_paged<paged_attention_mma_kernel<HD, 1, 1>>(a, c, smem, st)
+                       : launch_paged<paged_attention_mma_kernel<HD, 2, 1>>(a, c, smem, st);
+  return c.tile == 8 ? launch_paged<paged_attention_mma_kernel<HD, 1, 4>>(a, c, smem, st)
+                     : launch_paged<paged_attention_mma_kernel<HD, 2, 4>>(a, c, smem, st);
 }
 
-template <int HD>
-static cudaError_t run_fma(const PagedArgs& a, int tile, dim3 grid, cudaStream_t st) {
+template <int HD, int WPI>
+static cudaError_t run_fma(const PagedArgs& a, const PagedCut& c, cudaStream_t st) {
   constexpr int smem = FmaCfg<HD>::kSmem;
-  switch (tile) {
-    case 1: return launch_paged<paged_attention_fma_kernel<HD, 1>>(a, grid, smem, st);
-    case 2: return launch_paged<paged_attention_fma_kernel<HD, 2>>(a, grid, smem, st);
-    case 4: return launch_paged<paged_attention_fma_kernel<HD, 4>>(a, grid, smem, st);
-    default: return launch_paged<paged_attention_fma_kernel<HD, 8>>(a, grid, smem, st);
+  switch (c.tile) {
+    case 1: return launch_paged<paged_attention_fma_kernel<HD, 1, WPI>>(a, c, smem, st);
+    case 2: return launch_paged<paged_attention_fma_kernel<HD, 2, WPI>>(a, c, smem, st);
+    case 4: return launch_paged<paged_attention_fma_kernel<HD, 4, WPI>>(a, c, smem, st);
+    default: return launch_paged<paged_attention_fma_kernel<HD, 8, WPI>>(a, c, smem, st);
   }
 }
 
 template <typename T, int HD>
-static cudaError_t run_paged(const PagedArgs& a, const PagedCut& c, int64_t n_seqs,
-                             cudaStream_t st) {
-  const int tiles = (a.group + c.tile - 1) / c.tile;
-  const dim3 grid((unsigned)(c.splits * tiles), (unsigned)a.n_heads, (unsigned)n_seqs);
+static cudaError_t run_paged(const PagedArgs& a, const PagedCut& c, cudaStream_t st) {
   cudaError_t e;
   if constexpr (sizeof(T) == 2)
-    e = run_mma<HD>(a, c.tile, grid, st);
+    e = run_mma<HD>(a, c, st);
   else
-    e = run_fma<HD>(a, c.tile, grid, st);
-  if (e != cudaSuccess || c.splits == 1) return e;
-  const int64_t rows = n_seqs * a.n_heads * a.group;
+    e = c.warps == 1 ? run_fma<HD, 1>(a, c, st) : run_fma<HD, 4>(a, c, st);
+  if (e != cudaSuccess || c.chunk == 0) return e;
+  const int64_t rows = (int64_t)a.n_seqs * a.n_heads * a.group;
   PdlScope pdl(true);
-  return launch_k(paged_attention_join_kernel<T, HD>,
-                  dim3((unsigned)rows), dim3(kJoinThreads), 0, st, a);
+  if (c.splits <= kJoinFew)
+    return launch_k(paged_attention_join_few_kernel<T, HD>,
+                    dim3((unsigned)((rows + kPagedWarps - 1) / kPagedWarps)),
+                    dim3(kPagedThreads), 0, st, a, rows);
+  return launch_k(paged_attention_join_kernel<T, HD>, dim3((unsigned)rows), dim3(kJoinThreads), 0,
+                  st, a);
 }
 
 static int check_cut(const char* what, int64_t n_seqs, int64_t n_heads, int64_t group,
@@ -761,7 +956,7 @@ int64_t wx_paged_attention_workspace(int64_t n_seqs, int64_t n_heads, int64_t gr
   using namespace wx;
   const int s = check_cut("paged_attention_workspace", n_seqs, n_heads, group, head_dim, max_len);
   if (s != WX_OK) return s;
-  return paged_space(n_seqs * n_heads * group, paged_cut(n_seqs, n_heads, group, max_len, dtype),
+  return paged_space(n_seqs * n_heads * group, paged_cut(n_seqs, n_heads, group, head_dim, max_len, dtype),
                      head_dim);
 }
 
@@ -787,7 +982,7 @@ int wx_paged_attention(const void* q, int64_t q_seq_stride, int64_t q_head_strid
   const int es = dtype == WX_DTYPE_BF16 ? 2 : 4;
   if (((uintptr_t)q | (uintptr_t)out) % es)
     return fail(WX_ERR_INVALID, "paged_attention: q or out not aligned to its type");
-  const PagedCut c = paged_cut(n_seqs, n_heads, group, max_len, dtype);
+  const PagedCut c = paged_cut(n_seqs, n_heads, group, head_dim, max_len, dtype);
   const int64_t rows = n_seqs * n_heads * group, want = paged_space(rows, c, head_dim);
   if (want && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < want))
     return fail(WX_ERR_INVALID,
@@ -819,16 +1014,17 @@ int wx_paged_attention(const void* q, int64_t q_seq_stride, int64_t q_head_strid
   a.group = (int)group;
   a.page_size = (int)page_size;
   a.max_len = (int)max_len;
+  a.n_seqs = (int)n_seqs;
+  a.tiles = (int)((group + c.tile - 1) / c.tile);
   a.splits = c.splits;
   a.chunk = c.chunk;
   a.by_page = Div((uint32_t)page_size);
   a.scale_log2 = scale * 1.4426950408889634f;
   cudaStream_t st = as_stream(stream);
   if (dtype == WX_DTYPE_BF16)
-    WX_CUDA_TRY((head_dim == 64 ? run_paged<uint16_t, 64> : run_paged<uint16_t, 128>)(a, c,
-                                                                                      n_seqs, st));
+    WX_CUDA_TRY((head_dim == 64 ? run_paged<uint16_t, 64> : run_paged<uint16_t, 128>)(a, c, st));
   else
-    WX_CUDA_TRY((head_dim == 64 ? run_paged<float, 64> : run_paged<float, 128>)(a, c, n_seqs, st));
+    WX_CUDA_TRY((head_dim == 64 ? run_paged<float, 64> : run_paged<float, 128>)(a, c, st));
   return check_launch("paged_attention");
 }
 
