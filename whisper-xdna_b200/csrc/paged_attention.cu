@@ -37,10 +37,12 @@ struct PagedArgs {
   int64_t page_stride, tok_stride, head_stride, ld_table;
   int64_t n_pages;
   int n_seqs, n_heads, group, page_size, max_len, tiles;   // tiles: of a group's rows
-  // how the cache's length is split: chunk > 0: in chunks of that many keys, their
-  // parts joined by another kernel; else in `splits` even parts of each sequence's
-  // keys, by the CTAs of a cluster
+  // how the cache's length is split: chunk > 0: in chunks of that many keys or more
+  // (pick_chunk), `splits` at most, their parts joined by another kernel; else in
+  // `splits` even parts of each sequence's keys, by the CTAs of a cluster
   int splits, chunk;
+  int slots;              // CTAs that are resident at once
+  int* picked;            // the chunk, for the joining kernel
   Div by_page;            // page_size
   float scale_log2;       // scale * log2(e)
 };
@@ -90,6 +92,31 @@ __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+constexpr int kMaxChunk = 1024;
+
+// The keys of a chunk: as many as make the calls' keys one wave of CTAs, within
+// [a.chunk, kMaxChunk]. The host sees only a bound of the lengths, often the table's
+// whole width: cut by that, 44 K keys of a 65 K window kept 342 CTAs on 444 places.
+// Every thread of a CTA calls it.
+__device__ __forceinline__ int pick_chunk(const PagedArgs& a) {
+  __shared__ int64_t sh_keys[kPagedWarps];
+  if (a.chunk == kMaxChunk) return a.chunk;
+  int64_t keys = 0;
+  if ((int)threadIdx.x < a.n_seqs) {
+    const int end = min(a.lens[threadIdx.x], a.max_len);
+    keys = max(end - (a.starts ? max(a.starts[threadIdx.x], 0) : 0), 0);
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) keys += __shfl_xor_sync(0xffffffffu, keys, d);
+  if (lane_id() == 0) sh_keys[warp_id()] = keys;
+  __syncthreads();
+  keys = 0;
+#pragma unroll
+  for (int u = 0; u < kPagedWarps; u++) keys += sh_keys[u];
+  const int64_t want = keys * a.n_heads * a.tiles / a.slots;
+  return (int)min(max(want + 15, (int64_t)a.chunk), (int64_t)kMaxChunk) / 16 * 16;
+}
+
 // What a CTA (WPI = 4: its four warps share an item) or a warp (WPI = 1: each has an
 // item of its own) works on: query rows [g0, g0 + g_n) of a (sequence, head), keys
 // [c0, c1).
@@ -122,9 +149,16 @@ __device__ __forceinline__ PagedItem paged_item(const PagedArgs& a) {
   t.g_n = min(ROWS, a.group - t.g0);
   int first, end;
   key_range(a, t.seq, &first, &end);
-  if (a.chunk > 0) {
-    t.c0 = max(first, t.split * a.chunk);
-    t.c1 = min(end, (t.split + 1) * a.chunk);
+  if (WPI > 1 && a.chunk > 0) {
+    t.c0 = t.c1 = 0;
+    if ((int64_t)t.split * a.chunk >= end) {   // empty whatever the chunk
+      t.any = t.split == 0 && t.seq == 0 && t.head == 0;
+      if (!t.any) return t;
+    }
+    const int chunk = pick_chunk(a);
+    if (t.seq == 0 && t.head == 0 && blockIdx.x == 0 && threadIdx.x == 0) *a.picked = chunk;
+    t.c0 = max(first, t.split * chunk);
+    t.c1 = min(end, (t.split + 1) * chunk);
   } else {
     const int from = first / TOK * TOK;
     const int n = max(end - from, 0);
@@ -245,7 +279,7 @@ __device__ __forceinline__ float sum_lanes(float (&x)[NV]) {
 template <int HD>
 struct FmaCfg {
   static constexpr int kTok = 4;                           // keys of one tile
-  static constexpr int kStages = HD == 64 ? 6 : 4;
+  static constexpr int kStages = HD == 64 ? 4 : 2;
   static constexpr int kTileBytes = kTok * HD * 4;         // K or V of one tile
   static constexpr int kWarpBytes = kStages * 2 * kTileBytes;
   static constexpr int kSmem = kPagedWarps * kWarpBytes;
@@ -312,14 +346,19 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_fma_kernel(cons
     next = i + 1 < n_mine ? locate(i + 1) : -1;
   }
 
+  // query rows in pairs, so that one packed FMA serves two of them (GT = 1: one row
+  // and a zero one)
+  constexpr int GP = (GT + 1) / 2;
   const float* q = static_cast<const float*>(a.q) + seq * a.q_seq + head * a.q_head;
-  float qr[GT][4], o[GT][4];
+  float2 qr[GP][4], o[GP][4];
 #pragma unroll
-  for (int g = 0; g < GT; g++)
+  for (int g = 0; g < GP; g++)
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      o[g][e] = 0.0f;
-      qr[g][e] = g < g_n ? q[(g0 + g) * a.q_group + sub * 4 + e] * a.scale_log2 : 0.0f;
+      o[g][e] = make_float2(0.0f, 0.0f);
+      const float* p = q + (g0 + 2 * g) * a.q_group + sub * 4 + e;
+      qr[g][e].x = 2 * g < g_n ? p[0] * a.scale_log2 : 0.0f;
+      qr[g][e].y = 2 * g + 1 < g_n ? p[a.q_group] * a.scale_log2 : 0.0f;
     }
   // this lane's score: key my_r of the tile (r counts as the ring's rows), row my_g
   const int my = sub / kDup, my_g = my % GT, my_r = my / GT * kGroups + grp;
@@ -346,10 +385,15 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_fma_kernel(cons
 #pragma unroll
     for (int u = 0; u < kKeys; u++) {
       const float4 k = kt[(u * kGroups + grp) * kLanes + sub];
+      const float kd[4] = {k.x, k.y, k.z, k.w};
 #pragma unroll
-      for (int g = 0; g < GT; g++)
-        s[u * GT + g] = fmaf(qr[g][3], k.w, fmaf(qr[g][2], k.z, fmaf(qr[g][1], k.y,
-                                                                    qr[g][0] * k.x)));
+      for (int g = 0; g < GP; g++) {
+        float2 x = __fmul2_rn(qr[g][0], make_float2(kd[0], kd[0]));
+#pragma unroll
+        for (int e = 1; e < 4; e++) x = __ffma2_rn(qr[g][e], make_float2(kd[e], kd[e]), x);
+        s[u * GT + 2 * g] = x.x;
+        if (GT > 1) s[u * GT + (2 * g + 1) % GT] = x.y;
+      }
     }
     float x = sum_lanes<kLanes, NV>(s);
     if (!(live[0] >> my_r & 1)) x = -INFINITY;
@@ -365,10 +409,11 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_fma_kernel(cons
       m = y;
       l *= f;
 #pragma unroll
-      for (int g = 0; g < GT; g++) {
-        const float fg = __shfl_sync(0xffffffffu, f, g * kDup);
+      for (int g = 0; g < GP; g++) {
+        const float2 fg = {__shfl_sync(0xffffffffu, f, 2 * g * kDup),
+                           __shfl_sync(0xffffffffu, f, (2 * g + 1) % GT * kDup)};
 #pragma unroll
-        for (int e = 0; e < 4; e++) o[g][e] *= fg;
+        for (int e = 0; e < 4; e++) o[g][e] = __fmul2_rn(o[g][e], fg);
       }
     }
     x = fast_exp2(x - (m == -INFINITY ? 0.0f : m));
@@ -379,23 +424,23 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_fma_kernel(cons
     for (int u = 0; u < kKeys; u++) {
       const int r = u * kGroups + grp;
       const float4 v = vt[r * kLanes + sub];
-      float p[GT];
+      const float vd[4] = {v.x, v.y, v.z, v.w};
+      float2 p[GP];
       if constexpr (GT >= 4) {
 #pragma unroll
-        for (int g = 0; g < GT; g += 4)
-          *reinterpret_cast<float4*>(p + g) =
-              *reinterpret_cast<const float4*>(&sh_p[w][r * GT + g]);
+        for (int g = 0; g < GP; g += 2) {
+          const float4 x = *reinterpret_cast<const float4*>(&sh_p[w][r * GT + 2 * g]);
+          p[g] = make_float2(x.x, x.y);
+          p[g + 1] = make_float2(x.z, x.w);
+        }
       } else {
-#pragma unroll
-        for (int g = 0; g < GT; g++) p[g] = sh_p[w][r * GT + g];
+        p[0] = make_float2(sh_p[w][r * GT], GT > 1 ? sh_p[w][r * GT + GT - 1] : 0.0f);
       }
 #pragma unroll
-      for (int g = 0; g < GT; g++) {
-        o[g][0] = fmaf(p[g], v.x, o[g][0]);
-        o[g][1] = fmaf(p[g], v.y, o[g][1]);
-        o[g][2] = fmaf(p[g], v.z, o[g][2]);
-        o[g][3] = fmaf(p[g], v.w, o[g][3]);
-      }
+      for (int g = 0; g < GP; g++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          o[g][e] = __ffma2_rn(p[g], make_float2(vd[e], vd[e]), o[g][e]);
     }
 #pragma unroll
     for (int j = 0; j + 1 < Cfg::kStages; j++) live[j] = live[j + 1];
@@ -406,9 +451,12 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_fma_kernel(cons
   if (kGroups == 2) {
     l += __shfl_xor_sync(0xffffffffu, l, 16);
 #pragma unroll
-    for (int g = 0; g < GT; g++)
+    for (int g = 0; g < GP; g++)
 #pragma unroll
-      for (int e = 0; e < 4; e++) o[g][e] += __shfl_xor_sync(0xffffffffu, o[g][e], 16);
+      for (int e = 0; e < 4; e++) {
+        o[g][e].x += __shfl_xor_sync(0xffffffffu, o[g][e].x, 16);
+        o[g][e].y += __shfl_xor_sync(0xffffffffu, o[g][e].y, 16);
+      }
   }
   cp_async_wait<0>();
   item_sync<WPI>();   // the item's rings become its warps' parts of o
@@ -417,9 +465,13 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_fma_kernel(cons
   float* my_part = part + w % WPI * GT * HD;
   if (lane < kLanes) {
 #pragma unroll
-    for (int g = 0; g < GT; g++)
-      *reinterpret_cast<float4*>(my_part + g * HD + sub * 4) =
-          make_float4(o[g][0], o[g][1], o[g][2], o[g][3]);
+    for (int g = 0; g < GP; g++) {
+      *reinterpret_cast<float4*>(my_part + 2 * g * HD + sub * 4) =
+          make_float4(o[g][0].x, o[g][1].x, o[g][2].x, o[g][3].x);
+      if (GT > 1)
+        *reinterpret_cast<float4*>(my_part + (2 * g + 1) * HD + sub * 4) =
+            make_float4(o[g][0].y, o[g][1].y, o[g][2].y, o[g][3].y);
+    }
     if (my_r == 0 && sub % kDup == 0) {
       sh_m[w][my_g] = m;
       sh_l[w][my_g] = l;
@@ -688,9 +740,10 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_mma_kernel(cons
                                         part + WPI * kRows * HD);
 }
 
-// One warp a query row, for few splits: the parts of those that held keys, in order.
+// One warp a query row, for many rows: the parts of the splits that held keys, in
+// order.
 template <typename T, int HD>
-__global__ void __launch_bounds__(kPagedThreads) paged_attention_join_few_kernel(
+__global__ void __launch_bounds__(kPagedThreads) paged_attention_join_rows_kernel(
     const PagedArgs a, int64_t rows) {
   constexpr int N = HD / 32;
   const int64_t r = (int64_t)blockIdx.x * kPagedWarps + warp_id();
@@ -701,31 +754,40 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_join_few_kernel
   const int head = (int)(sh_row % a.n_heads), seq = (int)(sh_row / a.n_heads);
   int first, end;
   key_range(a, seq, &first, &end);
-  const int s0 = first / a.chunk, s1 = first < end ? (end + a.chunk - 1) / a.chunk : s0;
   const float2* ml = a.part_ml + r * a.splits;
   pdl_wait();
-  // lane s - s0 holds split s (at most 32 of them)
-  const float2 my = s0 + lane < s1 ? ml[s0 + lane] : make_float2(-INFINITY, 0.0f);
+  const int chunk = a.chunk == kMaxChunk ? kMaxChunk : *a.picked;
+  const int s0 = first / chunk, s1 = first < end ? (end + chunk - 1) / chunk : s0;
+  // lane s - s32 holds split s
+  float2 my = s0 + lane < s1 ? ml[s0 + lane] : make_float2(-INFINITY, 0.0f);
   float mx = my.x;
+  for (int s = s0 + 32 + lane; s < s1; s += 32) mx = fmaxf(mx, ml[s].x);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-  const float f = fast_exp2(my.x - (mx == -INFINITY ? 0.0f : mx));
-  float sum = my.y * f;
+  const float mu = mx == -INFINITY ? 0.0f : mx;
+  float sum = 0.0f, x[N] = {};
+  const float* p = a.part_o + r * a.splits * HD + lane * N;
+  for (int s32 = s0; s32 < s1; s32 += 32) {
+    if (s32 > s0) my = s32 + lane < s1 ? ml[s32 + lane] : make_float2(-INFINITY, 0.0f);
+    const float f = fast_exp2(my.x - mu);
+    sum = fmaf(my.y, f, sum);
+    const int n = min(32, s1 - s32);
+#pragma unroll 4
+    for (int s = 0; s < n; s++) {
+      const float fs = __shfl_sync(0xffffffffu, f, s);
+      float y[N];
+      if constexpr (N == 4)
+        *reinterpret_cast<float4*>(y) =
+            *reinterpret_cast<const float4*>(p + (int64_t)(s32 + s) * HD);
+      else
+        *reinterpret_cast<float2*>(y) =
+            *reinterpret_cast<const float2*>(p + (int64_t)(s32 + s) * HD);
+#pragma unroll
+      for (int e = 0; e < N; e++) x[e] = fmaf(y[e], fs, x[e]);
+    }
+  }
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-  float x[N] = {};
-  const float* p = a.part_o + r * a.splits * HD + lane * N;
-#pragma unroll 4
-  for (int s = s0; s < s1; s++) {
-    const float fs = __shfl_sync(0xffffffffu, f, s - s0);
-    float y[N];
-    if constexpr (N == 4)
-      *reinterpret_cast<float4*>(y) = *reinterpret_cast<const float4*>(p + (int64_t)s * HD);
-    else
-      *reinterpret_cast<float2*>(y) = *reinterpret_cast<const float2*>(p + (int64_t)s * HD);
-#pragma unroll
-    for (int e = 0; e < N; e++) x[e] = fmaf(y[e], fs, x[e]);
-  }
   T* out = static_cast<T*>(a.out) + seq * a.o_seq + head * a.o_head + g * a.o_group + lane * N;
 #pragma unroll
   for (int e = 0; e < N; e++) store_out(out + e, sum == 0.0f ? 0.0f : x[e] / sum);
@@ -733,10 +795,10 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_join_few_kernel
     a.lse[r] = sum == 0.0f ? -INFINITY : (mx + log2f(sum)) * 0.6931471805599453f;
 }
 
-constexpr int kJoinFew = 32;   // splits that the warp form takes
-constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32;
+constexpr int64_t kJoinRows = 8 * 148;   // rows from which on a warp each will do
+constexpr int kJoinThreads = 1024, kJoinWarps = kJoinThreads / 32;
 
-// One CTA a query row, for many splits: each warp's share of them in turn, then the
+// One CTA a query row, for few rows: each warp's share of them in turn, then the
 // warps' in order.
 template <typename T, int HD>
 __global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(const PagedArgs a) {
@@ -749,9 +811,10 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(cons
   const int head = (int)(sh_row % a.n_heads), seq = (int)(sh_row / a.n_heads);
   int first, end;
   key_range(a, seq, &first, &end);
-  const int s0 = first / a.chunk, s1 = first < end ? (end + a.chunk - 1) / a.chunk : s0;
   const float2* ml = a.part_ml + r * a.splits;
   pdl_wait();
+  const int chunk = a.chunk == kMaxChunk ? kMaxChunk : *a.picked;
+  const int s0 = first / chunk, s1 = first < end ? (end + chunk - 1) / chunk : s0;
   auto over_warps = [&](float x, bool max) {   // every thread gets it
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) {
@@ -814,7 +877,7 @@ struct PagedCut {
 };
 constexpr int64_t kShortKeys = 256, kShortItems = 8 * 148;
 constexpr int64_t kClusterKeys = 4096;
-constexpr int64_t kMinChunk = 128, kMaxChunk = 1024, kChunkCtas = 4 * 148;
+constexpr int64_t kMinChunk = 128, kChunkCtas = 32 * 148;
 
 static PagedCut paged_cut(int64_t n_seqs, int64_t n_heads, int64_t group, int64_t head_dim,
                           int64_t max_len, int dtype) {
@@ -833,7 +896,8 @@ static PagedCut paged_cut(int64_t n_seqs, int64_t n_heads, int64_t group, int64_
   } else if (max_len > kClusterKeys) {
     int64_t chunk = max_len * items / kChunkCtas;
     chunk = chunk < kMinChunk ? kMinChunk : chunk > kMaxChunk ? kMaxChunk : chunk;
-    chunk = (chunk + 63) / 64 * 64;
+    if (n_seqs > kPagedThreads) chunk = kMaxChunk;   // pick_chunk leaves it at that
+    chunk = (chunk + 15) / 16 * 16;
     c.chunk = (int)chunk;
     c.splits = (int)((max_len + chunk - 1) / chunk);
   }
@@ -841,7 +905,7 @@ static PagedCut paged_cut(int64_t n_seqs, int64_t n_heads, int64_t group, int64_
 }
 
 static int64_t paged_space(int64_t rows, const PagedCut& c, int64_t head_dim) {
-  return c.chunk > 0 ? rows * c.splits * (head_dim * 4 + 8) : 0;
+  return c.chunk > 0 ? 16 + rows * c.splits * (head_dim * 4 + 8) : 0;
 }
 
 // What a kernel needs to know of a device before its first launch there: its dynamic
@@ -870,6 +934,7 @@ static cudaError_t launch_paged(PagedArgs a, const PagedCut& c, int smem, cudaSt
   int ctas = 0;
   cudaError_t e = prepare_paged(resident, reinterpret_cast<const void*>(kernel), smem, &ctas);
   if (e != cudaSuccess) return e;
+  a.slots = ctas;
   const int64_t n_items = (int64_t)a.n_seqs * a.n_heads * a.tiles;
   if (c.chunk == 0 && c.warps > 1)
     while (a.splits < 8 && n_items * a.splits * 2 <= ctas && a.max_len >= 128 * a.splits)
@@ -925,8 +990,8 @@ static cudaError_t run_paged(const PagedArgs& a, const PagedCut& c, cudaStream_t
   if (e != cudaSuccess || c.chunk == 0) return e;
   const int64_t rows = (int64_t)a.n_seqs * a.n_heads * a.group;
   PdlScope pdl(true);
-  if (c.splits <= kJoinFew)
-    return launch_k(paged_attention_join_few_kernel<T, HD>,
+  if (rows >= kJoinRows)
+    return launch_k(paged_attention_join_rows_kernel<T, HD>,
                     dim3((unsigned)((rows + kPagedWarps - 1) / kPagedWarps)),
                     dim3(kPagedThreads), 0, st, a, rows);
   return launch_k(paged_attention_join_kernel<T, HD>, dim3((unsigned)rows), dim3(kJoinThreads), 0,
@@ -994,7 +1059,8 @@ int wx_paged_attention(const void* q, int64_t q_seq_stride, int64_t q_head_strid
   a.v = v_cache;
   a.out = out;
   a.lse = lse;
-  a.part_o = static_cast<float*>(workspace);
+  a.picked = static_cast<int*>(workspace);
+  a.part_o = static_cast<float*>(workspace) + 4;
   a.part_ml = reinterpret_cast<float2*>(a.part_o + rows * c.splits * head_dim);
   a.table = table;
   a.lens = lens;
