@@ -1,0 +1,65 @@
+"""A paged key-value cache for a text decoder on the encoder's features: the
+tensors that ops.kv_fork, kv_append, kv_compact and paged_attention work on, kept
+together. Nothing here waits for the GPU.
+
+A step of a decoder with beams:
+
+    cache.step(parents, grow)          # beams reordered, ended, started; pages found
+    for layer in range(cache.n_layers):
+        cache.append(layer, k, v)      # this step's tokens
+        o = cache.attend(layer, q)
+"""
+import torch
+
+from . import ops
+
+
+class PagedKVCache:
+    """n_layers pools of n_pages pages of page_size tokens, for n_seqs sequences of
+    up to max_len tokens (rounded up to whole pages). Tensors, all on the device:
+
+    k, v: (n_layers, n_pages, page_size, n_heads, head_dim), uninitialised
+    table: (n_seqs, width) int32 page table, -1 past a sequence's last page
+    lens: (n_seqs,) int32 tokens, the last step's included
+    refs: (n_pages,) int32 table entries that name a page, 0: free
+    grown: (n_seqs,) int32 tokens that the last step granted
+    status: int32 (pages left free, pages short) of the last step
+    """
+
+    def __init__(self, n_layers, n_pages, page_size, n_heads, head_dim, n_seqs, max_len,
+                 dtype=torch.bfloat16, device=None):
+        if min(n_layers, n_pages, page_size, n_heads, head_dim, n_seqs, max_len) < 1:
+            raise ValueError("PagedKVCache: every size must be at least 1")
+        device = torch.device("cuda", torch.cuda.current_device() if device is None else
+                              torch.device(device).index or 0)
+        self.n_layers, self.page_size, self.max_len = n_layers, page_size, max_len
+        shape = (n_layers, n_pages, page_size, n_heads, head_dim)
+        self.k = torch.empty(shape, dtype=dtype, device=device)
+        self.v = torch.empty(shape, dtype=dtype, device=device)
+        width = -(-max_len // page_size)
+        i32 = dict(dtype=torch.int32, device=device)
+        self.table = torch.full((n_seqs, width), -1, **i32)
+        self.lens = torch.zeros(n_seqs, **i32)
+        self.refs = torch.zeros(n_pages, **i32)
+        self.grown = torch.zeros(n_seqs, **i32)
+        self.status = torch.tensor([n_pages, 0], **i32)
+
+    def step(self, parents=None, grow=None):
+        """Sequence i goes on as parents[i] was (-1: it starts empty; None: as
+        itself) with grow[i] more tokens (None: none): see ops.kv_fork."""
+        self.table, self.lens, self.refs, self.grown, self.status = ops.kv_fork(
+            self.k, self.v, self.table, self.lens, self.refs, parents=parents, grow=grow)
+
+    def append(self, layer, k, v):
+        """The tokens that the last step granted: k, v (n_seqs, tokens, heads,
+        head_dim), of which row t < grown[i] is used, or (n_seqs, heads, head_dim)."""
+        ops.kv_append(k, v, self.k[layer], self.v[layer], self.table, self.lens,
+                      counts=self.grown)
+
+    def attend(self, layer, q, **kw):
+        """ops.paged_attention of one query token a sequence over a layer."""
+        return ops.paged_attention(q, self.k[layer], self.v[layer], self.table, self.lens, **kw)
+
+    def compact(self):
+        """Moves the pages in use to the front of the pools."""
+        self.table, self.refs, _ = ops.kv_compact(self.k, self.v, self.table, self.refs)
