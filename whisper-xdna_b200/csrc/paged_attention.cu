@@ -66,16 +66,25 @@ __device__ __forceinline__ void key_range(const PagedArgs& a, int seq, int* firs
 constexpr int kPagedThreads = 128;
 constexpr int kPagedWarps = kPagedThreads / 32;
 
-// Where key t of the sequence with this row of the table is, in elements from the
-// head's first; -1: on no page.
-__device__ __forceinline__ int64_t key_at(const PagedArgs& a, const int32_t* row, int t) {
-  const int slot = a.by_page(t);
-  const int page = __ldg(row + slot);
-  if (page < 0 || page >= a.n_pages) {
+// The page of a key, read a turn before its place is worked out: the load is not
+// waited for in between.
+struct PagedKey {
+  int t, page;   // the key, -1: none
+};
+__device__ __forceinline__ PagedKey read_page(const PagedArgs& a, const int32_t* row, int t,
+                                              bool is) {
+  PagedKey k = {is ? t : -1, 0};
+  if (is) k.page = __ldg(row + a.by_page(t));
+  return k;
+}
+// Where it is, in elements from the head's first; -1: nowhere.
+__device__ __forceinline__ int64_t place_key(const PagedArgs& a, const PagedKey& k) {
+  if (k.t < 0) return -1;
+  if (k.page < 0 || k.page >= a.n_pages) {
     atomicOr(&g_attend_err, WX_DEVERR_PAGE);
     return -1;
   }
-  return page * a.page_stride + (t - slot * a.page_size) * a.tok_stride;
+  return k.page * a.page_stride + (k.t - a.by_page(k.t) * a.page_size) * a.tok_stride;
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
@@ -293,7 +302,7 @@ struct FmaCfg {
 // ends with one (key, query row) and takes one exponential; the weights come back
 // to all lanes through shared memory.
 template <int HD, int GT, int WPI>
-__global__ void __launch_bounds__(kPagedThreads) paged_attention_fma_kernel(const PagedArgs a) {
+__global__ void __launch_bounds__(kPagedThreads, 4) paged_attention_fma_kernel(const PagedArgs a) {
   using Cfg = FmaCfg<HD>;
   constexpr int kLanes = HD / 4, kGroups = 32 / kLanes;
   constexpr int kKeys = Cfg::kTok / kGroups;         // of a group
@@ -319,10 +328,10 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_fma_kernel(cons
   constexpr int kTurn = WPI * Cfg::kTok;   // keys of one turn of the item's warps
   const int base = c0 + w % WPI * Cfg::kTok;
   const int n_mine = base < c1 ? (c1 - base + kTurn - 1) / kTurn : 0;
-  // where key (tile i, lane % kTok) is, -1: nowhere
-  auto locate = [&](int i) -> int64_t {
+  // key (tile i, lane % kTok)
+  auto locate = [&](int i) {
     const int t = base + i * kTurn + lane % Cfg::kTok;
-    return t < c1 ? key_at(a, row, t) : -1;
+    return read_page(a, row, t, i < n_mine && t < c1);
   };
   auto fetch = [&](int i, int64_t where) {
     const uint32_t slot = ring_at + (i % Cfg::kStages) * 2 * Cfg::kTileBytes;
@@ -336,14 +345,15 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_fma_kernel(cons
       cp_async16(dst + Cfg::kTileBytes, vp + from, at >= 0);
     }
   };
-  int64_t next = n_mine > 0 ? locate(0) : -1;
+  PagedKey next = locate(0);
   uint32_t live[Cfg::kStages];   // bit r: key r of the tile in this slot is one
 #pragma unroll
   for (int i = 0; i < Cfg::kStages - 1; i++) {
-    live[i] = __ballot_sync(0xffffffffu, next >= 0);
-    if (i < n_mine) fetch(i, next);
+    const int64_t where = place_key(a, next);
+    next = locate(i + 1);
+    live[i] = __ballot_sync(0xffffffffu, where >= 0);
+    if (i < n_mine) fetch(i, where);
     cp_async_commit();
-    next = i + 1 < n_mine ? locate(i + 1) : -1;
   }
 
   // query rows in pairs, so that one packed FMA serves two of them (GT = 1: one row
@@ -368,12 +378,12 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_fma_kernel(cons
   for (int i = 0; i < n_mine; i++) {
     {
       const int f = i + Cfg::kStages - 1;
+      const int64_t where = place_key(a, next);
+      next = locate(f + 1);
+      live[Cfg::kStages - 1] = __ballot_sync(0xffffffffu, where >= 0);
       __syncwarp();   // every lane has read the slot that is filled now
-      const uint32_t bits = __ballot_sync(0xffffffffu, next >= 0);
-      if (f < n_mine) fetch(f, next);
+      if (f < n_mine) fetch(f, where);
       cp_async_commit();
-      next = f + 1 < n_mine ? locate(f + 1) : -1;
-      live[Cfg::kStages - 1] = bits;
     }
     cp_async_wait<Cfg::kStages - 1>();
     __syncwarp();
@@ -559,10 +569,10 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_mma_kernel(cons
   const int base = c0 / kTok * kTok + w % WPI * kTok;
   const int n_mine = base < c1 ? (c1 - base + kTurn - 1) / kTurn : 0;
 
-  // where key (tile i, lane % 16) is, -1: nowhere
-  auto locate = [&](int i) -> int64_t {
+  // key (tile i, lane % 16)
+  auto locate = [&](int i) {
     const int t = base + i * kTurn + (lane & 15);
-    return t >= c0 && t < c1 ? key_at(a, row, t) : -1;
+    return read_page(a, row, t, i < n_mine && t >= c0 && t < c1);
   };
   // copies tile i (its keys at `where`) into its slot of the ring; returns which
   // keys have none
@@ -579,14 +589,15 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_mma_kernel(cons
     }
   };
 
-  int64_t next = n_mine > 0 ? locate(0) : -1;
+  PagedKey next = locate(0);
   uint32_t live[Cfg::kStages];   // bit r: key r of the tile in this slot is one
 #pragma unroll
   for (int i = 0; i < Cfg::kStages - 1; i++) {
-    live[i] = __ballot_sync(0xffffffffu, next >= 0);
-    if (i < n_mine) fetch(i, next);
+    const int64_t where = place_key(a, next);
+    next = locate(i + 1);
+    live[i] = __ballot_sync(0xffffffffu, where >= 0);
+    if (i < n_mine) fetch(i, where);
     cp_async_commit();
-    next = i + 1 < n_mine ? locate(i + 1) : -1;
   }
 
   // Q^T in fragments: row n = lane / 4, dimensions 2 (lane % 4) + {0, 1, 8, 9}
@@ -623,12 +634,12 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_mma_kernel(cons
   for (int i = 0; i < n_mine; i++) {
     {
       const int f = i + Cfg::kStages - 1;
+      const int64_t where = place_key(a, next);
+      next = locate(f + 1);
+      live[Cfg::kStages - 1] = __ballot_sync(0xffffffffu, where >= 0);
       __syncwarp();   // every lane has read the slot that is filled now
-      const uint32_t bits = __ballot_sync(0xffffffffu, next >= 0);
-      if (f < n_mine) fetch(f, next);
+      if (f < n_mine) fetch(f, where);
       cp_async_commit();
-      next = f + 1 < n_mine ? locate(f + 1) : -1;
-      live[Cfg::kStages - 1] = bits;
     }
     cp_async_wait<Cfg::kStages - 1>();
     __syncwarp();
