@@ -131,6 +131,35 @@ Tensor empty(int dev, at::IntArrayRef shape, at::ScalarType dtype) {
   return at::detail::empty_cuda(shape, dtype, at::Device(at::kCUDA, (c10::DeviceIndex)dev),
                                 std::nullopt);
 }
+// Several outputs in one allocation: an allocation costs the host as much as a launch
+// does. Each starts on 16 bytes.
+class Outputs {
+ public:
+  explicit Outputs(int dev) : dev_(dev) {}
+  // the place of an output of `bytes` bytes
+  int64_t add(int64_t bytes) {
+    const int64_t at = total_;
+    total_ += (bytes + 15) / 16 * 16;
+    return at;
+  }
+  void allocate() { all_ = empty(dev_, {total_}, at::kByte); }
+  char* at(int64_t place) const { return static_cast<char*>(all_.data_ptr()) + place; }
+  // a contiguous tensor on the output at `place`
+  Tensor tensor(int64_t place, at::IntArrayRef shape, at::ScalarType dtype) const {
+    const auto meta = c10::scalarTypeToTypeMeta(dtype);
+    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all_.storage()),
+                                                        all_.key_set(), meta);
+    t.unsafeGetTensorImpl()->set_storage_offset(place / (int64_t)meta.itemsize());
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(shape);
+    return t;
+  }
+
+ private:
+  int dev_;
+  int64_t total_ = 0;
+  Tensor all_;
+};
+
 void* stream(int dev) { return c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream(); }
 void check(int status) {
   if (status != WX_OK) throw Failed{status};
@@ -242,16 +271,21 @@ PyObject* kv_fork(PyObject* const* a) {
   const int32_t* grow = ints(plain_or_null(c.dev, a[6], "grow", at::kInt, {table.n}));
   const int64_t space = wx_kv_workspace(table.n, c.n_pages);
   const Tensor ws = empty(c.dev, {space}, at::kByte);
-  Tensor t = empty(c.dev, {table.n, table.width}, at::kInt), l = empty(c.dev, {table.n}, at::kInt),
-         r = empty(c.dev, {c.n_pages}, at::kInt), g = empty(c.dev, {table.n}, at::kInt),
-         s = empty(c.dev, {2}, at::kInt);
+  Outputs out(c.dev);
+  const int64_t t = out.add(4 * table.n * table.width), l = out.add(4 * table.n),
+                r = out.add(4 * c.n_pages), g = out.add(4 * table.n), s = out.add(8);
+  out.allocate();
   check(wx_kv_fork(c.k.data_ptr(), c.v.data_ptr(), c.n_layers, c.layer_stride, c.page_stride,
                    c.tok_stride, c.head_stride, c.n_heads, c.hd, c.n_pages, c.page, c.dtype,
-                   table.p, lens, refs, parents, grow, table.n, table.width, ints(t.data_ptr()),
-                   ints(l.data_ptr()), ints(r.data_ptr()), ints(g.data_ptr()), ints(s.data_ptr()),
+                   table.p, lens, refs, parents, grow, table.n, table.width, ints(out.at(t)),
+                   ints(out.at(l)), ints(out.at(r)), ints(out.at(g)), ints(out.at(s)),
                    ws.data_ptr(), space, stream(c.dev)));
-  return Py_BuildValue("(NNNNN)", THPVariable_Wrap(t), THPVariable_Wrap(l), THPVariable_Wrap(r),
-                       THPVariable_Wrap(g), THPVariable_Wrap(s));
+  return Py_BuildValue("(NNNNN)",
+                       THPVariable_Wrap(out.tensor(t, {table.n, table.width}, at::kInt)),
+                       THPVariable_Wrap(out.tensor(l, {table.n}, at::kInt)),
+                       THPVariable_Wrap(out.tensor(r, {c.n_pages}, at::kInt)),
+                       THPVariable_Wrap(out.tensor(g, {table.n}, at::kInt)),
+                       THPVariable_Wrap(out.tensor(s, {2}, at::kInt)));
 }
 
 // kv_compact(k_cache, v_cache, table, refs)
@@ -261,13 +295,18 @@ PyObject* kv_compact(PyObject* const* a) {
   const int32_t* refs = ints(plain(c.dev, tensor(a[3], "refs"), "refs", at::kInt, {c.n_pages}));
   const int64_t space = wx_kv_workspace(table.n, c.n_pages);
   const Tensor ws = empty(c.dev, {space}, at::kByte);
-  Tensor t = empty(c.dev, {table.n, table.width}, at::kInt),
-         r = empty(c.dev, {c.n_pages}, at::kInt), s = empty(c.dev, {2}, at::kInt);
+  Outputs out(c.dev);
+  const int64_t t = out.add(4 * table.n * table.width), r = out.add(4 * c.n_pages),
+                s = out.add(8);
+  out.allocate();
   check(wx_kv_compact(c.k.data_ptr(), c.v.data_ptr(), c.n_layers, c.layer_stride, c.page_stride,
                       c.tok_stride, c.head_stride, c.n_heads, c.hd, c.n_pages, c.page, c.dtype,
-                      table.p, refs, table.n, table.width, ints(t.data_ptr()), ints(r.data_ptr()),
-                      ints(s.data_ptr()), ws.data_ptr(), space, stream(c.dev)));
-  return Py_BuildValue("(NNN)", THPVariable_Wrap(t), THPVariable_Wrap(r), THPVariable_Wrap(s));
+                      table.p, refs, table.n, table.width, ints(out.at(t)), ints(out.at(r)),
+                      ints(out.at(s)), ws.data_ptr(), space, stream(c.dev)));
+  return Py_BuildValue("(NNN)",
+                       THPVariable_Wrap(out.tensor(t, {table.n, table.width}, at::kInt)),
+                       THPVariable_Wrap(out.tensor(r, {c.n_pages}, at::kInt)),
+                       THPVariable_Wrap(out.tensor(s, {2}, at::kInt)));
 }
 
 // token_logprobs(logits, tokens, top_k, temperature)
@@ -285,14 +324,19 @@ PyObject* token_logprobs(PyObject* const* a) {
     refuse("top_k " + std::to_string(top_k) + " not in [0, min(32, vocabulary " +
            std::to_string(vocab) + ")]");
   const double temperature = number(a[3]);
-  Tensor logprob = empty(dev, {rows}, at::kFloat), entropy = empty(dev, {rows}, at::kFloat),
-         top = empty(dev, {rows, top_k}, at::kFloat), index = empty(dev, {rows, top_k}, at::kInt);
+  Outputs out(dev);
+  const int64_t logprob = out.add(4 * rows), entropy = out.add(4 * rows),
+                top = out.add(4 * rows * top_k), index = out.add(4 * rows * top_k);
+  out.allocate();
+  auto floats = [&](int64_t place) { return reinterpret_cast<float*>(out.at(place)); };
   check(wx_token_logprobs(x.data_ptr(), dtype, rows, vocab, x.stride(0), tokens, top_k,
-                          (float)temperature, logprob.data_ptr<float>(),
-                          entropy.data_ptr<float>(), top_k ? top.data_ptr<float>() : nullptr,
-                          top_k ? ints(index.data_ptr()) : nullptr, stream(dev)));
-  return Py_BuildValue("(NNNN)", THPVariable_Wrap(logprob), THPVariable_Wrap(entropy),
-                       THPVariable_Wrap(top), THPVariable_Wrap(index));
+                          (float)temperature, floats(logprob), floats(entropy),
+                          top_k ? floats(top) : nullptr, top_k ? ints(out.at(index)) : nullptr,
+                          stream(dev)));
+  return Py_BuildValue("(NNNN)", THPVariable_Wrap(out.tensor(logprob, {rows}, at::kFloat)),
+                       THPVariable_Wrap(out.tensor(entropy, {rows}, at::kFloat)),
+                       THPVariable_Wrap(out.tensor(top, {rows, top_k}, at::kFloat)),
+                       THPVariable_Wrap(out.tensor(index, {rows, top_k}, at::kInt)));
 }
 
 // A function of `count` positional arguments; its errors as Python's.
