@@ -60,7 +60,7 @@ __device__ __forceinline__ uint64_t entry(float x, uint32_t index) {
 
 // The running sums of one thread or of a part of a row.
 struct Sums {
-  float m, s, u;   // maximum logit, sum 2^d, sum 2^d d (d in log2 units)
+  float m, s, u;   // reference logit, sum 2^d, sum 2^d d (d = (logit - m) c, log2 units)
 };
 
 // x with the reference m in place of its own, m at least x.m; c = log2(e) / T
@@ -161,16 +161,20 @@ __device__ __forceinline__ void find_reach(Candidates& c, uint32_t key, int top_
   }
   c.sorted[w][r] = key;
   __syncthreads();
-  int above = 0;   // largest logits above this one, by a search in each warp's
+  // the CTA's top_k-th is among its warps' first top_k
+  if (threadIdx.x < kScoreWarps * top_k) {
+    const uint32_t mine = c.sorted[threadIdx.x / top_k][threadIdx.x % top_k];
+    int above = 0;   // largest logits above this one, by a search in each warp's
 #pragma unroll
-  for (int u = 0; u < kScoreWarps; u++) {
-    int at = 0;
+    for (int u = 0; u < kScoreWarps; u++) {
+      int at = 0;
 #pragma unroll
-    for (int step = 16; step > 0; step >>= 1)
-      if (c.sorted[u][at + step - 1] > key) at += step;
-    above += at + (c.sorted[u][at] > key ? 1 : 0);
+      for (int step = 16; step > 0; step >>= 1)
+        if (c.sorted[u][at + step - 1] > mine) at += step;
+      above += at + (c.sorted[u][at] > mine ? 1 : 0);
+    }
+    if (above < top_k) atomicMin(&c.reach, mine);
   }
-  if (above < top_k) atomicMin(&c.reach, key);
   __syncthreads();
   if (key && key >= c.reach) c.owners[atomicAdd(&c.n_owners, 1)] = (uint8_t)threadIdx.x;
   __syncthreads();
@@ -323,10 +327,11 @@ __global__ void __launch_bounds__(kScoreThreads, 4) token_score_kernel(const Sco
   float m = -INFINITY;
   float2 s2 = {0.0f, 0.0f}, u2 = {0.0f, 0.0f};
   float largest = -INFINITY;   // the thread's
-  // the warp's maximum becomes that of vm where it is larger: seldom after a few
-  // steps, since the warp's lanes share it
+  // the reference moves to the warp's maximum where a logit passes it by more than
+  // 2^8 in weight: once or twice a row, since the warp's lanes share it
+  const float slack = 8.0f / c;
   auto raise = [&](float vm) {
-    if (!__any_sync(0xffffffffu, !(vm <= m))) return;
+    if (!__any_sync(0xffffffffu, !(vm <= m + slack))) return;
     const float to = max_nan(m, warp_max(vm));
     const Sums x = refer({m, s2.x, u2.x}, to, c), y = refer({m, s2.y, u2.y}, to, c);
     s2 = {x.s, y.s};
