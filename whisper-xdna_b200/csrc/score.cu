@@ -145,13 +145,18 @@ struct Candidates {
   uint64_t part[kScoreWarps];
   uint32_t sorted[kScoreWarps][32];   // each warp's largest logits, descending
   uint32_t reach;                     // the top_k-th largest of them: top_k reach it
-  int n, n_owners;
-  uint8_t owners[kScoreThreads];      // threads whose largest logit reaches it
+  int n, n_in_step, n_owners;
+  // threads whose largest logit reaches it: with the one step that has it (step <<
+  // 8), or, where another step's do too, for all their steps
+  uint32_t in_step[kScoreThreads];
+  uint8_t owners[kScoreThreads];
 };
 
 // Sets c.reach from each thread's largest logit (its order_key; 0: it has none), and
-// c.owners. Called by every thread, after a barrier; ends with one.
-__device__ __forceinline__ void find_reach(Candidates& c, uint32_t key, int top_k) {
+// the lists of threads that reach it: `step` has the largest, `other` is the largest
+// of the other steps. Called by every thread, after a barrier; ends with one.
+__device__ __forceinline__ void find_reach(Candidates& c, uint32_t key, int step, float other,
+                                           int top_k) {
   const int lane = lane_id(), w = warp_id();
   int r = 0;
 #pragma unroll
@@ -176,7 +181,12 @@ __device__ __forceinline__ void find_reach(Candidates& c, uint32_t key, int top_
     if (above < top_k) atomicMin(&c.reach, mine);
   }
   __syncthreads();
-  if (key && key >= c.reach) c.owners[atomicAdd(&c.n_owners, 1)] = (uint8_t)threadIdx.x;
+  if (key && key >= c.reach) {
+    if (order_key(other) >= c.reach)
+      c.owners[atomicAdd(&c.n_owners, 1)] = (uint8_t)threadIdx.x;
+    else
+      c.in_step[atomicAdd(&c.n_in_step, 1)] = ((uint32_t)step << 8) | threadIdx.x;
+  }
   __syncthreads();
 }
 static_assert(kScoreThreads <= 256, "a thread's number is kept in a byte");
@@ -277,10 +287,11 @@ __device__ __noinline__ void take_best(const Slice<T>& s, Candidates& c, int top
 //
 // A thread takes kScoreVecs 16-byte vectors a step, copied kScoreStages - 1 steps
 // ahead into shared memory; the warp shares the reference of its sums. For the
-// alternatives the pass keeps each thread's largest logit and nothing else. The
-// top_k-th of these is a logit that top_k reach, so the alternatives are among the
-// logits of the few threads whose largest reaches it: these are gone over again
-// (from shared memory or L2), and those that reach it are listed and put in order
+// alternatives the pass keeps each thread's largest logit, its step, and the largest
+// of the other steps. The top_k-th of the threads' largest is a logit that top_k reach,
+// so the alternatives are among the logits of the few threads whose largest reaches
+// it: that step, or all of theirs where another reaches it too, is gone over again
+// (from shared memory or L2), and the logits that reach it are listed and put in order
 // by counting ranks. The parts are joined in shared memory, then over the cluster's.
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kScoreThreads, 4) token_score_kernel(const ScoreArgs a) {
@@ -321,12 +332,14 @@ __global__ void __launch_bounds__(kScoreThreads, 4) token_score_kernel(const Sco
   for (int it = 0; it < kScoreStages - 1; it++) fetch(it);
   if (TOP && threadIdx.x == 0) {
     cand.reach = 0xFFFFFFFFu;
-    cand.n = cand.n_owners = 0;
+    cand.n = cand.n_in_step = cand.n_owners = 0;
   }
 
   float m = -INFINITY;
   float2 s2 = {0.0f, 0.0f}, u2 = {0.0f, 0.0f};
-  float largest = -INFINITY;   // the thread's
+  // the thread's largest logit, its step, and the largest of its other steps
+  float largest = -INFINITY, other = -INFINITY;
+  int largest_step = 0;
   // the reference moves to the warp's maximum where a logit passes it by more than
   // 2^8 in weight: once or twice a row, since the warp's lanes share it
   const float slack = 8.0f / c;
@@ -360,7 +373,12 @@ __global__ void __launch_bounds__(kScoreThreads, 4) token_score_kernel(const Sco
     for (int j = 0; j < kScoreVecs; j++)
 #pragma unroll
       for (int e = 0; e < N; e += 2) vm = max_nan(vm, v[j][e], v[j][e + 1]);
-    if (TOP) largest = max_nan(largest, vm);
+    if (TOP) {
+      const bool up = vm > largest;   // NaN: among the others, and so gone over
+      other = max_nan(other, up ? largest : vm);
+      largest_step = up ? it : largest_step;
+      largest = up ? vm : largest;
+    }
     raise(vm);
     const float ref = m == -INFINITY ? 0.0f : m;
     const float2 neg = {-ref, -ref}, c2 = {c, c};
@@ -401,32 +419,39 @@ __global__ void __launch_bounds__(kScoreThreads, 4) token_score_kernel(const Sco
   }
   if (TOP) {
     const bool has = s.v0 + Slice<T>::at(0, 0, threadIdx.x) < s.v1;
-    find_reach(cand, has ? order_key(largest) : 0, a.top_k);
+    find_reach(cand, has ? order_key(max_nan(largest, other)) : 0, largest_step, other, a.top_k);
     const uint32_t reach = cand.reach;
     auto list = [&](uint64_t e) {
       const int at = atomicAdd(&cand.n, 1);
       if (at < kCandidates) cand.list[at] = e;
     };
     if (edge && (uint32_t)(edge >> 32) >= reach) list(edge);
-    // the owners' vectors, dealt out over the CTA; what is left in the ring is there
-    const int per = s.n_steps * kScoreVecs, n = cand.n_owners * per;
+    // vector j of thread t's step it; what is left in the ring is there
     const bool in_ring = s.n_steps <= kScoreStages;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < n; i += kScoreThreads) {
-      const int t = cand.owners[i / per], f = i % per, it = f / kScoreVecs, j = f % kScoreVecs;
+    auto go_over = [&](int it, int j, int t) {
       const int k = s.v0 + Slice<T>::at(it, j, t);
-      if (k >= s.v1) continue;
+      if (k >= s.v1) return;
       float v[N];
       Lanes<T>::unpack(in_ring ? ring[it][j][t] : __ldg(s.vec + k), v);
       float vm = v[0];
 #pragma unroll
       for (int e = 0; e < N; e += 2) vm = max_nan(vm, v[e], v[e + 1]);
-      if (order_key(vm) < reach) continue;
+      if (order_key(vm) < reach) return;
 #pragma unroll
       for (int e = 0; e < N; e++) {
         const uint32_t y = order_key(v[e]);
         if (y >= reach) list(((uint64_t)y << 32) | ~(uint32_t)(s.lead + k * N + e));
       }
+    };
+    // dealt out over the CTA: the threads' one step, and all steps of the few others
+    const int n_one = cand.n_in_step * kScoreVecs, per = s.n_steps * kScoreVecs;
+    const int n_all = n_one + cand.n_owners * per;
+#pragma unroll 1
+    for (int i = threadIdx.x; i < n_all; i += kScoreThreads) {
+      const int u = i < n_one ? 0 : (i - n_one) / per, f = i < n_one ? i : i - n_one - u * per;
+      const uint32_t o = i < n_one ? cand.in_step[i / kScoreVecs]
+                                   : (uint32_t)(f / kScoreVecs) << 8 | cand.owners[u];
+      go_over((int)(o >> 8), f % kScoreVecs, (int)(o & 255));
     }
     __syncthreads();
     if (cand.n <= kCandidates)
