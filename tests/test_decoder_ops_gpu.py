@@ -113,6 +113,25 @@ def test_attend_long(cuda, dtype, lens, hd, group):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("seqs,width", [(130, 2048), (128, 300), (3, 5000)])
+def test_attend_long_tables(cuda, dtype, seqs, width):
+    """Tables that could hold far more than they do: the split goes by the keys there
+    are, and by the bound alone where sequences are many."""
+    lens = [9000, 0, 4100] + [(7 * i) % 90 for i in range(seqs - 3)]
+    k, v, table, n, gen = make_cache(lens, 64, 2, 64, dtype, seed=seqs, width=width)
+    check_attend(randn(gen, seqs, 6, 64, dtype=dtype), k, v, table, n)
+    check_attend(randn(gen, seqs, 6, 64, dtype=dtype), k, v, table, n, max_len=9000)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads,group", [(10, 3), (7, 11)])
+def test_attend_many_short_sequences(cuda, dtype, heads, group):
+    lens = [(37 * i) % 200 for i in range(301)]
+    k, v, table, n, gen = make_cache(lens, 16, heads, 64, dtype, seed=heads)
+    check_attend(randn(gen, 301, heads * group, 64, dtype=dtype), k, v, table, n)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_attend_window(cuda, dtype):
     lens = [40, 40, 40, 40, 700, 700, 0, 2500]
     starts = torch.tensor([0, 7, 39, 40, 16, 699, 3, 2100], dtype=torch.int32, device="cuda")
@@ -585,6 +604,27 @@ def test_scores_of_strided_rows(cuda, dtype, offset):
     x = (randn(gen, 9, 2111) * 3).to(dtype)[:, offset:offset + 2003]
     tokens = torch.randint(0, 2003, (9,), generator=gen, device="cuda")
     check_score(x, tokens, 7, 1.0)
+
+
+def test_scores_of_many_rows(cuda):
+    """More rows than a grid's second dimension."""
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    x = randn(gen, 65600, 37)
+    tokens = torch.randint(0, 37, (65600,), generator=gen, device="cuda")
+    check_score(x, tokens, 3, 1.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_scores_of_large_logits(cuda, dtype):
+    """Logits that rise and fall by far more than a power of two's range."""
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    x = torch.linspace(-3000, 3000, 30011, device="cuda").repeat(3, 1)
+    x[1] = x[1].flip(0)
+    x[2] = x[2, torch.randperm(30011, generator=gen, device="cuda")]
+    x = x.to(dtype)
+    tokens = torch.randint(0, 30011, (3,), generator=gen, device="cuda")
+    check_score(x, tokens, 20, 1.0)
+    check_score(x, tokens, 20, 0.01)
 
 
 def test_scores_same_each_time(cuda):

@@ -7,6 +7,7 @@
 // in units of log2). A row without keys gives o = 0 and lse = -inf. The cache's
 // length is split over CTAs where sequences and heads alone do not fill the
 // GPU; the parts' (maximum, sum, o) are then joined, always in the same order.
+#include <algorithm>
 #include <atomic>
 #include <cstdint>
 
@@ -109,7 +110,7 @@ constexpr int kMaxChunk = 1024;
 // Every thread of a CTA calls it.
 __device__ __forceinline__ int pick_chunk(const PagedArgs& a) {
   __shared__ int64_t sh_keys[kPagedWarps];
-  if (a.chunk == kMaxChunk) return a.chunk;
+  if (a.chunk >= kMaxChunk) return a.chunk;
   int64_t keys = 0;
   if ((int)threadIdx.x < a.n_seqs) {
     const int end = min(a.lens[threadIdx.x], a.max_len);
@@ -257,7 +258,8 @@ __device__ __forceinline__ void finish_item(const PagedArgs& a, const PagedItem&
                 [&](int u) { return peer_f32(mine + ROWS * (HD + 1) + g, u); },
                 [&](int u) { return peer_f32(mine + g * HD + d, u); }));
     }
-    // a CTA's shared memory outlives its readers: nothing is handed over
+    // a CTA's shared memory outlives its readers, whose values are in use by now:
+    // nothing is handed over
     asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::
                      : "memory");
   }
@@ -767,7 +769,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_join_rows_kerne
   key_range(a, seq, &first, &end);
   const float2* ml = a.part_ml + r * a.splits;
   pdl_wait();
-  const int chunk = a.chunk == kMaxChunk ? kMaxChunk : *a.picked;
+  const int chunk = a.chunk >= kMaxChunk ? a.chunk : *a.picked;
   const int s0 = first / chunk, s1 = first < end ? (end + chunk - 1) / chunk : s0;
   // lane s - s32 holds split s
   float2 my = s0 + lane < s1 ? ml[s0 + lane] : make_float2(-INFINITY, 0.0f);
@@ -824,7 +826,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(cons
   key_range(a, seq, &first, &end);
   const float2* ml = a.part_ml + r * a.splits;
   pdl_wait();
-  const int chunk = a.chunk == kMaxChunk ? kMaxChunk : *a.picked;
+  const int chunk = a.chunk >= kMaxChunk ? a.chunk : *a.picked;
   const int s0 = first / chunk, s1 = first < end ? (end + chunk - 1) / chunk : s0;
   auto over_warps = [&](float x, bool max) {   // every thread gets it
 #pragma unroll
@@ -889,6 +891,7 @@ struct PagedCut {
 constexpr int64_t kShortKeys = 256, kShortItems = 8 * 148;
 constexpr int64_t kClusterKeys = 4096;
 constexpr int64_t kMinChunk = 128, kChunkCtas = 32 * 148;
+constexpr int64_t kMostParts = 32768;   // bounds the workspace of many long sequences
 
 static PagedCut paged_cut(int64_t n_seqs, int64_t n_heads, int64_t group, int64_t head_dim,
                           int64_t max_len, int dtype) {
@@ -908,6 +911,7 @@ static PagedCut paged_cut(int64_t n_seqs, int64_t n_heads, int64_t group, int64_
     int64_t chunk = max_len * items / kChunkCtas;
     chunk = chunk < kMinChunk ? kMinChunk : chunk > kMaxChunk ? kMaxChunk : chunk;
     if (n_seqs > kPagedThreads) chunk = kMaxChunk;   // pick_chunk leaves it at that
+    chunk = std::max(chunk, max_len * items / kMostParts);
     chunk = (chunk + 15) / 16 * 16;
     c.chunk = (int)chunk;
     c.splits = (int)((max_len + chunk - 1) / chunk);

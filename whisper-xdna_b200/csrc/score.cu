@@ -471,7 +471,8 @@ __global__ void __launch_bounds__(kScoreThreads, 4) token_score_kernel(const Sco
       if (TOP && w < n_ctas && lane < a.top_k)
         cand.list[w * a.top_k + lane] = peer_u64(cluster_peer(cand.best + lane, w));
     }
-    // a CTA's shared memory outlives its readers: nothing is handed over
+    // a CTA's shared memory outlives its readers, whose values are in use by now:
+    // nothing is handed over
     asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;"
                  ::: "memory");
     if (rank != 0) return;
