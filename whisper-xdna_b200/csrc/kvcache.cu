@@ -52,8 +52,10 @@ constexpr int kAppendUnroll = 4;
 
 // A thread moves units of sizeof(U) bytes, kAppendUnroll of them in flight: (token,
 // head, unit) of sequence blockIdx.y, K or V by blockIdx.z. Consecutive threads take
-// consecutive units of a row, so both sides are full lines. Bound by latency for one
-// token (a launch), by the memory's bandwidth for a prompt's or a clip's worth.
+// consecutive units of a row, so both sides are full lines. Measured (B200): 64 clips
+// of 1500 frames, 20 heads of 64 in bf16 (983 MB read and written) 146 us, 6.7 TB/s,
+// the memory's bandwidth; one unit in flight a thread and hardware divisions 198 us.
+// One token of 320 sequences 2.2 us, a launch.
 template <typename U>
 __global__ void __launch_bounds__(256) kv_append_kernel(const AppendArgs a) {
   const int seq = blockIdx.y;
@@ -246,7 +248,7 @@ __device__ __forceinline__ unsigned long long keeper_rank(int now, int i) {
 //     end are not grown
 // Integer work of a few bytes a page, bound by the latency of its phases. This form
 // keeps its arrays in global memory, parted by a cluster's barrier: for tables that
-// do not fit one CTA's shared memory.
+// do not fit one CTA's shared memory. Measured (B200): 58 K table entries 31 us.
 __global__ void __launch_bounds__(kPlanThreads, 1) kv_fork_kernel(const ForkArgs a) {
   __shared__ int64_t part[33];
   pdl_launch_dependents();
@@ -405,7 +407,10 @@ __host__ __device__ constexpr int64_t fork_words(int64_t n_seqs, int64_t width, 
 }
 
 // The same plan by one CTA, its arrays in shared memory: a phase costs a barrier and
-// not a trip through L2.
+// not a trip through L2. Bound by one SM's instruction issue as the table grows.
+// Measured (B200), with the copies' launch, here against the cluster's form: 5 beams
+// 7.9 and 16.2 us, 320 beams (4800 entries, 77 MB copied) 27 and 35, 256 sequences
+// of 57 pages (14.6 K entries) 17.2 and 18.4: kCtaEntries is where they meet.
 __global__ void __launch_bounds__(kPlanThreads, 1) kv_fork_cta_kernel(const ForkArgs a) {
   extern __shared__ __align__(16) int32_t words[];
   __shared__ int64_t part[33];
@@ -635,7 +640,8 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_compact_kernel(const Compa
 // Words of shared memory that the one-CTA form of a compaction takes.
 __host__ __device__ constexpr int64_t compact_words(int64_t n_pages) { return 4 * n_pages; }
 
-// The same by one CTA, its arrays in shared memory.
+// The same by one CTA, its arrays in shared memory. Measured (B200): 96 pages, 11 of
+// them moved, 5.8 us with the copies; in the cluster's form 13.1.
 __global__ void __launch_bounds__(kPlanThreads, 1) kv_compact_cta_kernel(const CompactArgs a) {
   extern __shared__ __align__(16) int32_t words[];
   __shared__ int64_t part[33];
@@ -716,11 +722,13 @@ constexpr int kCopyResident = 4;   // CTAs on an SM (registers)
 
 constexpr int kCopyPart = kCopyThreads * kCopyUnroll;   // 16-byte chunks
 
-// One CTA a part of a copy at a time, K or V of layer blockIdx.y / 2: 32 KiB of the page's tokens, 16
-// bytes a thread, kCopyUnroll loads in flight before their stores. Source and target
-// pages are never the same page, nor is a target another copy's source: plans copy
-// pages in use to free ones. Bound by the memory's bandwidth, read + write; whole
-// pages a CTA (20 to 64 KB) left a last round that few CTAs ran.
+// One CTA a part of a copy at a time, K or V of layer blockIdx.y / 2: 32 KiB of the
+// page's tokens, 16 bytes a thread, kCopyUnroll loads in flight before their stores.
+// Source and target pages are never the same page, nor is a target another copy's
+// source: plans copy pages in use to free ones. Bound by the memory's bandwidth, read
+// + write. Measured (B200): 734 MB (700 pages of 64 KB in 4 layers) 134 us with the
+// plan, 5.5 TB/s; 16 KiB parts and 4 loads in flight 132, but 30 against 27 us for
+// the 77 MB of 320 beams.
 __global__ void __launch_bounds__(kCopyThreads, kCopyResident) kv_copy_kernel(const CopyArgs a) {
   pdl_wait();   // the plan
   const int which = blockIdx.y & 1, layer = blockIdx.y >> 1;

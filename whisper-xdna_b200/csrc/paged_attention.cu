@@ -303,6 +303,11 @@ struct FmaCfg {
 // keys of a tile each. A tile's scores are summed over the lanes so that each lane
 // ends with one (key, query row) and takes one exponential; the weights come back
 // to all lanes through shared memory.
+//
+// Measured (B200): 43.7 K keys of a window, 2 heads of 128 with 8 query rows each (89
+// MB) 30 us with the join, 3.0 TB/s: bound by the issue of some 140 instructions a key
+// at 0.5 a cycle. One row at a time, keys straight to registers and five shuffles a
+// score, took 64.
 template <int HD, int GT, int WPI>
 __global__ void __launch_bounds__(kPagedThreads, 4) paged_attention_fma_kernel(const PagedArgs a) {
   using Cfg = FmaCfg<HD>;
@@ -545,7 +550,15 @@ struct MmaCfg {
 // own, rows out of range are zeros), and keeps sums of its own: no barrier until
 // the four warps' parts are joined at the end. The rows' reference maximum moves
 // only when a score passes it by more than 2^8, so weights stay below 2^8 and
-// the rescaling is rare.
+// the rescaling is rare. A decode step has 1 to 16 query rows a head: 128-row
+// accumulators in tensor memory would stand nearly empty, and mma.sync is far from its
+// limit here.
+//
+// Bound by the memory: measured (B200), 16 clips' 1500 frames of 20 heads of 64, five
+// beams each (123 MB) 25.8 us, 4.8 TB/s; 64 clips 89 us, 5.5 TB/s; 64 sequences of 1 to
+// 16384 tokens, 8 heads of 128 with 4 query rows (504 MB) 91 us, 5.5 TB/s; 5 beams'
+// first tokens 3.3 us, a launch. Products on the FMA pipe took 110 and 200 us for the
+// first and third; four-stage rings, with fewer CTAs on an SM, 34 and 99.
 template <int HD, int NT, int WPI>
 __global__ void __launch_bounds__(kPagedThreads) paged_attention_mma_kernel(const PagedArgs a) {
   using Cfg = MmaCfg<HD>;
