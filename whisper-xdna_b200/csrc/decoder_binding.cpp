@@ -145,12 +145,16 @@ class Outputs {
   void allocate() { all_ = empty(dev_, {total_}, at::kByte); }
   char* at(int64_t place) const { return static_cast<char*>(all_.data_ptr()) + place; }
   // a contiguous tensor on the output at `place`
-  Tensor tensor(int64_t place, at::IntArrayRef shape, at::ScalarType dtype) const {
+  Tensor tensor(int64_t place, at::IntArrayRef shape, at::ScalarType dtype,
+                at::OptionalIntArrayRef strides = {}) const {
     const auto meta = c10::scalarTypeToTypeMeta(dtype);
     Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all_.storage()),
                                                         all_.key_set(), meta);
     t.unsafeGetTensorImpl()->set_storage_offset(place / (int64_t)meta.itemsize());
-    t.unsafeGetTensorImpl()->set_sizes_contiguous(shape);
+    if (strides)
+      t.unsafeGetTensorImpl()->set_sizes_and_strides(shape, *strides);
+    else
+      t.unsafeGetTensorImpl()->set_sizes_contiguous(shape);
     return t;
   }
 
@@ -196,25 +200,31 @@ PyObject* paged_attention(PyObject* const* a) {
   if (n[0] != table.n || n[q.dim() - 1] != c.hd || q.stride(-1) != 1)
     refuse("q of shape " + sizes(n) + " does not fit " + std::to_string(table.n) +
            " sequences of head_dim " + std::to_string(c.hd) + " (contiguous)");
-  Tensor out;
-  if (a[8] == Py_None) {
-    // dense and without overlap: q's strides; else in q's order
-    if (q.is_non_overlapping_and_dense())
-      out = at::detail::empty_strided_cuda(n, q.strides(), q.scalar_type(), q.device());
-    else
-      out = empty(c.dev, n, q.scalar_type());
-  } else {
+  const bool own = a[8] == Py_None, want_lse = PyObject_IsTrue(a[9]) == 1;
+  Tensor out, lse;
+  if (!own) {
     out = tensor(a[8], "out");
     if (out.sizes() != n || out.scalar_type() != q.scalar_type() || !out.is_cuda() ||
         out.get_device() != c.dev || out.stride(-1) != 1)
       refuse("out must be like q, with a contiguous head_dim");
   }
+  Outputs outputs(c.dev);
+  const int64_t rows = table.n * c.n_heads * group;
+  const int64_t o_at = outputs.add(own ? q.numel() * (int64_t)q.element_size() : 0),
+                lse_at = outputs.add(want_lse ? 4 * rows : 0);
+  if (own || want_lse) outputs.allocate();
+  if (own) {
+    // q dense and without overlap: its strides; else its order of dimensions
+    if (q.is_non_overlapping_and_dense())
+      out = outputs.tensor(o_at, n, q.scalar_type(), q.strides());
+    else
+      out = outputs.tensor(o_at, n, q.scalar_type());
+  }
+  if (want_lse) lse = outputs.tensor(lse_at, n.slice(0, q.dim() - 1), at::kFloat);
   const int32_t* starts = ints(plain_or_null(c.dev, a[6], "starts", at::kInt, {table.n}));
   const int64_t max_len = a[7] == Py_None ? table.width * c.page : integer(a[7]);
   const double scale = a[5] == Py_None ? 1.0 / std::sqrt((double)c.hd) : number(a[5]);
-  const bool want_lse = PyObject_IsTrue(a[9]) == 1;
-  Tensor lse, ws;
-  if (want_lse) lse = empty(c.dev, n.slice(0, q.dim() - 1), at::kFloat);
+  Tensor ws;
   const int64_t space =
       wx_paged_attention_workspace(table.n, c.n_heads, group, c.hd, max_len, c.dtype);
   if (space < 0) throw Failed{(int)space};
@@ -227,7 +237,7 @@ PyObject* paged_attention(PyObject* const* a) {
       group, c.hd, c.n_pages, c.page, max_len, (float)scale, c.dtype,
       space ? ws.data_ptr() : nullptr, space, stream(c.dev)));
   PyObject* o = a[8];
-  if (o == Py_None)
+  if (own)
     o = THPVariable_Wrap(out);
   else
     Py_INCREF(o);

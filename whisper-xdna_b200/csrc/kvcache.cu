@@ -58,6 +58,7 @@ constexpr int kAppendUnroll = 4;
 // One token of 320 sequences 2.2 us, a launch.
 template <typename U>
 __global__ void __launch_bounds__(256) kv_append_kernel(const AppendArgs a) {
+  pdl_begin();
   const int seq = blockIdx.y;
   const int len = a.lens[seq];
   int count = a.counts ? a.counts[seq] : a.n_tokens;
@@ -251,7 +252,7 @@ __device__ __forceinline__ unsigned long long keeper_rank(int now, int i) {
 // do not fit one CTA's shared memory. Measured (B200): 58 K table entries 31 us.
 __global__ void __launch_bounds__(kPlanThreads, 1) kv_fork_kernel(const ForkArgs a) {
   __shared__ int64_t part[33];
-  pdl_launch_dependents();
+  pdl_begin();
   const int cta = blockIdx.x;
   const int tid = cta * kPlanThreads + threadIdx.x;
   constexpr int kAll = kPlanCtas * kPlanThreads;
@@ -415,7 +416,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_fork_cta_kernel(const Fork
   extern __shared__ __align__(16) int32_t words[];
   __shared__ int64_t part[33];
   __shared__ int n_copies, taken;
-  pdl_launch_dependents();
+  pdl_begin();
   const int tid = threadIdx.x;
   const int n_entries = a.n_seqs * a.width, ps = a.page_size;
   unsigned long long* keeper = reinterpret_cast<unsigned long long*>(words);   // n_pages
@@ -555,7 +556,7 @@ struct CompactArgs {
 // arrays in global memory, for pools that do not fit one CTA's shared memory.
 __global__ void __launch_bounds__(kPlanThreads, 1) kv_compact_kernel(const CompactArgs a) {
   __shared__ int64_t part[33];
-  pdl_launch_dependents();
+  pdl_begin();
   const int cta = blockIdx.x;
   const int64_t tid = cta * kPlanThreads + threadIdx.x;
   constexpr int kAll = kPlanCtas * kPlanThreads;
@@ -645,7 +646,7 @@ __host__ __device__ constexpr int64_t compact_words(int64_t n_pages) { return 4 
 __global__ void __launch_bounds__(kPlanThreads, 1) kv_compact_cta_kernel(const CompactArgs a) {
   extern __shared__ __align__(16) int32_t words[];
   __shared__ int64_t part[33];
-  pdl_launch_dependents();
+  pdl_begin();
   const int tid = threadIdx.x;
   int32_t *refs = words, *holes = refs + a.n_pages, *movers = holes + a.n_pages,
           *remap = movers + a.n_pages;
@@ -730,7 +731,7 @@ constexpr int kCopyPart = kCopyThreads * kCopyUnroll;   // 16-byte chunks
 // plan, 5.5 TB/s; 16 KiB parts and 4 loads in flight 132, but 30 against 27 us for
 // the 77 MB of 320 beams.
 __global__ void __launch_bounds__(kCopyThreads, kCopyResident) kv_copy_kernel(const CopyArgs a) {
-  pdl_wait();   // the plan
+  pdl_begin();   // waits for the plan
   const int which = blockIdx.y & 1, layer = blockIdx.y >> 1;
   const int units = *a.n_copies * a.n_parts;   // at most the pool's pages * n_parts
   for (int u = blockIdx.x; u < units; u += gridDim.x) {
@@ -790,21 +791,6 @@ int check_pool(const char* what, const void* k, const void* v, int64_t page_stri
   return WX_OK;
 }
 
-template <typename Args>
-static cudaError_t launch_cluster(void (*kernel)(Args), const Args& a, cudaStream_t st) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(kPlanCtas);
-  cfg.blockDim = dim3(kPlanThreads);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = kPlanCtas;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, a);
-}
-
 // The one-CTA forms' bound: what one CTA reads before a cluster of eight overtakes it,
 // within its shared memory.
 constexpr int64_t kCtaEntries = 16384;
@@ -822,7 +808,7 @@ static cudaError_t launch_cta(void (*kernel)(Args), std::atomic<uint64_t>& done,
     if (e != cudaSuccess) return e;
     if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
   }
-  return launch_k(kernel, dim3(1), dim3(kPlanThreads), (size_t)words * 4, st, a);
+  return launch_after(kernel, dim3(1), kPlanThreads, (int)words * 4, 1, st, a);
 }
 
 struct Pool {
@@ -862,9 +848,8 @@ static int launch_copies(const char* what, const Pool& p, const PlanSpace& ws,
   a.by_part = Div((uint32_t)a.n_parts);
   const int64_t units = max_copies * a.n_parts, y = 2 * p.n_layers;
   const int64_t most = std::max<int64_t>(1, (int64_t)sm_count() * kCopyResident / y);
-  PdlScope pdl(true);
-  WX_CUDA_TRY(launch_k(kv_copy_kernel, dim3((unsigned)std::min(units, most), (unsigned)y),
-                       dim3(kCopyThreads), 0, st, a));
+  WX_CUDA_TRY(launch_after(kv_copy_kernel, dim3((unsigned)std::min(units, most), (unsigned)y),
+                           kCopyThreads, 0, 1, st, a));
   return check_launch(what);
 }
 
@@ -939,11 +924,11 @@ int wx_kv_append(const void* k, const void* v, int64_t src_seq_stride, int64_t s
   const dim3 grid((unsigned)(blocks < 65536 ? blocks : 65536), (unsigned)n_seqs, 2);
   cudaStream_t st = as_stream(stream);
   if (vec)
-    WX_CUDA_TRY(launch_k(kv_append_kernel<uint4>, grid, dim3(256), 0, st, a));
+    WX_CUDA_TRY(launch_after(kv_append_kernel<uint4>, grid, 256, 0, 1, st, a));
   else if (es == 2)
-    WX_CUDA_TRY(launch_k(kv_append_kernel<uint16_t>, grid, dim3(256), 0, st, a));
+    WX_CUDA_TRY(launch_after(kv_append_kernel<uint16_t>, grid, 256, 0, 1, st, a));
   else
-    WX_CUDA_TRY(launch_k(kv_append_kernel<uint32_t>, grid, dim3(256), 0, st, a));
+    WX_CUDA_TRY(launch_after(kv_append_kernel<uint32_t>, grid, 256, 0, 1, st, a));
   return check_launch("kv_append");
 }
 
@@ -994,7 +979,7 @@ int wx_kv_fork(void* k_cache, void* v_cache, int64_t n_layers, int64_t layer_str
   if (n_seqs * width <= kCtaEntries && words <= kCtaWords)
     WX_CUDA_TRY(launch_cta(kv_fork_cta_kernel, ready, a, words, st));
   else
-    WX_CUDA_TRY(launch_cluster(kv_fork_kernel, a, st));
+    WX_CUDA_TRY(launch_after(kv_fork_kernel, dim3(kPlanCtas), kPlanThreads, 0, kPlanCtas, st, a));
   WX_TRY(check_launch("kv_fork"));
   if (!grow) return WX_OK;   // nothing is written, so nothing is copied
   const Pool p = {k_cache, v_cache, n_layers, layer_stride, page_stride, tok_stride,
@@ -1035,7 +1020,8 @@ int wx_kv_compact(void* k_cache, void* v_cache, int64_t n_layers, int64_t layer_
   if (a.n_entries <= kCtaEntries && words <= kCtaWords)
     WX_CUDA_TRY(launch_cta(kv_compact_cta_kernel, ready, a, words, st));
   else
-    WX_CUDA_TRY(launch_cluster(kv_compact_kernel, a, st));
+    WX_CUDA_TRY(
+        launch_after(kv_compact_kernel, dim3(kPlanCtas), kPlanThreads, 0, kPlanCtas, st, a));
   WX_TRY(check_launch("kv_compact"));
   const Pool p = {k_cache, v_cache, n_layers, layer_stride, page_stride, tok_stride,
                   head_stride, n_heads, head_dim, page_size, dtype};

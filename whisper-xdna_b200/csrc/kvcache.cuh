@@ -1,5 +1,6 @@
 // Shared by the operators on the paged key-value cache.
 #pragma once
+#include "common.cuh"
 #include "wxb200_internal.h"
 
 namespace wx {
@@ -20,6 +21,52 @@ struct Div {
   }
 #endif
 };
+
+// The decoder's kernels are launched one after another, each of a few microseconds, so
+// each is a programmatic dependent of the kernel before it on the stream: it may take
+// its place while that one ends. pdl_begin() comes before a kernel's first access to
+// memory: it returns when all that was on the stream before is complete and visible,
+// and then lets the next kernel be placed. Every thread calls it, so that a kernel that
+// is complete stands for all before it. (The long kernels call pdl_wait() there, and
+// pdl_launch_dependents() when their loops are done.)
+#ifdef __CUDACC__
+__device__ __forceinline__ void pdl_begin() {
+  pdl_wait();
+  pdl_launch_dependents();
+}
+#endif
+
+// Launches a kernel so, or (early false) once the stream's last kernel has ended, in
+// clusters of `cluster` CTAs along x.
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch(bool early, void (*kernel)(KArgs...), dim3 grid, int threads, int smem,
+                          int cluster, cudaStream_t st, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (early) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = (unsigned)cluster;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    n++;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = (unsigned)n;
+  return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_after(void (*kernel)(KArgs...), dim3 grid, int threads, int smem,
+                                int cluster, cudaStream_t st, Args&&... args) {
+  return launch(true, kernel, grid, threads, smem, cluster, st, std::forward<Args>(args)...);
+}
 
 // Checks a pool's types, sizes, strides (elements) and alignment.
 int check_pool(const char* what, const void* k, const void* v, int64_t page_stride,

@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(kPagedThreads, 4) paged_attention_fma_kernel(c
   extern __shared__ __align__(128) char smem[];
   __shared__ float sh_m[kPagedWarps][GT], sh_l[kPagedWarps][GT];
   __shared__ __align__(16) float sh_p[kPagedWarps][Cfg::kTok * GT];
-  pdl_launch_dependents();   // the join waits for this kernel's end
+  pdl_wait();
 
   const PagedItem it = paged_item<WPI, GT, Cfg::kTok>(a);
   // nothing to do; in a cluster the others still wait for this CTA
@@ -476,6 +476,7 @@ __global__ void __launch_bounds__(kPagedThreads, 4) paged_attention_fma_kernel(c
       }
   }
   cp_async_wait<0>();
+  pdl_launch_dependents();
   item_sync<WPI>();   // the item's rings become its warps' parts of o
 
   float* part = reinterpret_cast<float*>(smem + (WPI == 1 ? w * Cfg::kWarpBytes : 0));
@@ -566,7 +567,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_mma_kernel(cons
   constexpr int kLoads = kTok * kCpr / 32;                         // a lane, K or V
   extern __shared__ __align__(128) char smem[];
   __shared__ float sh_m[kPagedWarps][kRows], sh_l[kPagedWarps][kRows];
-  pdl_launch_dependents();   // the join waits for this kernel's end
+  pdl_wait();
 
   const PagedItem it = paged_item<WPI, kRows, kTok>(a);
   // nothing to do; in a cluster the others still wait for this CTA
@@ -738,6 +739,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_mma_kernel(cons
     for (int j = 0; j + 1 < Cfg::kStages; j++) live[j] = live[j + 1];
   }
   cp_async_wait<0>();
+  pdl_launch_dependents();
   item_sync<WPI>();   // the item's rings become its warps' parts of o
 
   float* part = reinterpret_cast<float*>(smem + (WPI == 1 ? w * Cfg::kWarpBytes : 0));
@@ -772,6 +774,7 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(kPagedThreads) paged_attention_join_rows_kernel(
     const PagedArgs a, int64_t rows) {
   constexpr int N = HD / 32;
+  pdl_begin();
   const int64_t r = (int64_t)blockIdx.x * kPagedWarps + warp_id();
   if (r >= rows) return;
   const int lane = lane_id();
@@ -781,7 +784,6 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_join_rows_kerne
   int first, end;
   key_range(a, seq, &first, &end);
   const float2* ml = a.part_ml + r * a.splits;
-  pdl_wait();
   const int chunk = a.chunk >= kMaxChunk ? a.chunk : *a.picked;
   const int s0 = first / chunk, s1 = first < end ? (end + chunk - 1) / chunk : s0;
   // lane s - s32 holds split s
@@ -830,6 +832,7 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(const PagedArgs a) {
   constexpr int N = HD / 32;
   __shared__ float sh[kJoinWarps], sh_o[kJoinWarps][HD];
+  pdl_begin();
   const int64_t r = blockIdx.x;
   const int lane = lane_id(), w = warp_id();
   const int g = (int)(r % a.group);
@@ -838,7 +841,6 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(cons
   int first, end;
   key_range(a, seq, &first, &end);
   const float2* ml = a.part_ml + r * a.splits;
-  pdl_wait();
   const int chunk = a.chunk >= kMaxChunk ? a.chunk : *a.picked;
   const int s0 = first / chunk, s1 = first < end ? (end + chunk - 1) / chunk : s0;
   auto over_warps = [&](float x, bool max) {   // every thread gets it
@@ -903,6 +905,7 @@ struct PagedCut {
 };
 constexpr int64_t kShortKeys = 256, kShortItems = 8 * 148;
 constexpr int64_t kClusterKeys = 4096;
+constexpr int64_t kEarlyKeys = 65536;
 constexpr int64_t kMinChunk = 128, kChunkCtas = 32 * 148;
 constexpr int64_t kMostParts = 32768;   // bounds the workspace of many long sequences
 
@@ -967,24 +970,13 @@ static cudaError_t launch_paged(PagedArgs a, const PagedCut& c, int smem, cudaSt
   if (c.chunk == 0 && c.warps > 1)
     while (a.splits < 8 && n_items * a.splits * 2 <= ctas && a.max_len >= 128 * a.splits)
       a.splits *= 2;
-  if (c.warps == 1) {
-    return launch_k(kernel, dim3((unsigned)((n_items + kPagedWarps - 1) / kPagedWarps)),
-                    dim3(kPagedThreads), smem, st, a);
-  }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(a.splits * a.tiles), (unsigned)a.n_heads, (unsigned)a.n_seqs);
-  cfg.blockDim = dim3(kPagedThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  if (c.chunk == 0 && a.splits > 1) {
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)a.splits;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-  }
-  return cudaLaunchKernelEx(&cfg, kernel, a);
+  dim3 grid((unsigned)(a.splits * a.tiles), (unsigned)a.n_heads, (unsigned)a.n_seqs);
+  if (c.warps == 1) grid = dim3((unsigned)((n_items + kPagedWarps - 1) / kPagedWarps));
+  // Placed while the kernel before it ends, a wave of CTAs lands on the SMs that are free
+  // first, unevenly: 33.5 us became 36.8 (64 items of 4096 keys). A call of a few us
+  // gains the one that a launch costs: one clip's frames, 7.1 us, take 6.7.
+  const bool early = n_items * a.max_len <= kEarlyKeys;
+  return launch(early, kernel, grid, kPagedThreads, smem, c.chunk == 0 ? a.splits : 1, st, a);
 }
 
 template <int HD>
@@ -1017,13 +1009,12 @@ static cudaError_t run_paged(const PagedArgs& a, const PagedCut& c, cudaStream_t
     e = c.warps == 1 ? run_fma<HD, 1>(a, c, st) : run_fma<HD, 4>(a, c, st);
   if (e != cudaSuccess || c.chunk == 0) return e;
   const int64_t rows = (int64_t)a.n_seqs * a.n_heads * a.group;
-  PdlScope pdl(true);
   if (rows >= kJoinRows)
-    return launch_k(paged_attention_join_rows_kernel<T, HD>,
-                    dim3((unsigned)((rows + kPagedWarps - 1) / kPagedWarps)),
-                    dim3(kPagedThreads), 0, st, a, rows);
-  return launch_k(paged_attention_join_kernel<T, HD>, dim3((unsigned)rows), dim3(kJoinThreads), 0,
-                  st, a);
+    return launch_after(paged_attention_join_rows_kernel<T, HD>,
+                        dim3((unsigned)((rows + kPagedWarps - 1) / kPagedWarps)), kPagedThreads, 0,
+                        1, st, a, rows);
+  return launch_after(paged_attention_join_kernel<T, HD>, dim3((unsigned)rows), kJoinThreads, 0, 1,
+                      st, a);
 }
 
 static int check_cut(const char* what, int64_t n_seqs, int64_t n_heads, int64_t group,

@@ -11,6 +11,7 @@
 #include <cstdint>
 
 #include "common.cuh"
+#include "kvcache.cuh"
 
 namespace wx {
 
@@ -314,6 +315,7 @@ __global__ void __launch_bounds__(kScoreThreads, 4) token_score_kernel(const Sco
   const int64_t row = blockIdx.y;
   const T* x = static_cast<const T*>(a.logits) + row * a.ld;
   const float c = 1.4426950408889634f * a.inv_t;
+  pdl_wait();
 
   // the elements before the first and past the last whole vector are left for the
   // end
@@ -404,6 +406,7 @@ __global__ void __launch_bounds__(kScoreThreads, 4) token_score_kernel(const Sco
         u2 = __ffma2_rn(p, d, u2);
       }
   }
+  pdl_launch_dependents();
   // the row's edges
   uint64_t edge = 0;
   if (rank == 0 && w == 0) {
@@ -511,17 +514,8 @@ static_assert(kScoreMaxCtas * kScoreMaxTop <= kCandidates, "");
 
 template <typename T, bool TOP>
 static cudaError_t launch_score(const ScoreArgs& a, int ctas, int64_t rows, cudaStream_t st) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)ctas, (unsigned)rows);
-  cfg.blockDim = dim3(kScoreThreads);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)ctas;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, token_score_kernel<T, TOP>, a);
+  return launch_after(token_score_kernel<T, TOP>, dim3((unsigned)ctas, (unsigned)rows),
+                      kScoreThreads, 0, ctas, st, a);
 }
 
 }  // namespace wx
