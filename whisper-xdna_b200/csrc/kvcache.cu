@@ -135,6 +135,49 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* part, int64_t*
 }
 static_assert(kPlanThreads == 1024, "block_scan: a warp scans the warps' sums");
 
+// The one-CTA plans' scans: two 32-bit values side by side, exclusive, in place; their
+// sums in a0 and b0. `part` is 66 words.
+__device__ __forceinline__ void block_scan2(uint32_t& a, uint32_t& b, uint32_t* part, uint32_t* a0,
+                                            uint32_t* b0) {
+  const int lane = lane_id(), w = warp_id();
+  const uint32_t a_in = a, b_in = b;
+  auto warp_scan = [&](uint32_t& x, uint32_t& y) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t u = __shfl_up_sync(0xffffffffu, x, o), v = __shfl_up_sync(0xffffffffu, y, o);
+      if (lane >= o) {
+        x += u;
+        y += v;
+      }
+    }
+  };
+  warp_scan(a, b);
+  if (lane == 31) {
+    part[w + 1] = a;
+    part[33 + w + 1] = b;
+  }
+  __syncthreads();
+  if (w == 0) {
+    uint32_t x = part[lane + 1], y = part[33 + lane + 1];
+    warp_scan(x, y);
+    part[lane + 1] = x;
+    part[33 + lane + 1] = y;
+    if (lane == 0) part[0] = part[33] = 0;
+  }
+  __syncthreads();
+  *a0 = part[32];
+  *b0 = part[33 + 32];
+  a += part[w] - a_in;
+  b += part[33 + w] - b_in;
+}
+// The sum of every thread's value; `part` is 32 words, not in use before.
+__device__ __forceinline__ uint32_t block_sum(uint32_t v, uint32_t* part) {
+  v = __reduce_add_sync(0xffffffffu, v);
+  if (lane_id() == 0) part[warp_id()] = v;
+  __syncthreads();
+  return __reduce_add_sync(0xffffffffu, part[lane_id()]);
+}
+
 // One page copy: the first n_tok tokens of page src, every layer and head.
 struct PageCopy {
   int32_t src, dst, n_tok, pad;
@@ -225,9 +268,8 @@ __device__ __forceinline__ void fork_refs(const ForkArgs& a, int32_t* refs, int 
   if (was >= 0 && was < a.n_pages) atomicSub(refs + was, 1);
   if (is >= 0) atomicAdd(refs + is, 1);
 }
-// the tokens that sequence i is to grow by, as far as its row has room
-__device__ __forceinline__ int fork_grow(const ForkArgs& a, int i, int now) {
-  const int g = a.grow ? a.grow[i] : 0;
+// the tokens that a sequence of `now` is to grow by, as far as its row has room for g
+__device__ __forceinline__ int fork_grow(const ForkArgs& a, int g, int now) {
   return g > 0 && (int64_t)now + g <= (int64_t)a.width * a.page_size ? g : 0;
 }
 __device__ __forceinline__ unsigned long long keeper_rank(int now, int i) {
@@ -288,7 +330,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_fork_kernel(const ForkArgs
   for (int i = tid; i < a.n_seqs; i += kAll) {
     const int now = __ldcg(a.lens_out + i);
     const int col = a.by_page(now);
-    if (now == col * ps || !fork_grow(a, i, now)) continue;
+    if (now == col * ps || !fork_grow(a, a.grow ? a.grow[i] : 0, now)) continue;
     const int page = __ldcg(a.table_out + (int64_t)i * a.width + col);
     if (page >= 0 && __ldcg(a.refs_out + page) > 1) atomicMax(a.ws.column + page, col + 1);
   }
@@ -308,7 +350,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_fork_kernel(const ForkArgs
 
   // 5
   for (int i = tid; i < a.n_seqs; i += kAll) {
-    const int now = __ldcg(a.lens_out + i), grow = fork_grow(a, i, now);
+    const int now = __ldcg(a.lens_out + i), grow = fork_grow(a, a.grow ? a.grow[i] : 0, now);
     int need = 0;
     if (grow) {
       const int col = a.by_page(now);
@@ -367,7 +409,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_fork_kernel(const ForkArgs
 
   // 7
   for (int i = gw; i < a.n_seqs; i += kWarps) {
-    const int now = __ldcg(a.lens_out + i), grow = fork_grow(a, i, now);
+    const int now = __ldcg(a.lens_out + i), grow = fork_grow(a, a.grow ? a.grow[i] : 0, now);
     const int asked = __ldcg(a.ws.need + i), need = asked & ~kNeedsCopy;
     const int64_t scan = __ldcg(a.ws.scan + i), before = scan >> 32;
     const bool granted = grow && (need == 0 || before + need <= n_free);
@@ -404,17 +446,17 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_fork_kernel(const ForkArgs
 
 // Words of shared memory that the one-CTA form of a fork takes.
 __host__ __device__ constexpr int64_t fork_words(int64_t n_seqs, int64_t width, int64_t n_pages) {
-  return 2 * n_seqs * width + 6 * n_pages + 4 * n_seqs + 2;
+  return 2 * n_seqs * width + 6 * n_pages + 5 * n_seqs + 2;
 }
 
 // The same plan by one CTA, its arrays in shared memory: a phase costs a barrier and
 // not a trip through L2. Bound by one SM's instruction issue as the table grows.
 // Measured (B200), with the copies' launch, here against the cluster's form: 5 beams
-// 7.9 and 16.2 us, 320 beams (4800 entries, 77 MB copied) 27 and 35, 256 sequences
-// of 57 pages (14.6 K entries) 17.2 and 18.4: kCtaEntries is where they meet.
+// 6.7 and 16 us, 320 beams (4800 entries, 77 MB copied) 25 and 35, 256 sequences of
+// 57 pages (14.6 K entries) 16.6 and 18.4: kCtaEntries is about where they meet.
 __global__ void __launch_bounds__(kPlanThreads, 1) kv_fork_cta_kernel(const ForkArgs a) {
   extern __shared__ __align__(16) int32_t words[];
-  __shared__ int64_t part[33];
+  __shared__ uint32_t part[66];
   __shared__ int n_copies, taken;
   pdl_begin();
   const int tid = threadIdx.x;
@@ -425,25 +467,59 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_fork_cta_kernel(const Fork
   int32_t *is = list + a.n_pages, *was = is + n_entries;      // rows after and before
   int32_t *len = was + n_entries, *need = len + a.n_seqs;
   int32_t *pages_before = need + a.n_seqs, *copies_before = pages_before + a.n_seqs;
+  int32_t* grow_by = copies_before + a.n_seqs;
 
-  // 1: parents' rows as they stand, lengths, counts
-#pragma unroll 4
-  for (int e = tid; e < n_entries; e += kPlanThreads) {
-    const int i = a.by_width(e), par = a.parents ? a.parents[i] : i;
-    is[e] = a.table[par < 0 || par >= a.n_seqs ? e : e + (par - i) * a.width];
-    was[e] = a.table[e];
+  // 1: counts, lengths and parents' rows as they stand. The loads that do not hang on
+  // one another go first, so that two trips to memory are waited for and not six.
+  constexpr int kAhead = 4;
+  int par0 = tid, grow0 = 0, refs0 = 0, from[kAhead], now[kAhead], then[kAhead];
+  if (tid < a.n_seqs) {
+    if (a.parents) par0 = a.parents[tid];
+    if (a.grow) grow0 = a.grow[tid];
   }
-#pragma unroll 4
+  if (tid < a.n_pages) refs0 = a.refs[tid];
+  auto parent_of = [&](int e) {
+    return e < n_entries && a.parents ? a.parents[a.by_width(e)] : a.by_width(e);
+  };
+#pragma unroll
+  for (int j = 0; j < kAhead; j++) from[j] = parent_of(tid + j * kPlanThreads);
+  for (int e0 = tid; e0 < n_entries; e0 += kPlanThreads * kAhead) {
+#pragma unroll
+    for (int j = 0; j < kAhead; j++) {
+      const int e = e0 + j * kPlanThreads, i = a.by_width(e);
+      if (e >= n_entries) continue;
+      now[j] = a.table[from[j] < 0 || from[j] >= a.n_seqs ? e : e + (from[j] - i) * a.width];
+      then[j] = a.table[e];
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; j++) from[j] = parent_of(e0 + (j + kAhead) * kPlanThreads);
+    if (e0 == tid && tid < a.n_seqs) {
+      if (par0 >= a.n_seqs) kv_error();
+      len[tid] = fork_length(a, par0 >= a.n_seqs || par0 < 0 ? -1 : par0);
+      grow_by[tid] = grow0;
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; j++) {
+      const int e = e0 + j * kPlanThreads;
+      if (e >= n_entries) continue;
+      is[e] = now[j];
+      was[e] = then[j];
+    }
+  }
+  for (int i = tid + kPlanThreads; i < a.n_seqs; i += kPlanThreads) {
+    len[i] = fork_length(a, fork_parent(a, i));
+    grow_by[i] = a.grow ? a.grow[i] : 0;
+  }
   for (int p = tid; p < a.n_pages; p += kPlanThreads) {
-    refs[p] = a.refs[p];
+    refs[p] = p == tid ? refs0 : a.refs[p];
     keeper[p] = 0;
     sharers[p] = column[p] = 0;
   }
-  for (int i = tid; i < a.n_seqs; i += kPlanThreads) len[i] = fork_length(a, fork_parent(a, i));
   if (tid == 0) n_copies = taken = 0;
   __syncthreads();
 
   // 2
+#pragma unroll 4
   for (int e = tid; e < n_entries; e += kPlanThreads) {
     const int i = a.by_width(e), page = fork_entry(a, is[e], e - i * a.width, len[i]);
     is[e] = page;
@@ -454,13 +530,14 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_fork_cta_kernel(const Fork
   // 3
   for (int i = tid; i < a.n_seqs; i += kPlanThreads) {
     const int now = len[i], col = a.by_page(now);
-    if (now == col * ps || !fork_grow(a, i, now)) continue;
+    if (now == col * ps || !fork_grow(a, grow_by[i], now)) continue;
     const int page = is[i * a.width + col];
     if (page >= 0 && refs[page] > 1) atomicMax(column + page, col + 1);
   }
   __syncthreads();
 
   // 4
+#pragma unroll 4
   for (int e = tid; e < n_entries; e += kPlanThreads) {
     const int page = is[e];
     if (page < 0 || column[page] == 0) continue;
@@ -474,9 +551,11 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_fork_cta_kernel(const Fork
   // 5 and 6: each thread a run of sequences and of pages
   const int per = (a.n_seqs + kPlanThreads - 1) / kPlanThreads;
   const int i0 = min(a.n_seqs, tid * per), i1 = min(a.n_seqs, i0 + per);
-  int64_t asked = 0;   // pages, and the copies among them in the low half
+  // pages asked for, and the copies among them in the low 15 bits: with at most 2^14
+  // entries neither passes its field
+  uint32_t asked = 0;
   for (int i = i0; i < i1; i++) {
-    const int now = len[i], grow = fork_grow(a, i, now);
+    const int now = len[i], grow = fork_grow(a, grow_by[i], now);
     int n = 0;
     if (grow) {
       const int col = a.by_page(now);
@@ -488,30 +567,28 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_fork_cta_kernel(const Fork
         n = (n + 1) | kNeedsCopy;
     }
     need[i] = n;
-    asked += ((int64_t)(n & ~kNeedsCopy) << 32) | (n & kNeedsCopy ? 1 : 0);
+    asked += ((uint32_t)(n & ~kNeedsCopy) << 15) | (n & kNeedsCopy ? 1 : 0);
   }
   const int per_p = (a.n_pages + kPlanThreads - 1) / kPlanThreads;
   const int p0 = min(a.n_pages, tid * per_p), p1 = min(a.n_pages, p0 + per_p);
-  int free = 0;
+  uint32_t free = 0, total, n_free;
   for (int p = p0; p < p1; p++) free += refs[p] == 0;
-  int64_t total, n_free;
-  int64_t at = block_scan(asked, part, &total) - asked;
+  block_scan2(asked, free, part, &total, &n_free);
   for (int i = i0; i < i1; i++) {
-    pages_before[i] = (int)min(at >> 32, (int64_t)0x7fffffff);
-    copies_before[i] = (int)at;
-    at += ((int64_t)(need[i] & ~kNeedsCopy) << 32) | (need[i] & kNeedsCopy ? 1 : 0);
+    pages_before[i] = (int)(asked >> 15);
+    copies_before[i] = (int)(asked & 0x7fff);
+    asked += ((uint32_t)(need[i] & ~kNeedsCopy) << 15) | (need[i] & kNeedsCopy ? 1 : 0);
   }
-  at = block_scan(free, part, &n_free) - free;
   for (int p = p0; p < p1; p++)
-    if (refs[p] == 0) list[at++] = p;
+    if (refs[p] == 0) list[free++] = p;
   __syncthreads();
 
   // 7
   for (int i = tid; i < a.n_seqs; i += kPlanThreads) {
-    const int now = len[i], grow = fork_grow(a, i, now);
+    const int now = len[i], grow = fork_grow(a, grow_by[i], now);
     const int n = need[i] & ~kNeedsCopy, copy = need[i] & kNeedsCopy ? 1 : 0;
     const int before = pages_before[i];
-    const bool granted = grow && (n == 0 || (int64_t)before + n <= n_free);
+    const bool granted = grow && (n == 0 || before + n <= (int)n_free);
     a.lens_out[i] = granted ? now + grow : now;
     if (a.grown) a.grown[i] = granted ? grow : 0;
     if (!granted || n == 0) continue;
@@ -536,10 +613,10 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_fork_cta_kernel(const Fork
   for (int e = tid; e < n_entries; e += kPlanThreads) a.table_out[e] = is[e];
   for (int p = tid; p < a.n_pages; p += kPlanThreads) a.refs_out[p] = refs[p];
   if (tid == 0) {
-    const int64_t pages = total >> 32;
+    const int pages = (int)(total >> 15);
     *a.ws.n_copies = n_copies;
     a.status[0] = (int)n_free - taken;
-    a.status[1] = (int)(pages > n_free ? pages - n_free : 0);
+    a.status[1] = max(pages - (int)n_free, 0);
   }
 }
 
@@ -642,10 +719,10 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_compact_kernel(const Compa
 __host__ __device__ constexpr int64_t compact_words(int64_t n_pages) { return 4 * n_pages; }
 
 // The same by one CTA, its arrays in shared memory. Measured (B200): 96 pages, 11 of
-// them moved, 5.8 us with the copies; in the cluster's form 13.1.
+// them moved, 4.9 us with the copies; in the cluster's form 13.1.
 __global__ void __launch_bounds__(kPlanThreads, 1) kv_compact_cta_kernel(const CompactArgs a) {
   extern __shared__ __align__(16) int32_t words[];
-  __shared__ int64_t part[33];
+  __shared__ uint32_t part[66], sums[32];
   pdl_begin();
   const int tid = threadIdx.x;
   int32_t *refs = words, *holes = refs + a.n_pages, *movers = holes + a.n_pages,
@@ -656,24 +733,19 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_compact_cta_kernel(const C
   // each thread a run of pages
   const int per = (a.n_pages + kPlanThreads - 1) / kPlanThreads;
   const int p0 = min(a.n_pages, tid * per), p1 = min(a.n_pages, p0 + per);
-  int n = 0;
+  uint32_t n = 0;
   for (int p = p0; p < p1; p++) n += refs[p] > 0;
-  int64_t total;
-  block_scan(n, part, &total);
-  const int n_used = (int)total;
-  int64_t both = 0;   // holes, and movers in the low half
+  const int n_used = (int)block_sum(n, sums);
+  uint32_t hole = 0, mover = 0, n_holes, n_movers_u;
   for (int p = p0; p < p1; p++) {
-    if (p < n_used && refs[p] <= 0) both += 1ll << 32;
-    if (p >= n_used && refs[p] > 0) both += 1;
+    hole += p < n_used && refs[p] <= 0;
+    mover += p >= n_used && refs[p] > 0;
   }
-  int64_t at = block_scan(both, part, &total) - both;
-  const int n_movers = (int)total;
+  block_scan2(hole, mover, part, &n_holes, &n_movers_u);
+  const int n_movers = (int)n_movers_u;
   for (int p = p0; p < p1; p++) {
-    if (p < n_used && refs[p] <= 0) {
-      holes[at >> 32] = p;
-      at += 1ll << 32;
-    }
-    if (p >= n_used && refs[p] > 0) movers[(int)at++] = p;
+    if (p < n_used && refs[p] <= 0) holes[hole++] = p;
+    if (p >= n_used && refs[p] > 0) movers[mover++] = p;
   }
   __syncthreads();
   for (int m = tid; m < n_movers; m += kPlanThreads) {
@@ -728,8 +800,8 @@ constexpr int kCopyPart = kCopyThreads * kCopyUnroll;   // 16-byte chunks
 // Source and target pages are never the same page, nor is a target another copy's
 // source: plans copy pages in use to free ones. Bound by the memory's bandwidth, read
 // + write. Measured (B200): 734 MB (700 pages of 64 KB in 4 layers) 134 us with the
-// plan, 5.5 TB/s; 16 KiB parts and 4 loads in flight 132, but 30 against 27 us for
-// the 77 MB of 320 beams.
+// plan, 5.5 TB/s; 16 KiB parts and 4 loads in flight 132, but 30 against 27 us
+// for a fork of 320 beams (77 MB).
 __global__ void __launch_bounds__(kCopyThreads, kCopyResident) kv_copy_kernel(const CopyArgs a) {
   pdl_begin();   // waits for the plan
   const int which = blockIdx.y & 1, layer = blockIdx.y >> 1;
@@ -795,6 +867,7 @@ int check_pool(const char* what, const void* k, const void* v, int64_t page_stri
 // within its shared memory.
 constexpr int64_t kCtaEntries = 16384;
 constexpr int64_t kCtaWords = 220 * 1024 / 4;
+static_assert(kCtaEntries <= 1 << 14, "a fork's running sums: 17 and 15 bits");
 
 template <typename Args>
 static cudaError_t launch_cta(void (*kernel)(Args), std::atomic<uint64_t>& done, const Args& a,
