@@ -278,7 +278,7 @@ int wx_kv_compact(void* k_cache, void* v_cache, int64_t n_layers, int64_t layer_
  * row without keys (or with all scores -inf) gives o = 0 and lse = -inf. q, the
  * cache and out are of one dtype; head_dim 64 or 128; sums in fp32, the
  * result rounded once.
- * max_len: an upper bound of lens, at most ld_table * page_size (longer
+ * max_len: an upper bound of lens, at most ld_table * page_size and 2^29 (longer
  * sequences are cut there, WX_DEVERR_PAGE): it shapes the launch. The workspace
  * (wx_paged_attention_workspace bytes, 16-byte aligned; may be 0) needs no
  * preparation; calls that may overlap each need their own. */

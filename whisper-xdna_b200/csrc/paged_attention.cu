@@ -305,7 +305,7 @@ struct FmaCfg {
 // to all lanes through shared memory.
 //
 // Measured (B200): 43.7 K keys of a window, 2 heads of 128 with 8 query rows each (89
-// MB) 30 us with the join, 3.0 TB/s: bound by the issue of some 140 instructions a key
+// MB) 29 us with the join, 3.1 TB/s: bound by the issue of some 140 instructions a key
 // at 0.5 a cycle. One row at a time, keys straight to registers and five shuffles a
 // score, took 64.
 template <int HD, int GT, int WPI>
@@ -557,8 +557,8 @@ struct MmaCfg {
 //
 // Bound by the memory: measured (B200), 16 clips' 1500 frames of 20 heads of 64, five
 // beams each (123 MB) 25.8 us, 4.8 TB/s; 64 clips 89 us, 5.5 TB/s; 64 sequences of 1 to
-// 16384 tokens, 8 heads of 128 with 4 query rows (504 MB) 91 us, 5.5 TB/s; 5 beams'
-// first tokens 3.3 us, a launch. Products on the FMA pipe took 110 and 200 us for the
+// 16384 tokens, 8 heads of 128 with 4 query rows (504 MB) 89 us, 5.7 TB/s; 5 beams'
+// first tokens 3.1 us, a launch. Products on the FMA pipe took 110 and 200 us for the
 // first and third; four-stage rings, with fewer CTAs on an SM, 34 and 99.
 template <int HD, int NT, int WPI>
 __global__ void __launch_bounds__(kPagedThreads) paged_attention_mma_kernel(const PagedArgs a) {
@@ -875,8 +875,8 @@ constexpr int64_t kEarlyKeys = 65536;
 constexpr int64_t kMinChunk = 128, kChunkCtas = 32 * 148;
 constexpr int64_t kMostParts = 32768;   // bounds the workspace of many long sequences
 
-static PagedCut paged_cut(int64_t n_seqs, int64_t n_heads, int64_t group, int64_t head_dim,
-                          int64_t max_len, int dtype) {
+static PagedCut paged_cut(int64_t n_seqs, int64_t n_heads, int64_t group, int64_t max_len,
+                          int dtype) {
   PagedCut c = {};
   if (dtype == WX_DTYPE_BF16) {
     c.tile = group <= 8 ? 8 : 16;
@@ -893,7 +893,7 @@ static PagedCut paged_cut(int64_t n_seqs, int64_t n_heads, int64_t group, int64_
     int64_t chunk = max_len * items / kChunkCtas;
     chunk = chunk < kMinChunk ? kMinChunk : chunk > kMaxChunk ? kMaxChunk : chunk;
     if (n_seqs > kPagedThreads) chunk = kMaxChunk;   // pick_chunk leaves it at that
-    chunk = std::max(chunk, max_len * items / kMostParts);
+    chunk = std::min(std::max(chunk, max_len * items / kMostParts), max_len);
     chunk = (chunk + 15) / 16 * 16;
     c.chunk = (int)chunk;
     c.splits = (int)((max_len + chunk - 1) / chunk);
@@ -987,7 +987,7 @@ static int check_cut(const char* what, int64_t n_seqs, int64_t n_heads, int64_t 
                      int64_t head_dim, int64_t max_len) {
   if (n_seqs < 0 || n_seqs > 65535 || n_heads < 1 || n_heads > 65535 || group < 1 ||
       group > 65535 || n_seqs * n_heads * group > 0x7fffffff || max_len < 0 ||
-      max_len > (1 << 30))
+      max_len > (1 << 29))
     return fail(WX_ERR_INVALID,
                 "%s: bad shape: %lld sequences, %lld heads, group %lld, max_len %lld", what,
                 (long long)n_seqs, (long long)n_heads, (long long)group, (long long)max_len);
@@ -1006,8 +1006,8 @@ int64_t wx_paged_attention_workspace(int64_t n_seqs, int64_t n_heads, int64_t gr
   using namespace wx;
   const int s = check_cut("paged_attention_workspace", n_seqs, n_heads, group, head_dim, max_len);
   if (s != WX_OK) return s;
-  return paged_space(n_seqs * n_heads * group, paged_cut(n_seqs, n_heads, group, head_dim, max_len, dtype),
-                     head_dim);
+  return paged_space(n_seqs * n_heads * group,
+                     paged_cut(n_seqs, n_heads, group, max_len, dtype), head_dim);
 }
 
 int wx_paged_attention(const void* q, int64_t q_seq_stride, int64_t q_head_stride,
@@ -1032,7 +1032,7 @@ int wx_paged_attention(const void* q, int64_t q_seq_stride, int64_t q_head_strid
   const int es = dtype == WX_DTYPE_BF16 ? 2 : 4;
   if (((uintptr_t)q | (uintptr_t)out) % es)
     return fail(WX_ERR_INVALID, "paged_attention: q or out not aligned to its type");
-  const PagedCut c = paged_cut(n_seqs, n_heads, group, head_dim, max_len, dtype);
+  const PagedCut c = paged_cut(n_seqs, n_heads, group, max_len, dtype);
   const int64_t rows = n_seqs * n_heads * group, want = paged_space(rows, c, head_dim);
   if (want && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < want))
     return fail(WX_ERR_INVALID,
