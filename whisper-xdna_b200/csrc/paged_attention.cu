@@ -862,14 +862,18 @@ constexpr int64_t kJoinRows = 8 * 148;   // rows from which on a warp each will 
 // long caches chunks of keys that a second kernel joins. In between, a launch splits
 // an item over a cluster where that keeps every CTA in the first wave (launch_paged).
 //
-// Measured (B200): 6400 items of up to 224 keys, a warp each 27.8 us, a CTA each 34.7.
+// Measured (B200): a warp and a CTA each for 6400 items of 10 to 224 keys of 64 in bf16
+// 27.4 and 36.7 us, of 448 keys 124 and 116, of 224 in fp32 53.7 and 50.5; for 2560 items
+// of up to 224 keys of 128 29.3 and 36.3; for 1200 items 11.3 and 9.9, 600 10.4 and 7.0.
+// Tiles of 16 rows against two of 8, 64 items of 4096 keys, 16 rows each: 31.7 and 36.2.
 // 320 items of 1500 keys, a cluster of 1, 2, 4, 8 for each: 27.3, 25.8, 31.0, 38.4 us
 // (two waves from 4 on; 3 CTAs, which divide no GPC: 33.0); 20 such items 20.3, 13.3,
-// 8.7, 7.3. 64 sequences to 16384 keys, chunks of at most 512, 1024, 2048: 98, 91, 95.
+// 8.7, 7.3. 64 sequences to 16384 keys, chunks of at most 512, 1024, 2048: 98, 91, 95;
+// their 2048 rows joined by a warp and by 32 warps each, the whole call: 89 and 127.
 struct PagedCut {
   int tile, warps, splits, chunk;
 };
-constexpr int64_t kShortKeys = 256, kShortItems = 8 * 148;
+constexpr int64_t kShortKeys = 256, kShortItems = 16 * 148;   // bf16; fp32: half the keys
 constexpr int64_t kClusterKeys = 4096;
 constexpr int64_t kEarlyKeys = 65536;
 constexpr int64_t kMinChunk = 128, kChunkCtas = 32 * 148;
@@ -887,7 +891,7 @@ static PagedCut paged_cut(int64_t n_seqs, int64_t n_heads, int64_t group, int64_
   c.splits = 1;
   c.warps = 4;
   const int64_t items = n_seqs * n_heads * ((group + c.tile - 1) / c.tile);
-  if (max_len <= kShortKeys && items >= kShortItems) {
+  if (max_len * (dtype == WX_DTYPE_BF16 ? 1 : 2) <= kShortKeys && items >= kShortItems) {
     c.warps = 1;
   } else if (max_len > kClusterKeys) {
     int64_t chunk = max_len * items / kChunkCtas;
