@@ -271,6 +271,23 @@ PyObject* kv_append(PyObject* const* a) {
   Py_RETURN_NONE;
 }
 
+// A plan's workspace: beside the outputs where it is small, since an allocation costs as
+// much host time as the rest of the call, else apart, so that it does not live as long
+// as they do.
+struct PlanSpace {
+  int64_t bytes, place = -1;
+  Tensor apart;
+  PlanSpace(Outputs& out, int64_t n_seqs, int64_t n_pages)
+      : bytes(wx_kv_workspace(n_seqs, n_pages)) {
+    if (bytes <= 1 << 18) place = out.add(bytes);
+  }
+  void* get(const Outputs& out, int dev) {
+    if (place >= 0) return out.at(place);
+    apart = empty(dev, {bytes}, at::kByte);
+    return apart.data_ptr();
+  }
+};
+
 // kv_fork(k_cache, v_cache, table, lens, refs, parents, grow)
 PyObject* kv_fork(PyObject* const* a) {
   const Pools c(a[0], a[1], 5);
@@ -279,9 +296,8 @@ PyObject* kv_fork(PyObject* const* a) {
   const int32_t* refs = ints(plain(c.dev, tensor(a[4], "refs"), "refs", at::kInt, {c.n_pages}));
   const int32_t* parents = ints(plain_or_null(c.dev, a[5], "parents", at::kInt, {table.n}));
   const int32_t* grow = ints(plain_or_null(c.dev, a[6], "grow", at::kInt, {table.n}));
-  const int64_t space = wx_kv_workspace(table.n, c.n_pages);
-  const Tensor ws = empty(c.dev, {space}, at::kByte);
   Outputs out(c.dev);
+  PlanSpace ws(out, table.n, c.n_pages);
   const int64_t t = out.add(4 * table.n * table.width), l = out.add(4 * table.n),
                 r = out.add(4 * c.n_pages), g = out.add(4 * table.n), s = out.add(8);
   out.allocate();
@@ -289,7 +305,7 @@ PyObject* kv_fork(PyObject* const* a) {
                    c.tok_stride, c.head_stride, c.n_heads, c.hd, c.n_pages, c.page, c.dtype,
                    table.p, lens, refs, parents, grow, table.n, table.width, ints(out.at(t)),
                    ints(out.at(l)), ints(out.at(r)), ints(out.at(g)), ints(out.at(s)),
-                   ws.data_ptr(), space, stream(c.dev)));
+                   ws.get(out, c.dev), ws.bytes, stream(c.dev)));
   return Py_BuildValue("(NNNNN)",
                        THPVariable_Wrap(out.tensor(t, {table.n, table.width}, at::kInt)),
                        THPVariable_Wrap(out.tensor(l, {table.n}, at::kInt)),
@@ -303,16 +319,15 @@ PyObject* kv_compact(PyObject* const* a) {
   const Pools c(a[0], a[1], 5);
   const Table table(c.dev, a[2]);
   const int32_t* refs = ints(plain(c.dev, tensor(a[3], "refs"), "refs", at::kInt, {c.n_pages}));
-  const int64_t space = wx_kv_workspace(table.n, c.n_pages);
-  const Tensor ws = empty(c.dev, {space}, at::kByte);
   Outputs out(c.dev);
+  PlanSpace ws(out, table.n, c.n_pages);
   const int64_t t = out.add(4 * table.n * table.width), r = out.add(4 * c.n_pages),
                 s = out.add(8);
   out.allocate();
   check(wx_kv_compact(c.k.data_ptr(), c.v.data_ptr(), c.n_layers, c.layer_stride, c.page_stride,
                       c.tok_stride, c.head_stride, c.n_heads, c.hd, c.n_pages, c.page, c.dtype,
                       table.p, refs, table.n, table.width, ints(out.at(t)), ints(out.at(r)),
-                      ints(out.at(s)), ws.data_ptr(), space, stream(c.dev)));
+                      ints(out.at(s)), ws.get(out, c.dev), ws.bytes, stream(c.dev)));
   return Py_BuildValue("(NNN)",
                        THPVariable_Wrap(out.tensor(t, {table.n, table.width}, at::kInt)),
                        THPVariable_Wrap(out.tensor(r, {c.n_pages}, at::kInt)),
