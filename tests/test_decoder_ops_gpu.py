@@ -217,6 +217,49 @@ def test_attend_infinite_scores(cuda, dtype, n):
     assert lse[2:].isnan().all()
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("group", [5, 8, 9, 16])
+@pytest.mark.parametrize("lens", [[1, 0, 17, 777, 4096], [6000, 0, 300]])
+def test_attend_fp32_many_rows(cuda, hd, group, lens):
+    """Groups that the tensor cores take in fp32, over a cluster and in chunks, with a
+    window that begins inside a tile."""
+    k, v, table, n, gen = make_cache(lens, 16, 2, hd, torch.float32, seed=hd + group)
+    q = randn(gen, len(lens), 2 * group, hd)
+    check_attend(q, k, v, table, n)
+    starts = torch.tensor([x // 3 for x in lens], dtype=torch.int32, device="cuda")
+    check_attend(q, k, v, table, n, starts=starts)
+
+
+@pytest.mark.parametrize("group", [2, 5, 16])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("ks,qs", [(1e37, 1e-36), (1e-37, 1e37), (1e-30, 1e30), (1.0, 1e-38)])
+def test_attend_fp32_extremes(cuda, hd, group, ks, qs):
+    """Numbers near the ends of fp32's range, whose products are ordinary."""
+    k, v, table, n, gen = make_cache([300, 33], 16, 2, hd, torch.float32, seed=group, spoil=False)
+    k *= ks
+    check_attend(randn(gen, 2, 2 * group, hd) * qs, k, v, table, n)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("group", [1, 4, 5, 16])
+@pytest.mark.parametrize("n", [40, 2000])
+def test_attend_fp32_infinite_values(cuda, hd, group, n):
+    """An infinite or NaN number of V shows in its dimension alone."""
+    k, v, table, lens, gen = make_cache([n], 16, 2, hd, torch.float32, seed=group)
+    q = randn(gen, 1, 2 * group, hd)
+    want = ops.paged_attention(q, k, v, table, lens).unflatten(1, (2, group))
+    at = table[0, (n - 5) // 16].long(), (n - 5) % 16
+    v[at][0, 3] = math.inf
+    v[at][1, 7] = -math.inf
+    v[at][1, 62] = math.nan
+    got = ops.paged_attention(q, k, v, table, lens).unflatten(1, (2, group))
+    assert (got[:, 0, :, 3] == math.inf).all() and (got[:, 1, :, 7] == -math.inf).all()
+    assert got[:, 1, :, 62].isnan().all()
+    for h, d in ((0, [3]), (1, [7, 62])):
+        keep = [x for x in range(hd) if x not in d]
+        torch.testing.assert_close(got[:, h][..., keep], want[:, h][..., keep], rtol=0, atol=1e-5)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_attend_same_result_each_time_and_anywhere_in_a_batch(cuda, dtype):
     lens = [4000, 17, 900, 4000]

@@ -304,10 +304,10 @@ struct FmaCfg {
 // ends with one (key, query row) and takes one exponential; the weights come back
 // to all lanes through shared memory.
 //
-// Measured (B200): 43.7 K keys of a window, 2 heads of 128 with 8 query rows each (89
-// MB) 29 us with the join, 3.1 TB/s: bound by the issue of some 140 instructions a key
-// at 0.5 a cycle. One row at a time, keys straight to registers and five shuffles a
-// score, took 64.
+// Measured (B200): 64 items of 4096 keys of 128, 2 and 4 rows each, 44 and 46 us (6.1 and
+// 5.9 TB/s), 8 rows 59: from there on bound by the issue of some 17 instructions a key
+// and row, and left to the tensor cores (which take 49 for 4 rows too) unless short items
+// are many: 2560 of up to 120 keys of 64, 8 rows, 35 us a warp each, 37 on them.
 template <int HD, int GT, int WPI>
 __global__ void __launch_bounds__(kPagedThreads, 4) paged_attention_fma_kernel(const PagedArgs a) {
   using Cfg = FmaCfg<HD>;
@@ -768,6 +768,358 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_mma_kernel(cons
                                         part + WPI * kRows * HD);
 }
 
+// ---------------------------------------------------------------- fp32 on tensor cores
+
+// d += a (16 x 8, row) * b (8 x 8, col), tf32 in (fp32 whose lowest 13 bits are 0),
+// fp32 out
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const float (&a)[4], float b0, float b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(__float_as_uint(a[0])), "r"(__float_as_uint(a[1])), "r"(__float_as_uint(a[2])),
+        "r"(__float_as_uint(a[3])), "r"(__float_as_uint(b0)), "r"(__float_as_uint(b1)));
+}
+// x in two parts of 11 bits, the first rounded (to infinity at the very top, which the
+// kernel meets as it does infinities), the second cut: within 2^-22 of x together. NaN
+// stays NaN in the second.
+__device__ __forceinline__ float tf32_hi(float x) {
+  return __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xFFFFE000u);
+}
+__device__ __forceinline__ float tf32_lo(float x, float hi) {
+  return __uint_as_float(__float_as_uint(x - hi) & 0xFFFFE000u);
+}
+__device__ __forceinline__ void split_tf32(const float (&x)[4], float (&hi)[4], float (&lo)[4]) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    hi[e] = tf32_hi(x[e]);
+    lo[e] = tf32_lo(x[e], hi[e]);
+  }
+}
+
+// outside [2^-102, 2^64], 0 aside; by exponents, since compares of floats with their
+// branches were 2 us of a call with 16 rows
+__device__ __forceinline__ bool far_from_one(float x) {
+  const uint32_t b = __float_as_uint(x) << 1;
+  return (b != 0) & (b - (25u << 24) > (166u << 24));
+}
+
+template <int HD>
+struct Tf32Cfg {
+  static constexpr int kTileBytes = kTok * HD * 4;           // K or V of one tile
+  static constexpr int kHalves = 3;                          // K and V tiles in a ring
+  static constexpr int kWarpBytes = kHalves * kTileBytes;
+  static constexpr int kQueryBytes = HD / 8 * 32 * 16;   // 8 rows in two parts or 16 whole
+  static constexpr int kSmem = kPagedWarps * kWarpBytes + kQueryBytes;
+};
+
+// Up to 8 NT query rows of one (sequence, head) against the keys of one split, fp32: the
+// products of the bf16 kernel (S^T = K Q^T, O^T = V^T P^T) on tf32 operands. Each number
+// is in two parts and three of the four products of parts are taken, the fourth being
+// below 2^-22 of a product: 2^-20 in all, a few roundings of fp32. A part below 2^-126
+// counts as 0: an error of 2^-126 |v| in a weight's share of o and of 2^-126 p in a value's,
+// and in the scores none that shows, since a query with numbers so small or so large that
+// it could (see `whole`) gets its scores as sums of whole products. A key of 128 costs
+// some 90 instructions for up to 8 rows, mostly the splitting, where the FMA kernel takes
+// 17 a row.
+//
+// A warp's ring holds K and V tiles in turn, three of them: K of the next tile is under
+// way while this tile's V waits. Which dimension stands in which column of a product is
+// free as long as both operands agree (and for V, which row), so every operand is read
+// four dimensions at a time: K's columns t and t + 4 of two steps are dimensions
+// 4 t .. 4 t + 3 of 16, V's rows g and g + 8 of two tiles are 4 g .. 4 g + 3 of 32.
+//
+// Measured (B200), the FMA kernel (8 rows at a time) in brackets: 320 items of 1500 keys
+// of 64, 5 rows each, 53 us (81); 64 items of 4096 keys, 8 rows: of 64 30 (40), of 128 49
+// (59), 16 rows: 42 (70) and 69 (108). Eight warps on an SM for keys of 128 and twelve
+// for 64 carry it: bound by latency, of the copies and of the chain from a tile's scores
+// to its weights (3.7 TB/s for 8 rows; issue 37 %, tensor cores 23 %). Four CTAs on an
+// SM in place of three for keys of 64, with 128 registers: 58.7 for the 53. First parts
+// cut in place of rounded: 53.6, and twice the error.
+template <int HD, int NT>
+__global__ void __launch_bounds__(kPagedThreads, HD == 64 ? 3 : 2)
+    paged_attention_tf32_kernel(const PagedArgs a) {
+  using Cfg = Tf32Cfg<HD>;
+  constexpr int kRows = 8 * NT, kSteps = HD / 8, kBlocks = HD / 32, kCpr = HD / 4;
+  constexpr int kLoads = kTok * kCpr / 32;   // a lane, K or V
+  constexpr int kLd = NT == 1 ? 8 : 24;      // of a key's weights: no bank is met twice
+  extern __shared__ __align__(128) char smem[];
+  __shared__ float sh_m[kPagedWarps][kRows], sh_l[kPagedWarps][kRows];
+  __shared__ __align__(16) float sh_p[kPagedWarps][kTok][kLd];
+  pdl_wait();
+
+  const PagedItem it = paged_item<4, kRows, kTok>(a);
+  // nothing to do; in a cluster the others still wait for this CTA
+  if (!it.any || (it.c0 >= it.c1 && a.chunk > 0)) return;
+  const int seq = it.seq, head = it.head, g0 = it.g0, g_n = it.g_n, c0 = it.c0, c1 = it.c1;
+
+  const int lane = lane_id(), w = warp_id(), g = lane >> 2, t = lane & 3;
+  const float* kp = static_cast<const float*>(a.k) + head * a.head_stride;
+  const float* vp = static_cast<const float*>(a.v) + head * a.head_stride;
+  const float* q = static_cast<const float*>(a.q) + seq * a.q_seq + head * a.q_head;
+  const int32_t* row = a.table + seq * a.ld_table;
+  char* ring = smem + w * Cfg::kWarpBytes;
+  const uint32_t ring_at = smem_u32(ring);
+  char* sh_q = smem + kPagedWarps * Cfg::kWarpBytes;
+
+  constexpr int kTurn = kPagedWarps * kTok;
+  const int base = c0 / kTok * kTok + w * kTok;
+  const int n_mine = base < c1 ? (c1 - base + kTurn - 1) / kTurn : 0;
+  auto locate = [&](int i) {
+    const int key = base + i * kTurn + (lane & 15);
+    return read_page(a, row, key, i < n_mine && key >= c0 && key < c1);
+  };
+  // half h: K (even) or V (odd) of tile h / 2, whose keys are at `where`. Chunks of 16
+  // bytes are exchanged within a row so that a warp's reads meet no bank twice: K's
+  // eight lanes read two rows, V's four
+  auto fetch = [&](int h, int64_t where) {
+    const uint32_t slot = ring_at + h % Cfg::kHalves * Cfg::kTileBytes;
+#pragma unroll
+    for (int j = 0; j < kLoads; j++) {
+      const int r = j * (32 / kCpr) + lane / kCpr, c = lane % kCpr;
+      const int64_t at = __shfl_sync(0xffffffffu, where, r);
+      const int mix = h & 1 ? (r & 3) << 1 : (r & 1) << 2;
+      cp_async16(slot + r * HD * 4 + ((c ^ mix) << 4),
+                 (h & 1 ? vp : kp) + (at < 0 ? 0 : at + c * 4), at >= 0);
+    }
+  };
+  PagedKey next = locate(0);
+  int64_t where = place_key(a, next);   // of the tile whose V is fetched next
+  next = locate(1);
+  uint32_t live = __ballot_sync(0xffffffffu, where >= 0), live_next = 0;
+  if (n_mine > 0) fetch(0, where);
+  cp_async_commit();
+  if (n_mine > 0) fetch(1, where);
+  cp_async_commit();
+
+  // Q^T's fragments in the order of the steps: in two parts for one tile of rows, and
+  // whole for two, which leaves room for two CTAs on an SM
+  auto query = [&](int r, int d) {
+    return r < g_n ? q[(g0 + r) * a.q_group + d] * a.scale_log2 : 0.0f;
+  };
+  bool extreme = false;
+  for (int i = threadIdx.x; i < kSteps * 32; i += kPagedThreads) {
+    const int d = (i >> 6) * 16 + (i & 3) * 4 + (i >> 5 & 1) * 2, r = i >> 2 & 7;
+    const float x = query(r, d), y = query(r, d + 1);
+    const float hx = tf32_hi(x), hy = tf32_hi(y);
+    extreme |= far_from_one(x) | far_from_one(y);
+    if (NT > 1) extreme |= far_from_one(query(r + 8, d)) | far_from_one(query(r + 8, d + 1));
+    reinterpret_cast<float4*>(sh_q)[i] =
+        NT == 1 ? make_float4(hx, hy, tf32_lo(x, hx), tf32_lo(y, hy))
+                : make_float4(x, y, query(r + 8, d), query(r + 8, d + 1));
+  }
+  // what parts below 2^-126 cost a score: of k, hd 2^-126 |q| at most; of q, 2^-126 / |q|
+  // of the product. Neither shows while q is within these bounds.
+  const bool whole = __syncthreads_or(extreme);
+
+  // o[z][b][i][e]: dimensions 32 b + 4 g + 2 i (e < 2) and the next, rows 8 z + 2 t + e % 2
+  float o[NT][kBlocks][2][4] = {}, m[NT][2], l[NT][2] = {};
+#pragma unroll
+  for (int z = 0; z < NT; z++) m[z][0] = m[z][1] = -INFINITY;
+
+#pragma unroll 1
+  for (int i = 0; i < n_mine; i++) {
+    __syncwarp();   // every lane has read the slot that is filled now
+    where = place_key(a, next);
+    next = locate(i + 2);
+    live_next = __ballot_sync(0xffffffffu, where >= 0);
+    if (i + 1 < n_mine) fetch(2 * i + 2, where);
+    cp_async_commit();
+    cp_async_wait<2>();
+    __syncwarp();
+    const float4* kt =
+        reinterpret_cast<const float4*>(ring + 2 * i % Cfg::kHalves * Cfg::kTileBytes);
+    // six chains of products for a tile of rows: one would wait for each step's result
+    float s[NT][2][3][4] = {};
+#pragma unroll
+    for (int j = 0; j < kSteps / 2; j++) {
+      const int c = (4 * j + t) ^ ((g & 1) << 2);
+      const float4 x = kt[g * kCpr + c], y = kt[(g + 8) * kCpr + c];
+      const float k[2][4] = {{x.x, y.x, x.y, y.y}, {x.z, y.z, x.w, y.w}};
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        float hi[4], lo[4];
+        split_tf32(k[u], hi, lo);
+        const float4 b = reinterpret_cast<const float4*>(sh_q)[(2 * j + u) * 32 + lane];
+        const float q_all[4] = {b.x, b.y, b.z, b.w};
+        float q_hi[4], q_lo[4];
+        if constexpr (NT > 1) split_tf32(q_all, q_hi, q_lo);
+#pragma unroll
+        for (int z = 0; z < NT; z++) {
+          const float h0 = NT > 1 ? q_hi[2 * z] : b.x, h1 = NT > 1 ? q_hi[2 * z + 1] : b.y;
+          const float l0 = NT > 1 ? q_lo[2 * z] : b.z, l1 = NT > 1 ? q_lo[2 * z + 1] : b.w;
+          mma_tf32(s[z][u][0], hi, h0, h1);
+          mma_tf32(s[z][u][1], hi, l0, l1);
+          mma_tf32(s[z][u][2], lo, h0, h1);
+        }
+      }
+    }
+    // keys g and g + 8, query rows 8 z + 2 t + {0, 1}
+    const bool in0 = live >> g & 1, in1 = live >> (g + 8) & 1;
+    float x[NT][4];
+    bool odd = whole;
+#pragma unroll
+    for (int z = 0; z < NT; z++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        x[z][e] = (s[z][0][0][e] + s[z][1][0][e]) +
+                  ((s[z][0][1][e] + s[z][1][1][e]) + (s[z][0][2][e] + s[z][1][2][e]));
+        odd |= x[z][e] != x[z][e];
+      }
+    if (__any_sync(0xffffffffu, odd)) {
+      // an infinite number has no parts: the scores as sums of whole products
+#pragma unroll
+      for (int e = 0; e < 4 * NT; e++) {
+        const int r = g + (e >> 1 & 1) * 8;
+        float y = 0.0f;
+        for (int d = 0; d < HD; d++) {
+          const float kd = reinterpret_cast<const float*>(
+              kt)[r * HD + (((d >> 2) ^ ((r & 1) << 2)) << 2) + (d & 3)];
+          y = fmaf(query((e >> 2) * 8 + 2 * t + (e & 1), d), kd, y);
+        }
+        x[e >> 2][e & 3] = y;
+      }
+    }
+    float most[NT][2];
+    bool more = false;
+#pragma unroll
+    for (int z = 0; z < NT; z++) {
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (!(e < 2 ? in0 : in1)) x[z][e] = -INFINITY;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        most[z][h] = fmaxf(x[z][h], x[z][2 + h]);
+        more |= most[z][h] > m[z][h] + 8.0f;
+      }
+    }
+    if (__any_sync(0xffffffffu, more)) {
+#pragma unroll
+      for (int z = 0; z < NT; z++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          float y = most[z][h];
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, d));
+          y = fmaxf(y, m[z][h]);
+          const float f = m[z][h] == -INFINITY ? 0.0f : fast_exp2(m[z][h] - y);
+          m[z][h] = y;
+          l[z][h] *= f;
+#pragma unroll
+          for (int b = 0; b < kBlocks; b++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[z][b][e >> 1][(e & 1) * 2 + h] *= f;
+        }
+    }
+#pragma unroll
+    for (int z = 0; z < NT; z++) {
+      // a row that has met no score above -inf yet: its reference is 0
+      const float r0 = m[z][0] == -INFINITY ? 0.0f : m[z][0];
+      const float r1 = m[z][1] == -INFINITY ? 0.0f : m[z][1];
+#pragma unroll
+      for (int e = 0; e < 4; e++) x[z][e] = fast_exp2(x[z][e] - (e & 1 ? r1 : r0));
+      l[z][0] += x[z][0] + x[z][2];
+      l[z][1] += x[z][1] + x[z][3];
+      // from accumulators to operands: keys t and t + 4 of either eight, row g
+      *reinterpret_cast<float2*>(&sh_p[w][g][8 * z + 2 * t]) = make_float2(x[z][0], x[z][1]);
+      *reinterpret_cast<float2*>(&sh_p[w][g + 8][8 * z + 2 * t]) = make_float2(x[z][2], x[z][3]);
+    }
+    __syncwarp();   // also: every lane has read K's slot
+    if (i + 1 < n_mine) fetch(2 * i + 3, where);
+    cp_async_commit();
+    float p_hi[NT][4], p_lo[NT][4];
+#pragma unroll
+    for (int z = 0; z < NT; z++) {
+      float p[4];
+#pragma unroll
+      for (int e = 0; e < 4; e++) p[e] = sh_p[w][t + 4 * e][8 * z + g];
+      split_tf32(p, p_hi[z], p_lo[z]);
+    }
+    cp_async_wait<2>();
+    __syncwarp();
+    const float4* vt =
+        reinterpret_cast<const float4*>(ring + (2 * i + 1) % Cfg::kHalves * Cfg::kTileBytes);
+    // a tile's products are summed by themselves, then added in fp32; two blocks of
+    // dimensions share a vote on what has no parts
+#pragma unroll
+    for (int b0 = 0; b0 < kBlocks; b0 += 2) {
+      float d[NT][2][2][4] = {};
+#pragma unroll
+      for (int b = 0; b < 2; b++) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+          const int c = (8 * (b0 + b) + g) ^ (t << 1);
+          const float4 v0 = vt[(8 * u + t) * kCpr + c], v1 = vt[(8 * u + t + 4) * kCpr + c];
+          const float v[2][4] = {{v0.x, v0.y, v1.x, v1.y}, {v0.z, v0.w, v1.z, v1.w}};
+#pragma unroll
+          for (int n = 0; n < 2; n++) {
+            float hi[4], lo[4];
+            split_tf32(v[n], hi, lo);
+#pragma unroll
+            for (int z = 0; z < NT; z++) {
+              mma_tf32(d[z][b][n], lo, p_hi[z][2 * u], p_hi[z][2 * u + 1]);
+              mma_tf32(d[z][b][n], hi, p_lo[z][2 * u], p_lo[z][2 * u + 1]);
+              mma_tf32(d[z][b][n], hi, p_hi[z][2 * u], p_hi[z][2 * u + 1]);
+            }
+          }
+        }
+      }
+      odd = false;
+#pragma unroll
+      for (int e = 0; e < 16 * NT; e++) {
+        const float y = d[e >> 4][e >> 3 & 1][e >> 2 & 1][e & 3];
+        odd |= y != y;
+      }
+      if (__any_sync(0xffffffffu, odd)) {
+        // as above
+#pragma unroll
+        for (int e = 0; e < 16 * NT; e++) {
+          const int b = e >> 3 & 1, n = e >> 2 & 1;
+          const int dim = 32 * (b0 + b) + 4 * g + 2 * n + (e >> 1 & 1);
+          float y = 0.0f;
+          for (int r = 0; r < kTok; r++) {
+            const float vd = reinterpret_cast<const float*>(
+                vt)[r * HD + (((dim >> 2) ^ ((r & 3) << 1)) << 2) + (dim & 3)];
+            y = fmaf(sh_p[w][r][8 * (e >> 4) + 2 * t + (e & 1)], vd, y);
+          }
+          d[e >> 4][b][n][e & 3] = y;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 16 * NT; e++)
+        o[e >> 4][b0 + (e >> 3 & 1)][e >> 2 & 1][e & 3] +=
+            d[e >> 4][e >> 3 & 1][e >> 2 & 1][e & 3];
+    }
+    live = live_next;
+  }
+  cp_async_wait<0>();
+  pdl_launch_dependents();
+  __syncthreads();   // the rings become the warps' parts of o
+
+  float* part = reinterpret_cast<float*>(smem);   // [warp][row][HD]
+#pragma unroll
+  for (int z = 0; z < NT; z++)
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      float sum = l[z][h];
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      const int r = 8 * z + 2 * t + h;
+      if (lane < 4) {
+        sh_m[w][r] = m[z][h];
+        sh_l[w][r] = sum;
+      }
+#pragma unroll
+      for (int b = 0; b < kBlocks; b++)
+#pragma unroll
+        for (int n = 0; n < 2; n++)
+          *reinterpret_cast<float2*>(part + (w * kRows + r) * HD + 32 * b + 4 * g + 2 * n) =
+              make_float2(o[z][b][n][h], o[z][b][n][2 + h]);
+    }
+  __syncthreads();
+  finish_item<float, HD, kRows, 4>(a, it, part, sh_m, sh_l, part + kPagedWarps * kRows * HD);
+}
+
 // A query row's parts joined by W warps, which take the splits that held keys in turn
 // and are joined in order: one where rows are many (four rows a CTA), 32 where they are
 // few and their splits many. Measured (B200) with 273 parts for each of 16 rows, the
@@ -885,14 +1237,14 @@ static PagedCut paged_cut(int64_t n_seqs, int64_t n_heads, int64_t group, int64_
   if (dtype == WX_DTYPE_BF16) {
     c.tile = group <= 8 ? 8 : 16;
   } else {
-    c.tile = 1;
-    while (c.tile < 8 && c.tile < group) c.tile *= 2;
+    c.tile = group <= 2 ? (int)group : group <= 4 ? 4 : group <= 8 ? 8 : 16;
   }
   c.splits = 1;
   c.warps = 4;
   const int64_t items = n_seqs * n_heads * ((group + c.tile - 1) / c.tile);
   if (max_len * (dtype == WX_DTYPE_BF16 ? 1 : 2) <= kShortKeys && items >= kShortItems) {
     c.warps = 1;
+    if (dtype == WX_DTYPE_F32) c.tile = std::min(c.tile, 8);
   } else if (max_len > kClusterKeys) {
     int64_t chunk = max_len * items / kChunkCtas;
     chunk = chunk < kMinChunk ? kMinChunk : chunk > kMaxChunk ? kMaxChunk : chunk;
@@ -965,9 +1317,20 @@ static cudaError_t run_fma(const PagedArgs& a, const PagedCut& c, cudaStream_t s
   switch (c.tile) {
     case 1: return launch_paged<paged_attention_fma_kernel<HD, 1, WPI>>(a, c, smem, st);
     case 2: return launch_paged<paged_attention_fma_kernel<HD, 2, WPI>>(a, c, smem, st);
-    case 4: return launch_paged<paged_attention_fma_kernel<HD, 4, WPI>>(a, c, smem, st);
-    default: return launch_paged<paged_attention_fma_kernel<HD, 8, WPI>>(a, c, smem, st);
+    default: break;
   }
+  if constexpr (WPI == 1)
+    if (c.tile == 8) return launch_paged<paged_attention_fma_kernel<HD, 8, 1>>(a, c, smem, st);
+  return launch_paged<paged_attention_fma_kernel<HD, 4, WPI>>(a, c, smem, st);
+}
+
+template <int HD>
+static cudaError_t run_fp32(const PagedArgs& a, const PagedCut& c, cudaStream_t st) {
+  constexpr int smem = Tf32Cfg<HD>::kSmem;
+  if (c.warps == 1) return run_fma<HD, 1>(a, c, st);
+  if (c.tile == 8) return launch_paged<paged_attention_tf32_kernel<HD, 1>>(a, c, smem, st);
+  if (c.tile == 16) return launch_paged<paged_attention_tf32_kernel<HD, 2>>(a, c, smem, st);
+  return run_fma<HD, 4>(a, c, st);
 }
 
 template <typename T, int HD>
@@ -976,7 +1339,7 @@ static cudaError_t run_paged(const PagedArgs& a, const PagedCut& c, cudaStream_t
   if constexpr (sizeof(T) == 2)
     e = run_mma<HD>(a, c, st);
   else
-    e = c.warps == 1 ? run_fma<HD, 1>(a, c, st) : run_fma<HD, 4>(a, c, st);
+    e = run_fp32<HD>(a, c, st);
   if (e != cudaSuccess || c.chunk == 0) return e;
   const int64_t rows = (int64_t)a.n_seqs * a.n_heads * a.group;
   if (rows >= kJoinRows)
