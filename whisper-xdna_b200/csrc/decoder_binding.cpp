@@ -3,7 +3,7 @@
 //
 // A decoder calls these operators once a layer and token, on work of a few
 // microseconds, so what the host spends counts: checked and allocated in Python and
-// called through ctypes, a call cost 10 to 24 us; here it costs 3 to 10 (B200 host).
+// called through ctypes, a call cost 10 to 24 us; here it costs 3 to 7 (B200 host).
 // Everything computed is in libwxb200.so, whose entry points check sizes and
 // strides themselves.
 #include <Python.h>
