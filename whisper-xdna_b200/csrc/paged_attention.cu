@@ -306,7 +306,7 @@ struct FmaCfg {
 //
 // Measured (B200): 64 items of 4096 keys of 128, 2 and 4 rows each, 44 and 46 us (6.1 and
 // 5.9 TB/s), 8 rows 59: from there on bound by the issue of some 17 instructions a key
-// and row, and left to the tensor cores (which take 49 for 4 rows too) unless short items
+// and row, and left to the tensor cores (which take 48 for 4 rows too) unless short items
 // are many: 2560 of up to 120 keys of 64, 8 rows, 35 us a warp each, 37 on them.
 template <int HD, int GT, int WPI>
 __global__ void __launch_bounds__(kPagedThreads, 4) paged_attention_fma_kernel(const PagedArgs a) {
@@ -830,12 +830,13 @@ struct Tf32Cfg {
 // 4 t .. 4 t + 3 of 16, V's rows g and g + 8 of two tiles are 4 g .. 4 g + 3 of 32.
 //
 // Measured (B200), the FMA kernel (8 rows at a time) in brackets: 320 items of 1500 keys
-// of 64, 5 rows each, 53 us (81); 64 items of 4096 keys, 8 rows: of 64 30 (40), of 128 49
-// (59), 16 rows: 42 (70) and 69 (108). Eight warps on an SM for keys of 128 and twelve
+// of 64, 5 rows each, 48 us (81); 64 items of 4096 keys, 8 rows: of 64 29 (40), of 128 49
+// (59), 16 rows: 39 (70) and 66 (108). Eight warps on an SM for keys of 128 and twelve
 // for 64 carry it: bound by latency, of the copies and of the chain from a tile's scores
-// to its weights (3.7 TB/s for 8 rows; issue 37 %, tensor cores 23 %). Four CTAs on an
-// SM in place of three for keys of 64, with 128 registers: 58.7 for the 53. First parts
-// cut in place of rounded: 53.6, and twice the error.
+// to its weights (5.1 TB/s for 5 rows of 64; issue 37 %, tensor cores 23 % of their
+// cycles with 8 of 128). Four CTAs on an SM in place of three for keys of 64, with 128
+// registers: 58.7 us where three took 53.6. First parts cut in place of rounded: twice
+// the error, and no faster.
 template <int HD, int NT>
 __global__ void __launch_bounds__(kPagedThreads, HD == 64 ? 3 : 2)
     paged_attention_tf32_kernel(const PagedArgs a) {
@@ -871,17 +872,24 @@ __global__ void __launch_bounds__(kPagedThreads, HD == 64 ? 3 : 2)
   };
   // half h: K (even) or V (odd) of tile h / 2, whose keys are at `where`. Chunks of 16
   // bytes are exchanged within a row so that a warp's reads meet no bank twice: K's
-  // eight lanes read two rows, V's four
+  // eight lanes read two rows, V's four. A tile with all its keys needs no tests (16
+  // clips' frames 53.7 -> 48.3 us)
   auto fetch = [&](int h, int64_t where) {
     const uint32_t slot = ring_at + h % Cfg::kHalves * Cfg::kTileBytes;
+    const float* from = (h & 1 ? vp : kp) + lane % kCpr * 4;
+    auto rows = [&](auto copy) {
 #pragma unroll
-    for (int j = 0; j < kLoads; j++) {
-      const int r = j * (32 / kCpr) + lane / kCpr, c = lane % kCpr;
-      const int64_t at = __shfl_sync(0xffffffffu, where, r);
-      const int mix = h & 1 ? (r & 3) << 1 : (r & 1) << 2;
-      cp_async16(slot + r * HD * 4 + ((c ^ mix) << 4),
-                 (h & 1 ? vp : kp) + (at < 0 ? 0 : at + c * 4), at >= 0);
-    }
+      for (int j = 0; j < kLoads; j++) {
+        const int r = j * (32 / kCpr) + lane / kCpr;
+        const int64_t at = __shfl_sync(0xffffffffu, where, r);
+        const int mix = h & 1 ? (r & 3) << 1 : (r & 1) << 2;
+        copy(slot + r * HD * 4 + ((lane % kCpr ^ mix) << 4), at);
+      }
+    };
+    if (__all_sync(0xffffffffu, where >= 0))
+      rows([&](uint32_t to, int64_t at) { cp_async16(to, from + at, true); });
+    else
+      rows([&](uint32_t to, int64_t at) { cp_async16(to, from + (at < 0 ? 0 : at), at >= 0); });
   };
   PagedKey next = locate(0);
   int64_t where = place_key(a, next);   // of the tile whose V is fetched next
