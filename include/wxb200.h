@@ -276,8 +276,9 @@ int wx_kv_compact(void* k_cache, void* v_cache, int64_t n_layers, int64_t layer_
  * a clip's keys, or both: q and out are (n_seqs, n_heads, group, head_dim) with
  * any strides, head_dim contiguous. lse (n_seqs, n_heads, group) fp32 or NULL. A
  * row without keys (or with all scores -inf) gives o = 0 and lse = -inf. q, the
- * cache and out are of one dtype; head_dim 64 or 128; sums in fp32, the
- * result rounded once.
+ * cache and out are of one dtype; head_dim 64 or 128. Scores and sums are fp32's,
+ * each product within 2^-20 of itself (a weight times a bf16 v: 2^-15), and the
+ * result is rounded once.
  * max_len: an upper bound of lens, at most ld_table * page_size and 2^29 (longer
  * sequences are cut there, WX_DEVERR_PAGE): it shapes the launch. The workspace
  * (wx_paged_attention_workspace bytes, 16-byte aligned; may be 0) needs no
