@@ -671,18 +671,21 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_mma_kernel(cons
   uint32_t qf[NT][kSteps][2];
   {
     const uint16_t* q = static_cast<const uint16_t*>(a.q) + seq * a.q_seq + head * a.q_head;
+    auto load = [&](auto pair) {
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
-      const int g = n * 8 + lane / 4;
-      const uint16_t* p = q + (g0 + g) * a.q_group + (lane & 3) * 2;
+      for (int n = 0; n < NT; n++) {
+        const int g = n * 8 + lane / 4;
+        const uint16_t* p = q + (g0 + g) * a.q_group + (lane & 3) * 2;
 #pragma unroll
-      for (int k = 0; k < kSteps; k++)
+        for (int k = 0; k < kSteps; k++)
 #pragma unroll
-        for (int h = 0; h < 2; h++)
-          qf[n][k][h] = g < g_n ? (uint32_t)p[k * 16 + h * 8] |
-                                      ((uint32_t)p[k * 16 + h * 8 + 1] << 16)
-                                : 0;
-    }
+          for (int h = 0; h < 2; h++) qf[n][k][h] = g < g_n ? pair(p + k * 16 + h * 8) : 0;
+      }
+    };
+    if ((((uintptr_t)q | (uint64_t)(a.q_group * 2)) & 3) == 0)
+      load([](const uint16_t* p) { return *reinterpret_cast<const uint32_t*>(p); });
+    else
+      load([](const uint16_t* p) { return (uint32_t)p[0] | ((uint32_t)p[1] << 16); });
   }
 
   float o[NT][kSteps][4], m[NT][2], l[NT][2];
