@@ -133,6 +133,21 @@ def test_attend_many_short_sequences(cuda, dtype, heads, group):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("group", [1, 2, 3, 8, 13])
+def test_attend_many_tiny_sequences(cuda, dtype, hd, group):
+    """A warp for each item of at most 16 keys; q and out where no vector fits."""
+    lens = [i % 17 for i in range(301)]
+    k, v, table, n, gen = make_cache(lens, 16, 4, hd, dtype, seed=group)
+    wide = randn(gen, 301, 4 * group * hd + 3, dtype=dtype)
+    q = wide[:, 1:-2].unflatten(1, (4 * group, hd))
+    out = torch.empty_like(wide)[:, 1:-2].unflatten(1, (4 * group, hd))
+    got, _ = check_attend(q, k, v, table, n, out=out)
+    assert got.data_ptr() == out.data_ptr()
+    assert torch.equal(ops.paged_attention(q.contiguous(), k, v, table, n), got)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_attend_window(cuda, dtype):
     lens = [40, 40, 40, 40, 700, 700, 0, 2500]
     starts = torch.tensor([0, 7, 39, 40, 16, 699, 3, 2100], dtype=torch.int32, device="cuda")

@@ -358,7 +358,7 @@ struct FmaCfg {
 // Measured (B200): 64 items of 4096 keys of 128, 2 and 4 rows each, 44 and 46 us (6.1 and
 // 5.9 TB/s), 8 rows 59: from there on bound by the issue of some 17 instructions a key
 // and row, and left to the tensor cores (which take 48 for 4 rows too) unless short items
-// are many: 2560 of up to 120 keys of 64, 8 rows, 35 us a warp each, 37 on them.
+// are many (see PagedCut).
 template <int HD, int GT, int WPI>
 __global__ void __launch_bounds__(kPagedThreads, 4) paged_attention_fma_kernel(const PagedArgs a) {
   using Cfg = FmaCfg<HD>;
@@ -1284,9 +1284,12 @@ constexpr int64_t kJoinRows = 8 * 148;   // rows from which on a warp each will 
 // long caches chunks of keys that a second kernel joins. In between, a launch splits
 // an item over a cluster where that keeps every CTA in the first wave (launch_paged).
 //
-// Measured (B200): a warp and a CTA each for 6400 items of 10 to 224 keys of 64 in bf16
-// 27.4 and 36.7 us, of 448 keys 124 and 116, of 224 in fp32 53.7 and 50.5; for 2560 items
-// of up to 224 keys of 128 29.3 and 36.3; for 1200 items 11.3 and 9.9, 600 10.4 and 7.0.
+// Measured (B200), a warp and a CTA for each item of up to 16, 64, 128, 256 keys of 64,
+// us: in bf16 with 5 rows, 640 items 4.1 and 4.7, 5.8 and 4.7, 8.4 and 5.6, 12.5 and 6.8;
+// 2000 items 5.7 and 9.5, 7.4 and 10.3, 10.0 and 11.3, 15.8 and 13.8; 8000 items 13 and 31,
+// 18 and 35, 23 and 39, 32 and 44 (6400 of up to 448 keys: 124 and 116). In fp32 with one
+// row, 2000 items 5.0 and 8.1, 11.6 and 10.6, 20 and 14, 37 and 20; 8000 items 12 and 26,
+// 24 and 35, 36 and 42, 59 and 54; with 8 rows 26 and 65, 41 and 72, 59 and 80, 94 and 93.
 // Tiles of 16 rows against two of 8, 64 items of 4096 keys, 16 rows each: 31.7 and 36.2.
 // 320 items of 1500 keys, a cluster of 1, 2, 4, 8 for each: 27.3, 25.8, 31.0, 38.4 us
 // (two waves from 4 on; 3 CTAs, which divide no GPC: 33.0); 20 such items 20.3, 13.3,
@@ -1295,7 +1298,9 @@ constexpr int64_t kJoinRows = 8 * 148;   // rows from which on a warp each will 
 struct PagedCut {
   int tile, warps, splits, chunk;
 };
-constexpr int64_t kShortKeys = 256, kShortItems = 16 * 148;   // bf16; fp32: half the keys
+// An item of short sequences gets a warp where items are many: its time grows with the
+// keys, a CTA's with the waves.
+constexpr int64_t kShortKeys = 256, kShortItems = 300, kShortBf16 = 10, kShortFp32 = 30;
 constexpr int64_t kClusterKeys = 4096;
 constexpr int64_t kEarlyKeys = 65536;
 constexpr int64_t kMinChunk = 128, kChunkCtas = 32 * 148;
@@ -1311,10 +1316,14 @@ static PagedCut paged_cut(int64_t n_seqs, int64_t n_heads, int64_t group, int64_
   }
   c.splits = 1;
   c.warps = 4;
-  const int64_t items = n_seqs * n_heads * ((group + c.tile - 1) / c.tile);
-  if (max_len * (dtype == WX_DTYPE_BF16 ? 1 : 2) <= kShortKeys && items >= kShortItems) {
+  const int64_t pairs = n_seqs * n_heads, items = pairs * ((group + c.tile - 1) / c.tile);
+  const bool fp32 = dtype == WX_DTYPE_F32;
+  const int narrow = fp32 ? std::min(c.tile, 8) : c.tile;   // a warp's in fp32: the FMA pipe
+  const int64_t short_items = pairs * ((group + narrow - 1) / narrow);
+  if (max_len <= (fp32 ? kShortKeys / 2 : kShortKeys) &&
+      short_items >= kShortItems + max_len * (fp32 ? kShortFp32 : kShortBf16)) {
     c.warps = 1;
-    if (dtype == WX_DTYPE_F32) c.tile = std::min(c.tile, 8);
+    c.tile = narrow;
   } else if (max_len > kClusterKeys) {
     int64_t chunk = max_len * items / kChunkCtas;
     chunk = chunk < kMinChunk ? kMinChunk : chunk > kMaxChunk ? kMaxChunk : chunk;
