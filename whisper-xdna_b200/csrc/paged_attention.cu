@@ -356,9 +356,12 @@ struct FmaCfg {
 // to all lanes through shared memory.
 //
 // Measured (B200): 64 items of 4096 keys of 128, 2 and 4 rows each, 44 and 46 us (6.1 and
-// 5.9 TB/s), 8 rows 59: from there on bound by the issue of some 17 instructions a key
-// and row, and left to the tensor cores (which take 48 for 4 rows too) unless short items
-// are many (see PagedCut).
+// 5.9 TB/s), 8 rows 59: bound by the issue of some 17 instructions a key and row. From 3
+// rows on the tensor cores take over (keys of 64, 4 rows: 320 items of 1500 keys 46 us here
+// and 48 there, 64 of 4096 29.9 and 28.4, 44 of up to 2180 13.8 and 11.4; with 2 rows 42.8
+// and 47.7, 26.1 and 27.9, 12.9 and 11.3), but short items of 3 or 4 rows stay (1280 of up
+// to 256 keys of 128 23.9 and 28.8, of up to 64 11.8 and 17.6), and short ones that are
+// many, up to 8 rows at a time (see PagedCut).
 template <int HD, int GT, int WPI>
 __global__ void __launch_bounds__(kPagedThreads, 4) paged_attention_fma_kernel(const PagedArgs a) {
   using Cfg = FmaCfg<HD>;
@@ -858,11 +861,10 @@ __device__ __forceinline__ bool far_from_one(float x) {
   return (b != 0) & (b - (25u << 24) > (166u << 24));
 }
 
-template <int HD>
+template <int HD, int HALVES>
 struct Tf32Cfg {
   static constexpr int kTileBytes = kTok * HD * 4;           // K or V of one tile
-  static constexpr int kHalves = 3;                          // K and V tiles in a ring
-  static constexpr int kWarpBytes = kHalves * kTileBytes;
+  static constexpr int kWarpBytes = HALVES * kTileBytes;     // a ring of K and V tiles
   static constexpr int kQueryBytes = HD / 8 * 32 * 16;   // 8 rows in two parts or 16 whole
   static constexpr int kSmem = kPagedWarps * kWarpBytes + kQueryBytes;
 };
@@ -877,24 +879,27 @@ struct Tf32Cfg {
 // some 90 instructions for up to 8 rows, mostly the splitting, where the FMA kernel takes
 // 17 a row.
 //
-// A warp's ring holds K and V tiles in turn, three of them: K of the next tile is under
-// way while this tile's V waits. Which dimension stands in which column of a product is
+// A warp's ring holds K and V tiles in turn: three of them, so that K of the next tile is
+// under way while this tile's V waits, or two, which for keys of 128 leaves room for a
+// third CTA on an SM. Which dimension stands in which column of a product is
 // free as long as both operands agree (and for V, which row), so every operand is read
 // four dimensions at a time: K's columns t and t + 4 of two steps are dimensions
 // 4 t .. 4 t + 3 of 16, V's rows g and g + 8 of two tiles are 4 g .. 4 g + 3 of 32.
 //
 // Measured (B200), the FMA kernel (8 rows at a time) in brackets: 320 items of 1500 keys
-// of 64, 5 rows each, 48 us (81); 64 items of 4096 keys, 8 rows: of 64 29 (40), of 128 49
-// (59), 16 rows: 39 (70) and 66 (108). Eight warps on an SM for keys of 128 and twelve
-// for 64 carry it: bound by latency, of the copies and of the chain from a tile's scores
-// to its weights (5.1 TB/s for 5 rows of 64; issue 37 %, tensor cores 23 % of their
-// cycles with 8 of 128). Four CTAs on an SM in place of three for keys of 64, with 128
-// registers: 58.7 us where three took 53.6. First parts cut in place of rounded: twice
-// the error, and no faster.
-template <int HD, int NT>
-__global__ void __launch_bounds__(kPagedThreads, HD == 64 ? 3 : 2)
+// of 64, 5 rows each, 47 us (81); 64 items of 4096 keys, 8 rows: of 64 29 (40), of 128 47
+// (59), 16 rows: 38 (70) and 60 (108). Few warps carry it, twelve on an SM: bound by
+// latency, of the copies and of the chain from a tile's scores to its weights (5.2 TB/s
+// for 5 rows of 64; for 8 of 128 with eight warps, issue 37 % and tensor cores 23 % of
+// their cycles). Four CTAs on an SM in place of three for keys of 64, with 128 registers:
+// 58.7 us where three took 53.6. First parts cut in place of rounded: twice the error, and
+// no faster. Two tiles in place of three for keys of 128 and 5 rows: 320 items of 1500 keys
+// 81 us and 115 (444 places for CTAs, not 296), 44 items of up to 2180 16.4 and 22.5, but
+// 25.9 and 24.9 for 87 K keys in chunks, where the places are filled either way.
+template <int HD, int NT, int HALVES>
+__global__ void __launch_bounds__(kPagedThreads, HD == 64 || (NT == 1 && HALVES == 2) ? 3 : 2)
     paged_attention_tf32_kernel(const PagedArgs a) {
-  using Cfg = Tf32Cfg<HD>;
+  using Cfg = Tf32Cfg<HD, HALVES>;
   constexpr int kRows = 8 * NT, kSteps = HD / 8, kBlocks = HD / 32, kCpr = HD / 4;
   constexpr int kLoads = kTok * kCpr / 32;   // a lane, K or V
   constexpr int kLd = NT == 1 ? 8 : 24;      // of a key's weights: no bank is met twice
@@ -929,7 +934,7 @@ __global__ void __launch_bounds__(kPagedThreads, HD == 64 ? 3 : 2)
   // eight lanes read two rows, V's four. A tile with all its keys needs no tests (16
   // clips' frames 53.7 -> 48.3 us)
   auto fetch = [&](int h, int64_t where) {
-    const uint32_t slot = ring_at + h % Cfg::kHalves * Cfg::kTileBytes;
+    const uint32_t slot = ring_at + h % HALVES * Cfg::kTileBytes;
     const float* from = (h & 1 ? vp : kp) + lane % kCpr * 4;
     auto rows = [&](auto copy) {
 #pragma unroll
@@ -946,13 +951,15 @@ __global__ void __launch_bounds__(kPagedThreads, HD == 64 ? 3 : 2)
       rows([&](uint32_t to, int64_t at) { cp_async16(to, from + (at < 0 ? 0 : at), at >= 0); });
   };
   PagedKey next = locate(0);
-  int64_t where = place_key(a, next);   // of the tile whose V is fetched next
+  int64_t where = place_key(a, next);   // of the tile fetched last
   next = locate(1);
   uint32_t live = __ballot_sync(0xffffffffu, where >= 0), live_next = 0;
   if (n_mine > 0) fetch(0, where);
   cp_async_commit();
-  if (n_mine > 0) fetch(1, where);
-  cp_async_commit();
+  if (HALVES == 3) {
+    if (n_mine > 0) fetch(1, where);
+    cp_async_commit();
+  }
 
   // Q^T's fragments in the order of the steps: in two parts for one tile of rows, and
   // whole for two, which leaves room for two CTAs on an SM
@@ -990,15 +997,16 @@ __global__ void __launch_bounds__(kPagedThreads, HD == 64 ? 3 : 2)
 #pragma unroll 1
   for (int i = 0; i < n_mine; i++) {
     __syncwarp();   // every lane has read the slot that is filled now
+    if (HALVES == 2) fetch(2 * i + 1, where);
     where = place_key(a, next);
     next = locate(i + 2);
     live_next = __ballot_sync(0xffffffffu, where >= 0);
-    if (i + 1 < n_mine) fetch(2 * i + 2, where);
+    if (HALVES == 3 && i + 1 < n_mine) fetch(2 * i + 2, where);
     cp_async_commit();
-    cp_async_wait<2>();
+    cp_async_wait<HALVES - 1>();
     __syncwarp();
     const float4* kt =
-        reinterpret_cast<const float4*>(ring + 2 * i % Cfg::kHalves * Cfg::kTileBytes);
+        reinterpret_cast<const float4*>(ring + 2 * i % HALVES * Cfg::kTileBytes);
     // six chains of products for a tile of rows: one would wait for each step's result
     float s[NT][2][3][4] = {};
 #pragma unroll
@@ -1095,7 +1103,7 @@ __global__ void __launch_bounds__(kPagedThreads, HD == 64 ? 3 : 2)
       *reinterpret_cast<float2*>(&sh_p[w][g + 8][8 * z + 2 * t]) = make_float2(x[z][2], x[z][3]);
     }
     __syncwarp();   // also: every lane has read K's slot
-    if (i + 1 < n_mine) fetch(2 * i + 3, where);
+    if (i + 1 < n_mine) fetch(2 * i + HALVES, where);
     cp_async_commit();
     float p_hi[NT][4], p_lo[NT][4];
 #pragma unroll
@@ -1105,10 +1113,10 @@ __global__ void __launch_bounds__(kPagedThreads, HD == 64 ? 3 : 2)
       for (int e = 0; e < 4; e++) p[e] = sh_p[w][t + 4 * e][8 * z + g];
       split_tf32(p, p_hi[z], p_lo[z]);
     }
-    cp_async_wait<2>();
+    cp_async_wait<HALVES - 1>();
     __syncwarp();
     const float4* vt =
-        reinterpret_cast<const float4*>(ring + (2 * i + 1) % Cfg::kHalves * Cfg::kTileBytes);
+        reinterpret_cast<const float4*>(ring + (2 * i + 1) % HALVES * Cfg::kTileBytes);
     // a tile's products are summed by themselves, then added in fp32; two blocks of
     // dimensions share a vote on what has no parts
 #pragma unroll
@@ -1312,13 +1320,16 @@ static PagedCut paged_cut(int64_t n_seqs, int64_t n_heads, int64_t group, int64_
   if (dtype == WX_DTYPE_BF16) {
     c.tile = group <= 8 ? 8 : 16;
   } else {
-    c.tile = group <= 2 ? (int)group : group <= 4 ? 4 : group <= 8 ? 8 : 16;
+    c.tile = group <= 2 ? (int)group
+             : group <= 4 && max_len <= kShortKeys ? 4
+             : group <= 8 ? 8 : 16;
   }
   c.splits = 1;
   c.warps = 4;
   const int64_t pairs = n_seqs * n_heads, items = pairs * ((group + c.tile - 1) / c.tile);
   const bool fp32 = dtype == WX_DTYPE_F32;
-  const int narrow = fp32 ? std::min(c.tile, 8) : c.tile;   // a warp's in fp32: the FMA pipe
+  // a warp's tile in fp32, where it works on the FMA pipe
+  const int narrow = !fp32 || c.tile <= 4 ? c.tile : 8;
   const int64_t short_items = pairs * ((group + narrow - 1) / narrow);
   if (max_len <= (fp32 ? kShortKeys / 2 : kShortKeys) &&
       short_items >= kShortItems + max_len * (fp32 ? kShortFp32 : kShortBf16)) {
@@ -1390,26 +1401,28 @@ static cudaError_t run_mma(const PagedArgs& a, const PagedCut& c, cudaStream_t s
                      : launch_paged<paged_attention_mma_kernel<HD, 2, 4>>(a, c, smem, st);
 }
 
-template <int HD, int WPI>
-static cudaError_t run_fma(const PagedArgs& a, const PagedCut& c, cudaStream_t st) {
-  constexpr int smem = FmaCfg<HD>::kSmem;
-  switch (c.tile) {
-    case 1: return launch_paged<paged_attention_fma_kernel<HD, 1, WPI>>(a, c, smem, st);
-    case 2: return launch_paged<paged_attention_fma_kernel<HD, 2, WPI>>(a, c, smem, st);
-    default: break;
-  }
-  if constexpr (WPI == 1)
-    if (c.tile == 8) return launch_paged<paged_attention_fma_kernel<HD, 8, 1>>(a, c, smem, st);
-  return launch_paged<paged_attention_fma_kernel<HD, 4, WPI>>(a, c, smem, st);
-}
-
 template <int HD>
 static cudaError_t run_fp32(const PagedArgs& a, const PagedCut& c, cudaStream_t st) {
-  constexpr int smem = Tf32Cfg<HD>::kSmem;
-  if (c.warps == 1) return run_fma<HD, 1>(a, c, st);
-  if (c.tile == 8) return launch_paged<paged_attention_tf32_kernel<HD, 1>>(a, c, smem, st);
-  if (c.tile == 16) return launch_paged<paged_attention_tf32_kernel<HD, 2>>(a, c, smem, st);
-  return run_fma<HD, 4>(a, c, st);
+  constexpr int smem = FmaCfg<HD>::kSmem, ring = HD == 128 ? 2 : 3;
+  constexpr int smem3 = Tf32Cfg<HD, 3>::kSmem, smem_r = Tf32Cfg<HD, ring>::kSmem;
+  if (c.warps == 1) {
+    switch (c.tile) {
+      case 1: return launch_paged<paged_attention_fma_kernel<HD, 1, 1>>(a, c, smem, st);
+      case 2: return launch_paged<paged_attention_fma_kernel<HD, 2, 1>>(a, c, smem, st);
+      case 4: return launch_paged<paged_attention_fma_kernel<HD, 4, 1>>(a, c, smem, st);
+      default: return launch_paged<paged_attention_fma_kernel<HD, 8, 1>>(a, c, smem, st);
+    }
+  }
+  switch (c.tile) {
+    case 1: return launch_paged<paged_attention_fma_kernel<HD, 1, 4>>(a, c, smem, st);
+    case 2: return launch_paged<paged_attention_fma_kernel<HD, 2, 4>>(a, c, smem, st);
+    case 4: return launch_paged<paged_attention_fma_kernel<HD, 4, 4>>(a, c, smem, st);
+    case 8:
+      return c.chunk > 0
+                 ? launch_paged<paged_attention_tf32_kernel<HD, 1, 3>>(a, c, smem3, st)
+                 : launch_paged<paged_attention_tf32_kernel<HD, 1, ring>>(a, c, smem_r, st);
+    default: return launch_paged<paged_attention_tf32_kernel<HD, 2, ring>>(a, c, smem_r, st);
+  }
 }
 
 template <typename T, int HD>
