@@ -610,9 +610,9 @@ struct MmaCfg {
 // limit here.
 //
 // Bound by the memory: measured (B200), 16 clips' 1500 frames of 20 heads of 64, five
-// beams each (123 MB) 25.8 us, 4.8 TB/s; 64 clips 89 us, 5.5 TB/s; 64 sequences of 1 to
+// beams each (123 MB) 24.6 us, 5.0 TB/s; 64 clips 88 us, 5.6 TB/s; 64 sequences of 1 to
 // 16384 tokens, 8 heads of 128 with 4 query rows (504 MB) 89 us, 5.7 TB/s; 5 beams'
-// first tokens 3.1 us, a launch. Products on the FMA pipe took 110 and 200 us for the
+// first tokens 2.9 us, a launch. Products on the FMA pipe took 110 and 200 us for the
 // first and third; four-stage rings, with fewer CTAs on an SM, 34 and 99.
 template <int HD, int NT, int WPI>
 __global__ void __launch_bounds__(kPagedThreads) paged_attention_mma_kernel(const PagedArgs a) {
@@ -1300,8 +1300,8 @@ constexpr int64_t kJoinRows = 8 * 148;   // rows from which on a warp each will 
 // 24 and 35, 36 and 42, 59 and 54; with 8 rows 26 and 65, 41 and 72, 59 and 80, 94 and 93.
 // Tiles of 16 rows against two of 8, 64 items of 4096 keys, 16 rows each: 31.7 and 36.2.
 // 320 items of 1500 keys, a cluster of 1, 2, 4, 8 for each: 27.3, 25.8, 31.0, 38.4 us
-// (two waves from 4 on; 3 CTAs, which divide no GPC: 33.0); 20 such items 20.3, 13.3,
-// 8.7, 7.3. 64 sequences to 16384 keys, chunks of at most 512, 1024, 2048: 98, 91, 95;
+// (two waves from 4 on; 3 CTAs, which divide no GPC: 33.0; all a us less since queries are
+// read in pairs); 20 such items 20.3, 13.3, 8.7, 7.3. 64 sequences to 16384 keys, chunks of at most 512, 1024, 2048: 98, 91, 95;
 // their 2048 rows joined by a warp and by 32 warps each, the whole call: 89 and 127.
 struct PagedCut {
   int tile, warps, splits, chunk;
