@@ -220,7 +220,9 @@ int wx_attention(const void* q, const void* k, const void* v, void* o, int64_t B
  * sequence i's k and v goes to position lens[i] - counts[i] + t, that is, lens
  * counts the new tokens already (wx_kv_fork's lens_out and grown_out). k and v
  * are (n_seqs, n_tokens, n_heads, head_dim) with the given strides, head_dim
- * contiguous; column slices of one QKV buffer are fine. */
+ * contiguous; column slices of one QKV buffer are fine. counts[i] below 0 writes
+ * nothing, and past n_tokens the n_tokens rows there are, to the first of those
+ * positions; both are recorded as WX_DEVERR_PAGE. */
 int wx_kv_append(const void* k, const void* v, int64_t src_seq_stride, int64_t src_tok_stride,
                  int64_t src_head_stride, void* k_cache, void* v_cache, int64_t page_stride,
                  int64_t tok_stride, int64_t head_stride, const int32_t* table, int64_t ld_table,

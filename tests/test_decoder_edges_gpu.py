@@ -1,0 +1,77 @@
+"""The decoder operators where their device arrays contradict one another or a call
+meets a rare path: what is written, what is left out and what is reported."""
+import pytest
+import torch
+
+from test_decoder_ops_gpu import dev, make_cache, randn
+from wxb200 import _lib as L
+from wxb200 import ops
+from wxb200.kvcache import PagedKVCache
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.bfloat16, torch.float32]
+INT_MIN, INT_MAX = -2 ** 31, 2 ** 31 - 1
+
+
+@pytest.fixture(autouse=True)
+def no_device_error(cuda):
+    L.device_error()
+    yield
+    assert L.device_error() == 0
+
+
+# ------------------------------------------------------------------ append
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", ["token", "head", "padded"])
+@pytest.mark.parametrize("count", [4, 5, 9, 10, 12, INT_MAX, -1, INT_MIN])
+def test_append_counts_out_of_range(cuda, dtype, layout, count):
+    """Three rows where ten positions end at len 10 and `count` are announced: row t at
+    10 - count + t where that is one, a neighbour written as ever, and a report."""
+    page, tokens, lens = 4, 3, [10, 7]
+    k, v, table, n, gen = make_cache(lens, page, 2, 64, dtype, seed=1, layout=layout, spoil=False)
+    new = randn(gen, 2, tokens, 2, 64, dtype=dtype)
+    ek, ev = k.clone(), v.clone()
+    for i, c in enumerate((count, tokens)):
+        for t in range(min(c, tokens)):
+            pos = lens[i] - c + t
+            if pos >= 0:
+                at = table[i, pos // page].long()
+                ek[at, pos % page], ev[at, pos % page] = new[i, t], -new[i, t]
+    ops.kv_append(new, -new, k, v, table, n, counts=dev([count, tokens]))
+    assert L.device_error() == L.WX_DEVERR_PAGE
+    assert torch.equal(k, ek) and torch.equal(v, ev)
+
+
+@pytest.mark.parametrize("length", [INT_MIN, -1, 0, 2])
+def test_append_lengths_before_the_first_row(cuda, length):
+    """Positions below 0 are left out whatever length and count they come from."""
+    k, v, table, n, gen = make_cache([8], 4, 2, 64, torch.bfloat16, seed=2, spoil=False)
+    ek, ev = k.clone(), v.clone()
+    new = randn(gen, 1, 3, 2, 64, dtype=torch.bfloat16)
+    if length == 2:                     # rows 1 and 2 have a position, row 0 none
+        at = table[0, 0].long()
+        ek[at, :2], ev[at, :2] = new[0, 1:], -new[0, 1:]
+    ops.kv_append(new, -new, k, v, table, dev([length]), counts=dev([3]))
+    assert L.device_error() == L.WX_DEVERR_PAGE
+    assert torch.equal(k, ek) and torch.equal(v, ev)
+
+
+def test_cache_append_of_fewer_rows_than_granted(cuda):
+    """One row after a step of three: it is the first of the three, and reported."""
+    cache = PagedKVCache(1, 6, 4, 2, 64, 2, 12)
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    prompt = randn(gen, 2, 2, 2, 64, dtype=torch.bfloat16)
+    cache.step(grow=dev([2, 2]))
+    cache.append(0, prompt, -prompt)
+    cache.step(grow=dev([3, 1]))
+    cache.k.zero_()
+    row = randn(gen, 2, 2, 64, dtype=torch.bfloat16)
+    cache.append(0, row, -row)
+    assert L.device_error() == L.WX_DEVERR_PAGE
+    want = torch.zeros_like(cache.k)
+    for i in range(2):
+        want[0, cache.table[i, 0].long(), 2] = row[i]     # position 2 of either
+    assert torch.equal(cache.k, want)

@@ -51,8 +51,11 @@ class PagedKVCache:
             self.k, self.v, self.table, self.lens, self.refs, parents=parents, grow=grow)
 
     def append(self, layer, k, v):
-        """The tokens that the last step granted: k, v (n_seqs, tokens, heads,
-        head_dim), of which row t < grown[i] is used, or (n_seqs, heads, head_dim)."""
+        """The tokens that the last step granted, all in one call: k, v (n_seqs, tokens,
+        heads, head_dim), of which row t < grown[i] is used, or (n_seqs, heads,
+        head_dim) after a step of one token at most. Fewer rows than grown[i] are
+        written from the first granted position on, and reported by
+        _lib.device_error as WX_DEVERR_PAGE: the others hold no token yet."""
         ops.kv_append(k, v, self.k[layer], self.v[layer], self.table, self.lens,
                       counts=self.grown)
 

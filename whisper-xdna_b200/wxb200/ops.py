@@ -316,7 +316,8 @@ def kv_append(k, v, k_cache, v_cache, table, lens, counts=None):
     """Writes new tokens into a layer's cache, in place: k, v (n_seqs, tokens,
     heads, head_dim) or, for one token each, (n_seqs, heads, head_dim), of the
     cache's dtype; row t < counts[i] (all if None) of sequence i goes to position
-    lens[i] - counts[i] + t."""
+    lens[i] - counts[i] + t. A count below 0 or past the tokens given is a device
+    error (WX_DEVERR_PAGE); the rows there are go where they belong."""
     _decoder.kv_append(k, v, k_cache, v_cache, table, lens, counts)
 
 
