@@ -1,5 +1,7 @@
 """The decoder operators where their device arrays contradict one another or a call
 meets a rare path: what is written, what is left out and what is reported."""
+import math
+
 import pytest
 import torch
 
@@ -75,3 +77,25 @@ def test_cache_append_of_fewer_rows_than_granted(cuda):
     for i in range(2):
         want[0, cache.table[i, 0].long(), 2] = row[i]     # position 2 of either
     assert torch.equal(cache.k, want)
+
+
+# ------------------------------------------------------------------ scores
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("offset", [0, 1, 3])
+@pytest.mark.parametrize("rows,vocab", [(2, 1500), (4, 9001), (300, 1003), (3, 50001)])
+def test_scores_nan_at_the_first_token(cuda, dtype, offset, rows, vocab):
+    """Token 0 is NaN in a row where more logits tie than a list holds: NaN stands
+    above all, and among NaNs the lowest token comes first."""
+    wide = torch.full((rows, vocab + 8), -math.inf, dtype=dtype, device="cuda")
+    x = wide[:, offset:offset + vocab]
+    x[:, 0] = math.nan                          # the others masked
+    x[1] = math.nan                             # no number at all
+    none = torch.full((rows,), -1, device="cuda")
+    lp, entropy, top, index = ops.token_logprobs(x, none, top_k=8)
+    assert index.tolist() == [list(range(8))] * rows
+    assert top.isnan().all() and entropy.isnan().all() and (lp == 0).all()
+    x[0, 0], x[0, 7] = -math.inf, math.nan      # and one that is not the first
+    index = ops.token_logprobs(x, none, top_k=8)[3]
+    assert index[0].tolist() == [7, 0, 1, 2, 3, 4, 5, 6]

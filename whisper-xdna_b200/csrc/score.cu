@@ -220,10 +220,10 @@ struct Slice {
   }
 };
 
-// The largest entry below `bar` among thread t's vectors, found by t's whole warp
-// (each lane gets it).
+// The largest entry up to `bar`, itself included, among thread t's vectors, found by
+// t's whole warp (each lane gets it). NaN at token 0 is the largest number there is.
 template <typename T>
-__device__ __forceinline__ uint64_t best_below(const Slice<T>& s, int t, uint64_t bar) {
+__device__ __forceinline__ uint64_t best_up_to(const Slice<T>& s, int t, uint64_t bar) {
   constexpr int N = Lanes<T>::N;
   uint64_t mx = 0;
   for (int i = lane_id(); i < s.n_steps * kScoreVecs; i += 32) {
@@ -234,7 +234,7 @@ __device__ __forceinline__ uint64_t best_below(const Slice<T>& s, int t, uint64_
 #pragma unroll
     for (int e = 0; e < N; e++) {
       const uint64_t y = entry(v[e], (uint32_t)(s.lead + k * N + e));
-      if (y < bar && y > mx) mx = y;
+      if (y <= bar && y > mx) mx = y;
     }
   }
 #pragma unroll
@@ -254,7 +254,7 @@ __device__ __noinline__ void take_best(const Slice<T>& s, Candidates& c, int top
   const int lane = lane_id(), w = warp_id();
   uint64_t mine = 0;   // the thread's largest vector entry not yet taken
   for (int l = 0; l < 32; l++) {
-    const uint64_t y = best_below(s, w * 32 + l, ~0ull);
+    const uint64_t y = best_up_to(s, w * 32 + l, ~0ull);
     if (l == lane) mine = y;
   }
   for (int r = 0; r < top_k; r++) {
@@ -276,7 +276,7 @@ __device__ __noinline__ void take_best(const Slice<T>& s, Candidates& c, int top
       if (edge == all) edge = 0;
       if (who) {
         const int l = __ffs(who) - 1;
-        const uint64_t y = best_below(s, w * 32 + l, all);
+        const uint64_t y = best_up_to(s, w * 32 + l, all - 1);
         if (l == lane) mine = y;
       }
     }
