@@ -261,7 +261,8 @@ int wx_kv_fork(void* k_cache, void* v_cache, int64_t n_layers, int64_t layer_str
 
 /* Moves the pages in use to the front of the pool, in all layers: with n_used
  * pages in use, those numbered n_used or more go to the free ones below, both in
- * ascending order, and the table is renumbered (table_out may be table).
+ * ascending order, and the table is renumbered (table_out may be table). An entry
+ * that names a page which refs calls free becomes -1 (WX_DEVERR_PAGE).
  * status_out[2]: n_used and the pages moved. */
 int wx_kv_compact(void* k_cache, void* v_cache, int64_t n_layers, int64_t layer_stride,
                   int64_t page_stride, int64_t tok_stride, int64_t head_stride, int64_t n_heads,

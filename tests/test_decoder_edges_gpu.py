@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_decoder_ops_gpu import dev, make_cache, randn
+from test_decoder_ops_gpu import dev, make_cache, make_pool, randn
 from wxb200 import _lib as L
 from wxb200 import ops
 from wxb200.kvcache import PagedKVCache
@@ -99,3 +99,35 @@ def test_scores_nan_at_the_first_token(cuda, dtype, offset, rows, vocab):
     x[0, 0], x[0, 7] = -math.inf, math.nan      # and one that is not the first
     index = ops.token_logprobs(x, none, top_k=8)[3]
     assert index[0].tolist() == [7, 0, 1, 2, 3, 4, 5, 6]
+
+
+# ------------------------------------------------------------------ compact
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n_pages", [12, 20000])
+def test_compact_entries_that_the_counts_call_free(cuda, dtype, n_pages):
+    """An entry whose page nobody counts has no tokens: it is left out and reported,
+    wherever the page lies, and does not end up naming another sequence's page."""
+    gen = torch.Generator(device="cuda").manual_seed(n_pages)
+    k = make_pool(gen, n_pages, 4, 2, 64, dtype, layers=2)
+    v = make_pool(gen, n_pages, 4, 2, 64, dtype, layers=2)
+    last = n_pages - 1
+    # used: 0, 2, last - 1, last; free below their number: 1 and 3
+    good = [[2, last], [0, last - 1]]
+    refs = [0] * n_pages
+    for p in (0, 2, last - 1, last):
+        refs[p] = 1
+    for bad, count in ((1, 0), (3, 0), (last - 2, 0), (3, -1), (5, -7), (n_pages, 0)):
+        table = [good[0] + [-1], good[1] + [bad]]
+        r = list(refs)
+        if bad < n_pages:
+            r[bad] = count
+        pools = k.clone(), v.clone()
+        got = ops.kv_compact(*pools, dev(table), dev(r))
+        assert L.device_error() == L.WX_DEVERR_PAGE
+        assert got[0].tolist() == [[2, 3, -1], [0, 1, -1]]
+        assert got[1].tolist() == [1] * 4 + [0] * (n_pages - 4) and got[2].tolist() == [4, 2]
+        for new, old in zip(pools, (k, v)):
+            assert torch.equal(new[:, 3], old[:, last]) and torch.equal(new[:, 1], old[:, last - 1])
+            assert torch.equal(new[:, [0, 2]], old[:, [0, 2]])

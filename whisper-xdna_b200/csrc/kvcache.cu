@@ -189,7 +189,7 @@ struct PageCopy {
 struct PlanSpace {
   PageCopy* copies;     // max(n_seqs, n_pages)
   int32_t* list;        // n_pages: free pages or holes, ascending
-  int32_t* remap;       // n_pages: where compaction moves a page
+  int32_t* remap;       // n_pages: where a page is after a compaction, -1: nobody's
   unsigned long long* keeper;   // n_pages: the longest sharer of a page to be written
   int32_t* sharers;     // n_pages: how many share it, 0 before
   int32_t* column;      // n_pages: its column + 1, 0: not to be written
@@ -630,6 +630,17 @@ struct CompactArgs {
   int page_size, n_pages;
 };
 
+// A table entry after a compaction. One that names no page, or a page that the counts
+// call free, has no tokens: kept, it could name the page that another sequence's are
+// moved to.
+template <typename Load>
+__device__ __forceinline__ int compact_entry(const CompactArgs& a, int page, Load remap) {
+  if (page < 0) return page;
+  const int to = page < a.n_pages ? remap(page) : -1;
+  if (to < 0) kv_error();
+  return to;
+}
+
 // The used pages past the first n_used go to the free ones among them, both in
 // ascending order: the fewest moves that leave the pool dense. This form keeps its
 // arrays in global memory, for pools that do not fit one CTA's shared memory.
@@ -682,7 +693,10 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_compact_kernel(const Compa
     const int64_t upto = block_scan(((int64_t)hole << 32) | (uint32_t)mover, part, &total);
     if (hole) a.ws.list[hole_at + (int)(upto >> 32) - 1] = q;
     if (mover) a.ws.copies[mover_at + (int)(upto & 0xffffffff) - 1].src = q;
-    if (q < p1) a.refs_out[q] = q < n_used ? max(r, 0) : 0;
+    if (q < p1) {
+      a.refs_out[q] = q < n_used ? max(r, 0) : 0;
+      a.ws.remap[q] = r > 0 ? q : -1;   // a mover's is set below
+    }
     hole_at += (int)(total >> 32);
     mover_at += (int)(total & 0xffffffff);
   }
@@ -699,22 +713,9 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_compact_kernel(const Compa
     a.refs_out[dst] = a.refs[src];
   }
   cluster_sync();
-  for (int64_t i = tid; i < a.n_entries; i += kAll) {
-    int page = a.table[i];
-    if (page >= a.n_pages) {
-      kv_error();
-      page = -1;
-    } else if (page >= n_used) {
-      // a page that the table names and the counts call free has no place to go
-      if (a.refs[page] > 0) {
-        page = __ldcg(a.ws.remap + page);
-      } else {
-        kv_error();
-        page = -1;
-      }
-    }
-    a.table_out[i] = page;
-  }
+  for (int64_t i = tid; i < a.n_entries; i += kAll)
+    a.table_out[i] =
+        compact_entry(a, a.table[i], [&](int p) { return __ldcg(a.ws.remap + p); });
 }
 
 // Words of shared memory that the one-CTA form of a compaction takes.
@@ -746,6 +747,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_compact_cta_kernel(const C
   block_scan2(hole, mover, part, &n_holes, &n_movers_u);
   const int n_movers = (int)n_movers_u;
   for (int p = p0; p < p1; p++) {
+    remap[p] = refs[p] > 0 ? p : -1;   // a mover's is set below
     if (p < n_used && refs[p] <= 0) holes[hole++] = p;
     if (p >= n_used && refs[p] > 0) movers[mover++] = p;
   }
@@ -765,16 +767,8 @@ __global__ void __launch_bounds__(kPlanThreads, 1) kv_compact_cta_kernel(const C
   for (int p = tid; p < a.n_pages; p += kPlanThreads)
     a.refs_out[p] = p < n_used ? max(refs[p], 0) : 0;
 #pragma unroll 4
-  for (int64_t i = tid; i < a.n_entries; i += kPlanThreads) {
-    int page = a.table[i];
-    if (page >= a.n_pages || (page >= n_used && refs[page] <= 0)) {
-      kv_error();   // not a page, or one that the counts call free
-      page = -1;
-    } else if (page >= n_used) {
-      page = remap[page];
-    }
-    a.table_out[i] = page;
-  }
+  for (int64_t i = tid; i < a.n_entries; i += kPlanThreads)
+    a.table_out[i] = compact_entry(a, a.table[i], [&](int p) { return remap[p]; });
 }
 
 // ---------------------------------------------------------------- page copies
