@@ -5,7 +5,8 @@ import math
 import pytest
 import torch
 
-from test_decoder_ops_gpu import dev, make_cache, make_pool, randn
+import decoder_ref as R
+from test_decoder_ops_gpu import check_fork, dev, make_cache, make_pool, randn
 from wxb200 import _lib as L
 from wxb200 import ops
 from wxb200.kvcache import PagedKVCache
@@ -131,3 +132,50 @@ def test_compact_entries_that_the_counts_call_free(cuda, dtype, n_pages):
         for new, old in zip(pools, (k, v)):
             assert torch.equal(new[:, 3], old[:, last]) and torch.equal(new[:, 1], old[:, last - 1])
             assert torch.equal(new[:, [0, 2]], old[:, [0, 2]])
+
+
+# ------------------------------------------------------------------ copies of large pages
+
+
+@pytest.mark.parametrize("layout", ["token", "head", "padded"])
+@pytest.mark.parametrize("dtype,page,heads,hd", [(torch.bfloat16, 16, 20, 64),
+                                                 (torch.float32, 33, 5, 128)])
+def test_fork_copies_large_pages(cuda, dtype, layout, page, heads, hd):
+    """Pages of 2560 and 5280 vectors, which go in two and three parts, the last one not
+    full: copies that end in the first part, on either side of its end and in a later
+    one, more parts in all than there are CTAs."""
+    clips, beams, layers = 12, 6, 4
+    gen = torch.Generator(device="cuda").manual_seed(page)
+    filled = [m for m in (1, 12, 13, 15, 25, 26, 32) if m < page]
+    lens = [page + filled[c % len(filled)] for c in range(clips) for _ in range(beams)]
+    n_pages = 2 * clips + clips * beams
+    table = [[2 * c + 1, 2 * c, -1] for c in range(clips) for _ in range(beams)]
+    refs = [beams] * (2 * clips) + [0] * (clips * beams)
+    k = make_pool(gen, n_pages, page, heads, hd, dtype, layout, layers=layers)
+    v = make_pool(gen, n_pages, page, heads, hd, dtype, layout, layers=layers)
+    parents = [c * beams + (7 * b) % beams for c in range(clips) for b in range(beams)]
+    t, n, r, grown = check_fork(k, v, table, lens, refs, parents, [1] * (clips * beams), page)
+    assert sum(x > 0 for x in r) == clips + clips * beams and min(grown) == 1
+
+
+@pytest.mark.parametrize("layout", ["token", "head", "padded"])
+@pytest.mark.parametrize("dtype,page,heads,hd", [(torch.bfloat16, 16, 20, 64),
+                                                 (torch.float32, 33, 5, 128)])
+def test_compact_moves_large_pages(cuda, dtype, layout, page, heads, hd):
+    """As above, whole pages."""
+    layers, n_pages, n_used = 4, 150, 70
+    gen = torch.Generator(device="cuda").manual_seed(page)
+    k = make_pool(gen, n_pages, page, heads, hd, dtype, layout, layers=layers)
+    v = make_pool(gen, n_pages, page, heads, hd, dtype, layout, layers=layers)
+    used = torch.randperm(n_pages, generator=torch.Generator().manual_seed(page))[:n_used]
+    table = used.view(7, 10).tolist()
+    refs = [0] * n_pages
+    for p in used.tolist():
+        refs[p] = 1
+    t, r, st, moves = R.compact_ref(table, refs)
+    src, dst = (torch.tensor(x, device="cuda") for x in zip(*moves))
+    ek, ev = k.clone(), v.clone()
+    ek[:, dst], ev[:, dst] = k[:, src], v[:, src]
+    got = ops.kv_compact(k, v, dev(table), dev(refs))
+    assert got[0].tolist() == t and got[1].tolist() == r and got[2].tolist() == st
+    assert torch.equal(k, ek) and torch.equal(v, ev)
