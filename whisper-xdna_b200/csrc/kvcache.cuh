@@ -28,7 +28,9 @@ struct Div {
 // memory: it returns when all that was on the stream before is complete and visible,
 // and then lets the next kernel be placed. Every thread calls it, so that a kernel that
 // is complete stands for all before it. (The long kernels call pdl_wait() there, and
-// pdl_launch_dependents() when their loops are done.)
+// pdl_launch_dependents() when their loops are done.) Nothing that another kernel may
+// write is read by a read-only load: that would promise that it stays as it is from this
+// kernel's start on, when the kernel before it may still be writing.
 #ifdef __CUDACC__
 __device__ __forceinline__ void pdl_begin() {
   pdl_wait();

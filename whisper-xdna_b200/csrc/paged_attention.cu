@@ -75,7 +75,7 @@ struct PagedKey {
 __device__ __forceinline__ PagedKey read_page(const PagedArgs& a, const int32_t* row, int t,
                                               bool is) {
   PagedKey k = {is ? t : -1, 0};
-  if (is) k.page = __ldg(row + a.by_page(t));
+  if (is) k.page = row[a.by_page(t)];
   return k;
 }
 // Where it is, in elements from the head's first; -1: nowhere.

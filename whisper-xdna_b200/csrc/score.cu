@@ -230,7 +230,7 @@ __device__ __forceinline__ uint64_t best_up_to(const Slice<T>& s, int t, uint64_
     const int k = s.v0 + Slice<T>::at(i / kScoreVecs, i % kScoreVecs, t);
     if (k >= s.v1) continue;
     float v[N];
-    Lanes<T>::unpack(__ldg(s.vec + k), v);
+    Lanes<T>::unpack(s.vec[k], v);
 #pragma unroll
     for (int e = 0; e < N; e++) {
       const uint64_t y = entry(v[e], (uint32_t)(s.lead + k * N + e));
@@ -444,7 +444,7 @@ __global__ void __launch_bounds__(kScoreThreads, 4) token_score_kernel(const Sco
       const int k = s.v0 + Slice<T>::at(it, j, t);
       if (k >= s.v1) return;
       float v[N];
-      Lanes<T>::unpack(in_ring ? ring[it][j][t] : __ldg(s.vec + k), v);
+      Lanes<T>::unpack(in_ring ? ring[it][j][t] : s.vec[k], v);
       float vm = v[0];
 #pragma unroll
       for (int e = 0; e < N; e += 2) vm = max_nan(vm, v[e], v[e + 1]);
