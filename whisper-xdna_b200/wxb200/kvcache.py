@@ -16,7 +16,8 @@ from . import ops
 
 class PagedKVCache:
     """n_layers pools of n_pages pages of page_size tokens, for n_seqs sequences of
-    up to max_len tokens (rounded up to whole pages). Tensors, all on the device:
+    up to max_len tokens (rounded up to whole pages). Tensors, all on `device`, by
+    default the current one; calls are made with that device current:
 
     k, v: (n_layers, n_pages, page_size, n_heads, head_dim), uninitialised
     table: (n_seqs, width) int32 page table, -1 past a sequence's last page
@@ -30,8 +31,11 @@ class PagedKVCache:
                  dtype=torch.bfloat16, device=None):
         if min(n_layers, n_pages, page_size, n_heads, head_dim, n_seqs, max_len) < 1:
             raise ValueError("PagedKVCache: every size must be at least 1")
-        device = torch.device("cuda", torch.cuda.current_device() if device is None else
-                              torch.device(device).index or 0)
+        device = torch.device("cuda" if device is None else device)
+        if device.type != "cuda":
+            raise ValueError(f"PagedKVCache: device must be a CUDA device, got {device}")
+        if device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
         self.n_layers, self.page_size, self.max_len = n_layers, page_size, max_len
         shape = (n_layers, n_pages, page_size, n_heads, head_dim)
         self.k = torch.empty(shape, dtype=dtype, device=device)
