@@ -210,7 +210,8 @@ int wx_attention(const void* q, const void* k, const void* v, void* o, int64_t B
  * [i * page_size, (i + 1) * page_size). refs (n_pages, int32) counts the table
  * entries that name a page; 0 is free. A page that several sequences share
  * stands at the same place in their rows, as wx_kv_fork leaves it. All of these
- * are device memory, and no call reads them on the host.
+ * are device memory, and no call reads them on the host. Rows of a pool may share
+ * memory (strides of 0) where it is only read, by wx_paged_attention.
  *
  * A page, length or parent out of range in those arrays is left out (its tokens
  * are not written, or not attended to) and recorded as WX_DEVERR_PAGE, which
@@ -277,11 +278,11 @@ int wx_kv_compact(void* k_cache, void* v_cache, int64_t n_layers, int64_t layer_
  *   o = sum_j softmax_j(scale * q . k_j) v_j,  lse = log sum_j e^(scale * q . k_j).
  * group is the query heads that share a key-value head, or the beams that share
  * a clip's keys, or both: q and out are (n_seqs, n_heads, group, head_dim) with
- * any strides, head_dim contiguous. lse (n_seqs, n_heads, group) fp32 or NULL. A
- * row without keys (or with all scores -inf) gives o = 0 and lse = -inf. q, the
- * cache and out are of one dtype; head_dim 64 or 128. Scores and sums are fp32's,
- * each product within 2^-20 of itself (a weight times a bf16 v: 2^-15), and the
- * result is rounded once.
+ * any strides, head_dim contiguous, no two rows of out on the same memory. lse
+ * (n_seqs, n_heads, group) fp32 or NULL. A row without keys (or with all scores
+ * -inf) gives o = 0 and lse = -inf. q, the cache and out are of one dtype; head_dim
+ * 64 or 128. Scores and sums are fp32's, each product within 2^-20 of itself (a
+ * weight times a bf16 v: 2^-15), and the result is rounded once.
  * max_len: an upper bound of lens, at most ld_table * page_size and 2^29 (longer
  * sequences are cut there, WX_DEVERR_PAGE): it shapes the launch. The workspace
  * (wx_paged_attention_workspace bytes, 16-byte aligned; may be 0) needs no

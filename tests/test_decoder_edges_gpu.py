@@ -179,3 +179,28 @@ def test_compact_moves_large_pages(cuda, dtype, layout, page, heads, hd):
     got = ops.kv_compact(k, v, dev(table), dev(refs))
     assert got[0].tolist() == t and got[1].tolist() == r and got[2].tolist() == st
     assert torch.equal(k, ek) and torch.equal(v, ev)
+
+
+# ------------------------------------------------------------------ rows that share memory
+
+
+def test_outputs_that_share_memory_are_refused(cuda):
+    """Read, such a cache is one key-value head for several; written, or as a result, it
+    is refused."""
+    k, v, table, n, gen = make_cache([9, 30], 8, 1, 64, torch.bfloat16, seed=1, spoil=False)
+    q = randn(gen, 2, 4, 64, dtype=torch.bfloat16)
+    row = torch.empty(2, 1, 64, dtype=torch.bfloat16, device="cuda")
+    for out in (row.expand(2, 4, 64), row.transpose(0, 1).repeat(1, 2, 1).expand(2, 4, 64)):
+        with pytest.raises(ValueError, match="share memory"):
+            ops.paged_attention(q, k, v, table, n, out=out)
+    k2, v2 = k.expand(-1, -1, 2, 64), v.expand(-1, -1, 2, 64)
+    assert torch.equal(ops.paged_attention(q, k2, v2, table, n),
+                       ops.paged_attention(q, k2.contiguous(), v2.contiguous(), table, n))
+    refs = torch.zeros(k.shape[0], dtype=torch.int32, device="cuda")
+    for call in (lambda: ops.kv_append(q[:, :2], q[:, 2:], k2, v2, table, n),
+                 lambda: ops.kv_fork(k2[None], v2[None], table, n, refs, grow=n),
+                 lambda: ops.kv_compact(k2[None], v2[None], table, refs),
+                 lambda: ops.kv_compact(k.expand(2, -1, -1, 1, 64), v.expand(2, -1, -1, 1, 64),
+                                        table, refs)):
+        with pytest.raises(ValueError):
+            call()

@@ -5,9 +5,17 @@ from pathlib import Path
 import pytest
 import torch
 
+from test_decoder_capi import NUL, P, append, at, attend, fork, lib  # noqa: F401
 from wxb200.kvcache import PagedKVCache
 
 CSRC = Path(__file__).resolve().parents[1] / "whisper-xdna_b200" / "csrc"
+
+
+def compact(l, **kw):
+    a = dict(layers=1, ks=(16384, 1024, 64, 64), heads=1, pages=10, page=16)
+    a.update(kw)
+    return l.wx_kv_compact(P, P, a["layers"], *a["ks"], a["heads"], 64, a["pages"], a["page"], 0,
+                           at(1), at(3), 2, 4, at(4), at(6), at(8), at(9), 1 << 20, NUL)
 
 
 @pytest.mark.parametrize("name", ["paged_attention.cu", "kvcache.cu", "kvcache.cuh", "score.cu"])
@@ -35,3 +43,30 @@ def test_cache_refuses_other_devices():
     for device in ("cpu", torch.device("meta")):
         with pytest.raises(ValueError, match="CUDA"):
             PagedKVCache(1, 4, 16, 2, 64, 1, 40, device=device)
+
+
+@pytest.mark.parametrize("kw", [dict(os=(0, 64, 64)), dict(os=(63, 64, 64)), dict(os=(-63, 64, 64)),
+                                dict(heads=2, os=(128, 0, 64)), dict(group=2, os=(128, 64, 1))])
+def test_attention_refuses_an_out_on_itself(lib, kw):
+    """Rows of out that share memory would be written by several CTAs at once."""
+    l, L = lib
+    assert attend(l, **kw) == L.WX_ERR_INVALID
+    assert "share memory" in L.last_error()
+
+
+@pytest.mark.parametrize("call", [append, fork, compact])
+@pytest.mark.parametrize("pages,page,heads,ks", [(2, 1, 1, (0, 64, 64)), (1, 2, 1, (128, 0, 64)),
+                                                 (1, 1, 2, (128, 128, 0)),
+                                                 (2, 1, 1, (56, 64, 64))])
+def test_writers_refuse_a_cache_on_itself(lib, call, pages, page, heads, ks):
+    l, L = lib
+    if call is not append:
+        ks = (16384,) + ks
+    assert call(l, pages=pages, page=page, heads=heads, ks=ks) == L.WX_ERR_INVALID
+    assert "share memory" in L.last_error()
+
+
+@pytest.mark.parametrize("call", [fork, compact])
+def test_plans_refuse_layers_on_one_another(lib, call):
+    l, L = lib
+    assert call(l, layers=2, ks=(0, 1024, 64, 64)) == L.WX_ERR_INVALID

@@ -836,7 +836,7 @@ __global__ void __launch_bounds__(kCopyThreads, kCopyResident) kv_copy_kernel(co
 
 int check_pool(const char* what, const void* k, const void* v, int64_t page_stride,
                int64_t tok_stride, int64_t head_stride, int64_t n_heads, int64_t head_dim,
-               int64_t n_pages, int64_t page_size, int dtype) {
+               int64_t n_pages, int64_t page_size, int dtype, bool written) {
   if (dtype != WX_DTYPE_BF16 && dtype != WX_DTYPE_F32)
     return fail(WX_ERR_INVALID, "%s: bad dtype %d", what, dtype);
   if (n_heads < 1 || n_heads > 65535 || head_dim < 1 || n_pages < 1 || page_size < 1 ||
@@ -855,6 +855,12 @@ int check_pool(const char* what, const void* k, const void* v, int64_t page_stri
                 (long long)head_stride);
   if (page_stride < 0 || tok_stride < 0 || head_stride < 0)
     return fail(WX_ERR_INVALID, "%s: negative stride", what);
+  if (written && (rows_overlap(n_pages, page_stride, head_dim) ||
+                  rows_overlap(page_size, tok_stride, head_dim) ||
+                  rows_overlap(n_heads, head_stride, head_dim)))
+    return fail(WX_ERR_INVALID,
+                "%s: the cache is written, but its rows share memory (strides %lld, %lld, %lld)",
+                what, (long long)page_stride, (long long)tok_stride, (long long)head_stride);
   if (!k || !v) return fail(WX_ERR_INVALID, "%s: NULL cache", what);
   return WX_OK;
 }
@@ -922,10 +928,11 @@ static int launch_copies(const char* what, const Pool& p, const PlanSpace& ws,
   return check_launch(what);
 }
 
-static int check_plan(const char* what, int64_t n_layers, int64_t layer_stride, int64_t es,
-                      int64_t n_seqs, int64_t width, const void* ws, int64_t ws_bytes,
-                      int64_t n_pages) {
-  if (n_layers < 1 || n_layers > 32767 || layer_stride < 0 || layer_stride * es % 16)
+static int check_plan(const char* what, int64_t n_layers, int64_t layer_stride,
+                      int64_t head_dim, int64_t es, int64_t n_seqs, int64_t width,
+                      const void* ws, int64_t ws_bytes, int64_t n_pages) {
+  if (n_layers < 1 || n_layers > 32767 || layer_stride < 0 || layer_stride * es % 16 ||
+      rows_overlap(n_layers, layer_stride, head_dim))
     return fail(WX_ERR_INVALID, "%s: bad layers: %lld, stride %lld", what, (long long)n_layers,
                 (long long)layer_stride);
   if (n_seqs < 1 || n_seqs > (1 << 20) || width < 1 || width > 0x7fffffff)
@@ -950,7 +957,7 @@ int wx_kv_append(const void* k, const void* v, int64_t src_seq_stride, int64_t s
                  int dtype, void* stream) {
   using namespace wx;
   WX_TRY(check_pool("kv_append", k_cache, v_cache, page_stride, tok_stride, head_stride, n_heads,
-                    head_dim, n_pages, page_size, dtype));
+                    head_dim, n_pages, page_size, dtype, true));
   if (n_seqs < 0 || n_seqs > 65535 || n_tokens < 0 || n_tokens > 0x7fffffff)
     return fail(WX_ERR_INVALID, "kv_append: bad shape: %lld sequences, %lld tokens",
                 (long long)n_seqs, (long long)n_tokens);
@@ -1015,9 +1022,9 @@ int wx_kv_fork(void* k_cache, void* v_cache, int64_t n_layers, int64_t layer_str
                int32_t* status_out, void* workspace, int64_t workspace_bytes, void* stream) {
   using namespace wx;
   WX_TRY(check_pool("kv_fork", k_cache, v_cache, page_stride, tok_stride, head_stride, n_heads,
-                    head_dim, n_pages, page_size, dtype));
-  WX_TRY(check_plan("kv_fork", n_layers, layer_stride, dtype == WX_DTYPE_BF16 ? 2 : 4, n_seqs,
-                    width, workspace, workspace_bytes, n_pages));
+                    head_dim, n_pages, page_size, dtype, true));
+  WX_TRY(check_plan("kv_fork", n_layers, layer_stride, head_dim, dtype == WX_DTYPE_BF16 ? 2 : 4,
+                    n_seqs, width, workspace, workspace_bytes, n_pages));
   if (!table || !lens || !refs || !table_out || !lens_out || !refs_out || !status_out)
     return fail(WX_ERR_INVALID, "kv_fork: NULL argument");
   if (table == table_out || lens == lens_out || refs == refs_out)
@@ -1064,9 +1071,10 @@ int wx_kv_compact(void* k_cache, void* v_cache, int64_t n_layers, int64_t layer_
                   int64_t workspace_bytes, void* stream) {
   using namespace wx;
   WX_TRY(check_pool("kv_compact", k_cache, v_cache, page_stride, tok_stride, head_stride, n_heads,
-                    head_dim, n_pages, page_size, dtype));
-  WX_TRY(check_plan("kv_compact", n_layers, layer_stride, dtype == WX_DTYPE_BF16 ? 2 : 4, n_seqs,
-                    width, workspace, workspace_bytes, n_pages));
+                    head_dim, n_pages, page_size, dtype, true));
+  WX_TRY(check_plan("kv_compact", n_layers, layer_stride, head_dim,
+                    dtype == WX_DTYPE_BF16 ? 2 : 4, n_seqs, width, workspace, workspace_bytes,
+                    n_pages));
   if (!table || !refs || !table_out || !refs_out || !status_out)
     return fail(WX_ERR_INVALID, "kv_compact: NULL argument");
   if (refs == refs_out)

@@ -70,10 +70,16 @@ inline cudaError_t launch_after(void (*kernel)(KArgs...), dim3 grid, int threads
   return launch(true, kernel, grid, threads, smem, cluster, st, std::forward<Args>(args)...);
 }
 
-// Checks a pool's types, sizes, strides (elements) and alignment.
+// Whether rows of head_dim elements, `stride` apart, lie over one another.
+inline bool rows_overlap(int64_t n, int64_t stride, int64_t head_dim) {
+  return n > 1 && stride < head_dim && stride > -head_dim;
+}
+
+// Checks a pool's types, sizes, strides (elements) and alignment; `written`: and that no
+// two of its rows share memory, which a pool that is only read may do.
 int check_pool(const char* what, const void* k, const void* v, int64_t page_stride,
                int64_t tok_stride, int64_t head_stride, int64_t n_heads, int64_t head_dim,
-               int64_t n_pages, int64_t page_size, int dtype);
+               int64_t n_pages, int64_t page_size, int dtype, bool written);
 
 // WX_DEVERR_PAGE as recorded by the cache's kernels on the current device: OR it
 // into *flags, and clear it when asked.

@@ -1481,7 +1481,7 @@ int wx_paged_attention(const void* q, int64_t q_seq_stride, int64_t q_head_strid
   using namespace wx;
   WX_TRY(check_cut("paged_attention", n_seqs, n_heads, group, head_dim, max_len));
   WX_TRY(check_pool("paged_attention", k_cache, v_cache, page_stride, tok_stride, head_stride,
-                    n_heads, head_dim, n_pages, page_size, dtype));
+                    n_heads, head_dim, n_pages, page_size, dtype, false));
   if (n_seqs == 0) return WX_OK;
   if (!q || !out || !lens || !table || ld_table < 1)
     return fail(WX_ERR_INVALID, "paged_attention: NULL argument or empty page table");
@@ -1491,6 +1491,11 @@ int wx_paged_attention(const void* q, int64_t q_seq_stride, int64_t q_head_strid
   const int es = dtype == WX_DTYPE_BF16 ? 2 : 4;
   if (((uintptr_t)q | (uintptr_t)out) % es)
     return fail(WX_ERR_INVALID, "paged_attention: q or out not aligned to its type");
+  if (rows_overlap(n_seqs, o_seq_stride, head_dim) ||
+      rows_overlap(n_heads, o_head_stride, head_dim) ||
+      rows_overlap(group, o_group_stride, head_dim))
+    return fail(WX_ERR_INVALID, "paged_attention: out's rows share memory (strides %lld, %lld, %lld)",
+                (long long)o_seq_stride, (long long)o_head_stride, (long long)o_group_stride);
   const PagedCut c = paged_cut(n_seqs, n_heads, group, max_len, dtype);
   const int64_t rows = n_seqs * n_heads * group, want = paged_space(rows, c, head_dim);
   if (want && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < want))
