@@ -102,6 +102,20 @@ def test_scores_nan_at_the_first_token(cuda, dtype, offset, rows, vocab):
     assert index[0].tolist() == [7, 0, 1, 2, 3, 4, 5, 6]
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_scores_at_the_least_temperature(cuda, dtype):
+    """As temperature goes to 0 the largest logit takes all."""
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    x = randn(gen, 3, 5003, dtype=dtype)
+    tokens = x.argmax(1)
+    x[torch.arange(3, device="cuda"), tokens] = 8.0     # alone at the top
+    for t in (4.5e-39, 1e-38, 1e-30):
+        lp, entropy, top, index = ops.token_logprobs(x, tokens, top_k=2, temperature=t)
+        assert (lp == 0).all() and (entropy == 0).all()
+        assert (top[:, 0] == 0).all() and torch.equal(index[:, 0].long(), tokens)
+        assert (top[:, 1] < -1e28).all()
+
+
 # ------------------------------------------------------------------ compact
 
 

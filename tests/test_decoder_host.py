@@ -5,7 +5,7 @@ from pathlib import Path
 import pytest
 import torch
 
-from test_decoder_capi import NUL, P, append, at, attend, fork, lib  # noqa: F401
+from test_decoder_capi import NUL, P, append, at, attend, fork, lib, score  # noqa: F401
 from wxb200.kvcache import PagedKVCache
 
 CSRC = Path(__file__).resolve().parents[1] / "whisper-xdna_b200" / "csrc"
@@ -70,3 +70,11 @@ def test_writers_refuse_a_cache_on_itself(lib, call, pages, page, heads, ks):
 def test_plans_refuse_layers_on_one_another(lib, call):
     l, L = lib
     assert call(l, layers=2, ks=(0, 1024, 64, 64)) == L.WX_ERR_INVALID
+
+
+@pytest.mark.parametrize("t", [3e-39, 4.2e-39])
+def test_scores_refuse_a_temperature_past_the_exponents(lib, t):
+    """log2(e) / t is what logits are multiplied by: infinite, it makes every score NaN."""
+    l, L = lib
+    assert score(l, t=t) == L.WX_ERR_INVALID
+    assert "temperature" in L.last_error()

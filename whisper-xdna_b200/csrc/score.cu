@@ -533,7 +533,9 @@ extern "C" int wx_token_logprobs(const void* logits, int dtype, int64_t rows, in
   if (top_k < 0 || top_k > kScoreMaxTop || top_k > vocab)
     return fail(WX_ERR_INVALID, "token_logprobs: top_k %lld not in [0, min(%d, vocabulary)]",
                 (long long)top_k, kScoreMaxTop);
-  if (!(temperature > 0.0f) || !(1.0f / temperature <= FLT_MAX) || !(temperature <= FLT_MAX))
+  // the kernel's factor, log2(e) / temperature, has to be finite too
+  if (!(temperature > 0.0f) || !(1.4426950408889634f * (1.0f / temperature) <= FLT_MAX) ||
+      !(temperature <= FLT_MAX))
     return fail(WX_ERR_INVALID, "token_logprobs: temperature must be positive and finite");
   if (rows == 0) return WX_OK;
   const int es = dtype == WX_DTYPE_BF16 ? 2 : 4;
