@@ -218,3 +218,16 @@ def test_outputs_that_share_memory_are_refused(cuda):
                                         table, refs)):
         with pytest.raises(ValueError):
             call()
+
+
+# ------------------------------------------------------------------ arguments
+
+
+def test_return_lse_without_a_truth_value(cuda):
+    """The caller's own error, and nothing launched."""
+    k, v, table, n, gen = make_cache([9], 8, 2, 64, torch.bfloat16, seed=1)
+    q = randn(gen, 1, 2, 64, dtype=torch.bfloat16)
+    out = torch.full_like(q, 5.0)
+    with pytest.raises(RuntimeError, match="ambiguous"):
+        ops.paged_attention(q, k, v, table, n, out=out, return_lse=torch.zeros(2))
+    assert (out == 5).all()

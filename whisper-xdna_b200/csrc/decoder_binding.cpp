@@ -51,6 +51,11 @@ int64_t integer(PyObject* o) {
   if (v == -1 && PyErr_Occurred()) throw Raised();
   return v;
 }
+bool truth(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw Raised();
+  return v == 1;
+}
 double number(PyObject* o) {
   const double v = PyFloat_AsDouble(o);
   if (v == -1.0 && PyErr_Occurred()) throw Raised();
@@ -200,7 +205,7 @@ PyObject* paged_attention(PyObject* const* a) {
   if (n[0] != table.n || n[q.dim() - 1] != c.hd || q.stride(-1) != 1)
     refuse("q of shape " + sizes(n) + " does not fit " + std::to_string(table.n) +
            " sequences of head_dim " + std::to_string(c.hd) + " (contiguous)");
-  const bool own = a[8] == Py_None, want_lse = PyObject_IsTrue(a[9]) == 1;
+  const bool own = a[8] == Py_None, want_lse = truth(a[9]);
   Tensor out, lse;
   if (!own) {
     out = tensor(a[8], "out");
