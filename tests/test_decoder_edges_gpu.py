@@ -231,3 +231,49 @@ def test_return_lse_without_a_truth_value(cuda):
     with pytest.raises(RuntimeError, match="ambiguous"):
         ops.paged_attention(q, k, v, table, n, out=out, return_lse=torch.zeros(2))
     assert (out == 5).all()
+
+
+# ------------------------------------------------------------------ a captured step
+
+
+def test_cache_step_replayed_from_a_graph(cuda):
+    """A step captured with its new tables copied back is the same step, replay after
+    replay, as one that is called."""
+    page, beams, steps = 4, 3, 9
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    rows = randn(gen, steps + 1, beams, 2, 64, dtype=torch.bfloat16)
+    order = [dev([(b * (t + 1)) % beams for b in range(beams)]) for t in range(steps)]
+    parents, grow, row = dev([0, 1, 2]), dev([1] * beams), rows[0].clone()
+
+    def begin():
+        cache = PagedKVCache(1, 20, page, 2, 64, beams, 12)
+        cache.step(grow=grow)
+        cache.append(0, rows[0], -rows[0])
+        return cache
+
+    def step(cache):
+        cache.step(parents, grow)
+        cache.append(0, row, -row)
+        return cache.attend(0, row)
+
+    plain, want = begin(), []
+    for t in range(steps):
+        parents.copy_(order[t])
+        row.copy_(rows[t + 1])
+        want.append((step(plain).clone(), plain.table.clone(), plain.lens.clone()))
+    cache = begin()
+    held = cache.table, cache.lens, cache.refs
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(cache)
+        for old, new in zip(held, (cache.table, cache.lens, cache.refs)):
+            old.copy_(new)
+    cache.table, cache.lens, cache.refs = held
+    for t in range(steps):
+        parents.copy_(order[t])
+        row.copy_(rows[t + 1])
+        graph.replay()
+        assert torch.equal(out, want[t][0])
+        assert torch.equal(cache.table, want[t][1]) and torch.equal(cache.lens, want[t][2])
+        assert cache.grown.tolist() == [1] * beams

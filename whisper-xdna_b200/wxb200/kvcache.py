@@ -50,7 +50,9 @@ class PagedKVCache:
 
     def step(self, parents=None, grow=None):
         """Sequence i goes on as parents[i] was (-1: it starts empty; None: as
-        itself) with grow[i] more tokens (None: none): see ops.kv_fork."""
+        itself) with grow[i] more tokens (None: none): see ops.kv_fork. The table,
+        lens, refs, grown and status are new tensors: a step captured in a CUDA graph
+        to be replayed ends by copying the first three into those it began with."""
         self.table, self.lens, self.refs, self.grown, self.status = ops.kv_fork(
             self.k, self.v, self.table, self.lens, self.refs, parents=parents, grow=grow)
 
