@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from test_decoder_capi import NUL, P, append, at, attend, fork, lib, score  # noqa: F401
+from wxb200 import _build
 from wxb200.kvcache import PagedKVCache
 
 CSRC = Path(__file__).resolve().parents[1] / "whisper-xdna_b200" / "csrc"
@@ -78,3 +79,26 @@ def test_scores_refuse_a_temperature_past_the_exponents(lib, t):
     l, L = lib
     assert score(l, t=t) == L.WX_ERR_INVALID
     assert "temperature" in L.last_error()
+
+
+def test_binding_is_built_again_for_another_torch(monkeypatch, tmp_path):
+    """It is linked against torch's C++ interface, which no source file's time tells of."""
+    ran = []
+
+    def run(cmd, **kw):
+        ran.append(cmd)
+        (tmp_path / "_decoder.so").write_bytes(b"")
+        return type("Done", (), {"returncode": 0, "stdout": "", "stderr": ""})
+
+    monkeypatch.setattr(_build, "BUILD", tmp_path)
+    monkeypatch.setattr(_build, "BINDING", tmp_path / "_decoder.so")
+    monkeypatch.setattr(_build.subprocess, "run", run)
+    _build.build_binding()
+    _build.build_binding()
+    assert len(ran) == 1
+    monkeypatch.setattr(torch, "__version__", torch.__version__ + "1")
+    _build.build_binding()
+    _build.build_binding()
+    assert len(ran) == 2
+    _build.build_binding(force=True)
+    assert len(ran) == 3

@@ -79,25 +79,30 @@ def build(verbose=False, force=False):
 
 def build_binding(force=False):
     """_decoder.so: csrc/decoder_binding.cpp against torch's headers, linked with
-    libwxb200.so beside it."""
-    src = CSRC / "decoder_binding.cpp"
-    newest = max(src.stat().st_mtime, (ROOT / "include" / "wxb200.h").stat().st_mtime)
-    if not force and BINDING.exists() and BINDING.stat().st_mtime > newest:
-        return
+    libwxb200.so beside it; built again where a source is newer, or the torch or the
+    command is another than it was built with."""
     import torch
     torch_dir = Path(torch.__file__).resolve().parent
     cuda = Path(_nvcc()).resolve().parents[1] if os.path.isabs(_nvcc()) else Path("/usr/local/cuda")
     includes = [torch_dir / "include", torch_dir / "include" / "torch" / "csrc" / "api" / "include",
                 cuda / "include", sysconfig.get_paths()["include"]]
+    src = CSRC / "decoder_binding.cpp"
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++20", "-fPIC", "-shared",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
            *(f"-I{p}" for p in includes), str(src), "-o", str(BINDING),
            f"-L{LIB.parent}", f"-l:{LIB.name}", "-Wl,-rpath,$ORIGIN",
            f"-L{torch_dir / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-lc10",
            "-lc10_cuda"]
+    built_with, made = BUILD / "decoder_binding.txt", " ".join([torch.__version__, *cmd])
+    newest = max(src.stat().st_mtime, (ROOT / "include" / "wxb200.h").stat().st_mtime)
+    if not force and BINDING.exists() and BINDING.stat().st_mtime > newest and \
+            built_with.exists() and built_with.read_text() == made:
+        return
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed on {src.name}:\n{r.stdout}\n{r.stderr}")
+    BUILD.mkdir(exist_ok=True)
+    built_with.write_text(made)
 
 
 if __name__ == "__main__":
