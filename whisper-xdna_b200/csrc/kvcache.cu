@@ -63,8 +63,8 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const AppendArgs a) {
   // a count past the rows given still says where row 0 goes; none is below 0
   const int asked = a.counts ? a.counts[seq] : a.n_tokens;
   const int count = min(max(asked, 0), a.n_tokens);
-  if (asked != count && (threadIdx.x | blockIdx.x | blockIdx.z) == 0) kv_error();
-  const int64_t first = (int64_t)a.lens[seq] - asked;
+  // row 0's position; cut off where all positions are below 0 anyhow
+  const int first = (int)max((int64_t)a.lens[seq] - asked, (int64_t)INT32_MIN);
   const uint32_t per_token = (uint32_t)a.n_heads * a.row_units;
   const uint32_t total = (uint32_t)count * per_token;
   const char* src = a.src[blockIdx.z] + seq * a.s_seq;
@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const AppendArgs a) {
       const int h = a.by_row(r), u = r - h * a.row_units;
       x[j] = *reinterpret_cast<const U*>(src + t * a.s_tok + h * a.s_head +
                                          u * (int64_t)sizeof(U));
-      const int pos = (int)max(first + t, (int64_t)-1);
+      const int pos = first + t;
       const int slot = a.by_page(max(pos, 0));
       const int page = pos >= 0 && slot < a.width ? row[slot] : -1;
       if (page < 0 || page >= a.n_pages)
@@ -96,6 +96,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const AppendArgs a) {
     for (int j = 0; j < kAppendUnroll; j++)
       if (to[j] >= 0) *reinterpret_cast<U*>(dst + to[j]) = x[j];
   }
+  if (asked != count && (threadIdx.x | blockIdx.x | blockIdx.z) == 0) kv_error();
 }
 
 // ---------------------------------------------------------------- page plans
