@@ -31,7 +31,7 @@ extern "C" {
 
 /* bits of the device error word (wx_device_error) */
 #define WX_DEVERR_TIMEOUT 1 /* a bounded wait inside a kernel gave up */
-#define WX_DEVERR_PAGE 2    /* a cache kernel met a page, length or parent out of range */
+#define WX_DEVERR_PAGE 2    /* a cache kernel met a page, length, count or parent out of range */
 
 /* element types */
 #define WX_DTYPE_BF16 0
@@ -213,8 +213,8 @@ int wx_attention(const void* q, const void* k, const void* v, void* o, int64_t B
  * are device memory, and no call reads them on the host. Rows of a pool may share
  * memory (strides of 0) where it is only read, by wx_paged_attention.
  *
- * A page, length or parent out of range in those arrays is left out (its tokens
- * are not written, or not attended to) and recorded as WX_DEVERR_PAGE, which
+ * A page, length, count or parent out of range in those arrays is left out (its
+ * tokens are not written, or not attended to) and recorded as WX_DEVERR_PAGE, which
  * wx_device_error reports and clears. dtype is WX_DTYPE_BF16 or WX_DTYPE_F32. */
 
 /* Writes new tokens: row t < counts[i] (all n_tokens if counts is NULL) of
@@ -312,7 +312,13 @@ int wx_paged_attention(const void* q, int64_t q_seq_stride, int64_t q_head_strid
  * A token below 0 is none and has logprob 0; one at or past vocab has -inf.
  * Logits of -inf are masked tokens (probability 0). A row that is all -inf has
  * logprob and top_logprob -inf and entropy 0; one that holds NaN or +inf has NaN
- * scores, and its order puts NaN above +inf. top_k <= 32 and <= vocab.
+ * scores, and its order puts NaN above +inf. top_k <= 32 and <= vocab; temperature
+ * is finite and at least 4.3e-39 (log2(e) / temperature is finite).
+ * Exponents and sums are fp32's, the sums in a fixed order. With e(z) = 2^-21 (6 +
+ * |z - max z|) a term e^(z - max z) is within e(z) of itself; with b(z) = e(z) +
+ * (vocab / 256 + 64) 2^-24, a log probability is off by its own e(z) and the mean of b
+ * under softmax(z) at most, the entropy by the mean of (12 + 2 |z - max z|) b, besides
+ * their last bits.
  * logprob (with tokens) and entropy may be NULL; so may the top outputs if
  * top_k is 0. */
 int wx_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ld,

@@ -1386,7 +1386,11 @@ static cudaError_t launch_paged(PagedArgs a, const PagedCut& c, int smem, cudaSt
   if (c.warps == 1) grid = dim3((unsigned)((n_items + kPagedWarps - 1) / kPagedWarps));
   // Placed while the kernel before it ends, a wave of CTAs lands on the SMs that are free
   // first, unevenly: 33.5 us became 36.8 (64 items of 4096 keys). A call of a few us
-  // gains the one that a launch costs: one clip's frames, 7.1 us, take 6.7.
+  // gains half of what a launch costs. Early and not, bf16, heads of 64, us: 100 items of
+  // a table of 448 keys (45 K) 5.5 and 6.0, one clip's frames (30 K) 6.0 and 6.4; 320 of
+  // 224 (72 K) 7.3 and 7.0, of 448 (143 K) 11.2 and 10.7, of 1500 (481 K) 24.5 and 24.0.
+  // Calls of several waves would gain that half again, which this rule leaves: 6400 items
+  // of 224 (1.4 M) 59.3 and 60.0.
   const bool early = n_items * a.max_len <= kEarlyKeys;
   return launch(early, kernel, grid, kPagedThreads, smem, c.chunk == 0 ? a.splits : 1, st, a);
 }

@@ -330,7 +330,9 @@ def kv_fork(k_cache, v_cache, table, lens, refs, parents=None, grow=None):
 
     Returns new int32 tensors (table, lens, refs, grown, status): lens counts the
     tokens granted (grown), status is (pages left free, pages short). A sequence
-    whose pages the pool does not hold is not grown."""
+    whose pages the pool does not hold is not grown. The five share one allocation
+    (so do the outputs of the other calls here): one that is kept keeps them all, a
+    clone does not."""
     return _decoder.kv_fork(k_cache, v_cache, table, lens, refs, parents, grow)
 
 
