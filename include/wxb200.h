@@ -251,7 +251,8 @@ int64_t wx_kv_workspace(int64_t n_seqs, int64_t n_pages);
  * table_out (n_seqs x width, -1 past the last page), lens_out (with the tokens
  * granted), refs_out, grown_out (tokens granted; may be NULL) and status_out[2]
  * (pages left free, pages short) are written; none of them may be an input. The
- * k and v pools are written only in pages that were free. */
+ * table has 2^30 entries at most, a row 2^30 tokens. The k and v pools are written
+ * only in pages that were free. */
 int wx_kv_fork(void* k_cache, void* v_cache, int64_t n_layers, int64_t layer_stride,
                int64_t page_stride, int64_t tok_stride, int64_t head_stride, int64_t n_heads,
                int64_t head_dim, int64_t n_pages, int64_t page_size, int dtype,

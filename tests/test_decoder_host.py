@@ -102,3 +102,12 @@ def test_binding_is_built_again_for_another_torch(monkeypatch, tmp_path):
     assert len(ran) == 2
     _build.build_binding(force=True)
     assert len(ran) == 3
+
+
+@pytest.mark.parametrize("n,width", [(1 << 20, 1 << 11), (1 << 20, (1 << 10) + 1)])
+def test_fork_refuses_a_table_that_its_sums_do_not_hold(lib, n, width):
+    """The pages asked for are summed in 32 bits: past them a sum below 0 would pass for
+    one that the pool holds."""
+    l, L = lib
+    assert fork(l, n=n, width=width, page=1, space=1 << 40) == L.WX_ERR_INVALID
+    assert "page table" in L.last_error()

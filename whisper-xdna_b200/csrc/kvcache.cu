@@ -1032,6 +1032,10 @@ int wx_kv_fork(void* k_cache, void* v_cache, int64_t n_layers, int64_t layer_str
     return fail(WX_ERR_INVALID, "kv_fork: the new page table cannot be written over the old one");
   if (n_heads * head_dim * page_size > 0x7fffffff || width * page_size > (1 << 30))
     return fail(WX_ERR_INVALID, "kv_fork: a page of over 2^31 - 1 elements or a row of over 2^30 tokens");
+  // the running sum of pages asked for is in 32 bits, a row's width and a copy each at most
+  if (n_seqs * width > (1 << 30))
+    return fail(WX_ERR_INVALID, "kv_fork: a page table of over 2^30 entries: %lld x %lld",
+                (long long)n_seqs, (long long)width);
   ForkArgs a = {};
   a.table = table;
   a.lens = lens;
